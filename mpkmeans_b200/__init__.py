@@ -78,6 +78,13 @@ class mpkStats(ctypes.Structure):
                 ("t_update_ms", ctypes.c_double)]
 
 
+class mpkRouteParams(ctypes.Structure):
+    """mpkRouteParams (include/mpkexperts.h)."""
+    _fields_ = [("experts", ctypes.c_int), ("top_k", ctypes.c_int), ("score", ctypes.c_int), ("groups", ctypes.c_int),
+                ("top_groups", ctypes.c_int), ("group_score", ctypes.c_int), ("renormalize", ctypes.c_int),
+                ("scale", ctypes.c_float)]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _LL = ctypes.c_longlong
@@ -86,9 +93,10 @@ _D = ctypes.c_double
 _I64 = ctypes.c_int64
 _PARAMS = ctypes.POINTER(mpkParams)
 _STATS = ctypes.POINTER(mpkStats)
+_ROUTE = ctypes.POINTER(mpkRouteParams)
 
-# name -> (restype, argtypes).  Every symbol include/mpkmeans.h and
-# include/mpemu.h declare is listed here; tests check the library exports all.
+# name -> (restype, argtypes).  Every symbol include/mpkmeans.h, include/mpemu.h
+# and include/mpkexperts.h declare is listed here; tests check the library exports all.
 SIGNATURES = {
     "mpkParamsInit": (None, [_PARAMS]),
     "mpkEpsilon": (_D, [_I, _I]),
@@ -201,6 +209,17 @@ SIGNATURES = {
     "mpkDebugAssignPair": (_I, [_P, _I]),
     "mpkDebugOverlapRefine": (_I, [_P, _I]),
     "mpkDebugClearStatus": (_I, [_P]),
+    # include/mpkexperts.h
+    "mpkRouteParamsInit": (None, [_ROUTE]),
+    "mpkRoute": (_I, [_P, _ROUTE, _P, _I, _LL, _LL, _P, _P, _P]),
+    "mpkRouteGrad": (_I, [_P, _ROUTE, _P, _I, _LL, _LL, _P, _P, _P, _LL]),
+    "mpkExpertPlanBytes": (ctypes.c_size_t, [_LL, _I, _I]),
+    "mpkExpertPlan": (_I, [_P, _P, _LL, _I, _I, _P, _P, _P, _P, ctypes.c_size_t]),
+    "mpkExpertGemm": (_I, [_P, _I, _P, _LL, _P, _LL, _LL, _P, _P, _I, _LL, _I, _I, _I, _P, _LL]),
+    "mpkExpertGemmGradX": (_I, [_P, _I, _P, _LL, _P, _LL, _LL, _P, _LL, _I, _I, _I, _P, _LL]),
+    "mpkExpertGemmGradW": (_I, [_P, _I, _P, _LL, _P, _LL, _P, _P, _I, _LL, _I, _I, _I, _P, _LL, _LL]),
+    "mpkExpertCombine": (_I, [_P, _I, _P, _LL, _P, _P, _LL, _I, _I, _P, _LL]),
+    "mpkExpertCombineGrad": (_I, [_P, _I, _P, _LL, _P, _LL, _P, _P, _P, _LL, _I, _I, _P, _LL, _P]),
 }
 
 _lib = None
@@ -484,3 +503,272 @@ class Engine:
 
     def __exit__(self, *a):
         self.close()
+
+
+# --------------------------------------------- rows routed to experts (mpkexperts.h) --
+
+_SCORES = {"softmax": 0, "sigmoid": 1}
+_GROUP_SCORES = {"max": 0, "top2": 1}
+_type_codes = None
+
+
+def _types() -> dict:
+    """torch dtype -> mpkType."""
+    global _type_codes
+    if _type_codes is None:
+        import torch
+        _type_codes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    return _type_codes
+
+
+def _matrix(name: str, t, dtypes=None, rows: int | None = None, cols: int | None = None) -> tuple[int, int]:
+    """(address, row stride) of a 2-D CUDA tensor whose rows are contiguous."""
+    if t.dim() != 2 or (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[1] != cols):
+        want = f"{'n' if rows is None else rows} x {'m' if cols is None else cols}"
+        raise ValueError(f"{name}: expected a {want} tensor, got {tuple(t.shape)}")
+    if dtypes is not None and t.dtype not in dtypes:
+        raise ValueError(f"{name}: dtype {t.dtype} is not one of {', '.join(map(str, dtypes))}")
+    if not t.is_cuda:
+        raise ValueError(f"{name}: expected a CUDA tensor")
+    n, c = t.shape
+    ld, inner = t.stride()
+    if c > 1 and inner != 1:
+        raise ValueError(f"{name}: rows must be contiguous")
+    if n <= 1:
+        ld = c
+    elif ld < c:
+        raise ValueError(f"{name}: rows overlap (row stride {ld} under {c} columns)")
+    return t.data_ptr(), ld
+
+
+def _matrices(name: str, t, dtype, shape: tuple) -> tuple[int, int, int]:
+    """(address, row stride, matrix stride) of experts x rows x columns."""
+    if t.dim() != 3 or any(a is not None and a != b for a, b in zip(shape, t.shape)):
+        raise ValueError(f"{name}: expected experts x width x k = {shape}, got {tuple(t.shape)}")
+    if t.dtype != dtype:
+        raise ValueError(f"{name}: dtype {t.dtype}, expected {dtype}")
+    if not t.is_cuda:
+        raise ValueError(f"{name}: expected a CUDA tensor")
+    e, r, c = t.shape
+    se, sr, sc = t.stride()
+    if c > 1 and sc != 1:
+        raise ValueError(f"{name}: rows must be contiguous")
+    if r <= 1:
+        sr = c
+    elif sr < c:
+        raise ValueError(f"{name}: rows overlap")
+    if e <= 1:
+        se = (r - 1) * sr + c
+    elif se < (r - 1) * sr + c:
+        raise ValueError(f"{name}: matrices overlap")
+    return t.data_ptr(), sr, se
+
+
+def _int32(name: str, t, shape: tuple) -> int:
+    import torch
+    if tuple(t.shape) != shape or t.dtype != torch.int32:
+        raise ValueError(f"{name}: expected int32 of shape {shape}, got {t.dtype} of {tuple(t.shape)}")
+    return _ptr(t)
+
+
+def _fp32(name: str, t, shape: tuple) -> int:
+    import torch
+    if tuple(t.shape) != shape or t.dtype != torch.float32:
+        raise ValueError(f"{name}: expected float32 of shape {shape}, got {t.dtype} of {tuple(t.shape)}")
+    return _ptr(t)
+
+
+def _run(fn_name: str, tensors: tuple, *args) -> None:
+    """Call fn_name(stream, *args) on the tensors' device (all on one) and torch's
+    current stream there, the stream that outputs and scratch are allocated on."""
+    import torch
+    device = tensors[0].device
+    for t in tensors:
+        if t.device != device:
+            raise ValueError(f"{fn_name}: tensors on {device} and {t.device}")
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if device.index == torch.cuda.current_device():
+        status = getattr(lib(), fn_name)(stream, *args)
+    else:
+        with torch.cuda.device(device):
+            status = getattr(lib(), fn_name)(stream, *args)
+    check(fn_name, status)
+
+
+def _route_params(experts, top_k, score, groups, top_groups, group_score, renormalize, scale) -> mpkRouteParams:
+    if score not in _SCORES:
+        raise ValueError(f"score: {score!r} is not one of {', '.join(_SCORES)}")
+    if group_score not in _GROUP_SCORES:
+        raise ValueError(f"group_score: {group_score!r} is not one of {', '.join(_GROUP_SCORES)}")
+    return mpkRouteParams(experts, top_k, _SCORES[score], groups, top_groups, _GROUP_SCORES[group_score],
+                          int(bool(renormalize)), scale)
+
+
+def route(logits, top_k: int, *, score: str = "softmax", bias=None, groups: int = 1, top_groups: int = 1,
+          group_score: str = "max", renormalize: bool = True, scale: float = 1.0):
+    """Choose top_k experts for every token (mpkRoute).  logits: n x experts, FP32,
+    FP16 or BF16; bias: one FP32 value an expert, added to the scores for the
+    choice only.  Returns (ids, weights), n x top_k int32 and FP32, best first;
+    id -1 with weight 0 where no expert is left (logits or bias of -inf mask)."""
+    import torch
+    address, ld = _matrix("logits", logits, _types())
+    n, experts = logits.shape
+    params = _route_params(experts, top_k, score, groups, top_groups, group_score, renormalize, scale)
+    used = (logits,) if bias is None else (logits, bias)
+    pbias = None if bias is None else _fp32("bias", bias, (experts,))
+    ids = torch.empty((n, max(top_k, 0)), dtype=torch.int32, device=logits.device)
+    weights = torch.empty((n, max(top_k, 0)), dtype=torch.float32, device=logits.device)
+    _run("mpkRoute", used, ctypes.byref(params), address, _types()[logits.dtype], n, ld, pbias, ids.data_ptr(),
+         weights.data_ptr())
+    return ids, weights
+
+
+def route_grad(grad_weights, logits, ids, *, score: str = "softmax", renormalize: bool = True, scale: float = 1.0,
+               out=None):
+    """Gradient of route's weights with respect to its logits (mpkRouteGrad), of the
+    logits' type; the choice (ids, as route returned them) is a constant."""
+    import torch
+    address, ld = _matrix("logits", logits, _types())
+    n, experts = logits.shape
+    if ids.dim() != 2:
+        raise ValueError(f"ids: expected n x top_k, got {tuple(ids.shape)}")
+    top_k = ids.shape[1]
+    params = _route_params(experts, top_k, score, 1, 1, "max", renormalize, scale)
+    if out is None:
+        out = torch.empty((n, experts), dtype=logits.dtype, device=logits.device)
+    address_out, ldg = _matrix("out", out, (logits.dtype,), n, experts)
+    _run("mpkRouteGrad", (logits, ids, grad_weights, out), ctypes.byref(params), address,
+         _types()[logits.dtype], n, ld, _int32("ids", ids, (n, top_k)),
+         _fp32("grad_weights", grad_weights, (n, top_k)), address_out, ldg)
+    return out
+
+
+class ExpertPlan:
+    """The routed rows sorted by expert: ``offsets`` (experts + 1), ``order`` (n * top_k:
+    the entry t * top_k + s of every sorted row, -1 behind the last) and ``pos``
+    (n x top_k: the sorted row of every entry, -1 where dropped), all int32."""
+
+    __slots__ = ("offsets", "order", "pos", "n", "top_k", "rows", "experts")
+
+    def __init__(self, offsets, order, pos):
+        if pos.dim() != 2 or offsets.dim() != 1 or offsets.shape[0] < 2:
+            raise ValueError(f"plan: expected offsets of experts + 1 and pos of n x top_k, got "
+                             f"{tuple(offsets.shape)} and {tuple(pos.shape)}")
+        self.n, self.top_k = pos.shape
+        self.rows = self.n * self.top_k
+        self.experts = offsets.shape[0] - 1
+        _int32("offsets", offsets, (self.experts + 1,))
+        _int32("order", order, (self.rows,))
+        _int32("pos", pos, (self.n, self.top_k))
+        self.offsets, self.order, self.pos = offsets, order, pos
+
+
+def expert_plan(ids, experts: int) -> ExpertPlan:
+    """Sort the entries of ids (n x top_k int32) by expert, stably (mpkExpertPlan);
+    ids outside [0, experts) are dropped."""
+    import torch
+    if ids.dim() != 2:
+        raise ValueError(f"ids: expected n x top_k, got {tuple(ids.shape)}")
+    n, top_k = ids.shape
+    address = _int32("ids", ids, (n, top_k))
+    need = int(lib().mpkExpertPlanBytes(n, top_k, experts))
+    buf = torch.empty(max(experts, 0) + 1 + 2 * n * top_k, dtype=torch.int32, device=ids.device)
+    offsets, order, pos = buf.split([max(experts, 0) + 1, n * top_k, n * top_k])
+    work = torch.empty(need, dtype=torch.uint8, device=ids.device) if need else None
+    _run("mpkExpertPlan", (ids,), address, n, top_k, experts, offsets.data_ptr(), order.data_ptr(),
+         pos.data_ptr(), None if work is None else work.data_ptr(), need)
+    return ExpertPlan(offsets, order, pos.view(n, top_k))
+
+
+def expert_gemm(x, w, plan: ExpertPlan, *, gather: bool = True, out=None):
+    """Every routed row times its expert's matrix (mpkExpertGemm): out[r] = w[e] x[r].
+    w: experts x width x k, FP16 or BF16.  x: n x k token rows (gather) or n * top_k
+    rows already sorted.  Returns n * top_k x width, rows without an expert zero."""
+    import torch
+    half = (torch.float16, torch.bfloat16)
+    address, ldx = _matrix("x", x, half, plan.n if gather else plan.rows)
+    pw, ldw, sw = _matrices("w", w, x.dtype, (plan.experts, None, x.shape[1]))
+    width, k = w.shape[1], w.shape[2]
+    if out is None:
+        out = torch.empty((plan.rows, width), dtype=x.dtype, device=x.device)
+    po, ldo = _matrix("out", out, (x.dtype,), plan.rows, width)
+    _run("mpkExpertGemm", (x, w, plan.offsets, plan.order, out), _types()[x.dtype], address, ldx, pw, ldw, sw,
+         plan.offsets.data_ptr(), plan.order.data_ptr() if gather else None, plan.top_k, plan.rows, plan.experts,
+         width, k, po, ldo)
+    return out
+
+
+def expert_gemm_grad_x(grad, w, plan: ExpertPlan, *, out=None):
+    """Gradient of expert_gemm for its sorted rows (mpkExpertGemmGradX): out[r] = w[e]^T
+    grad[r], n * top_k x k.  For gathered tokens, expert_combine(out, plan) adds a
+    token's rows up.  Also the product for weights stored experts x k x width."""
+    import torch
+    half = (torch.float16, torch.bfloat16)
+    address, ldg = _matrix("grad", grad, half, plan.rows)
+    pw, ldw, sw = _matrices("w", w, grad.dtype, (plan.experts, grad.shape[1], None))
+    width, k = w.shape[1], w.shape[2]
+    if out is None:
+        out = torch.empty((plan.rows, k), dtype=grad.dtype, device=grad.device)
+    po, ldo = _matrix("out", out, (grad.dtype,), plan.rows, k)
+    _run("mpkExpertGemmGradX", (grad, w, plan.offsets, out), _types()[grad.dtype], address, ldg, pw, ldw, sw,
+         plan.offsets.data_ptr(), plan.rows, plan.experts, width, k, po, ldo)
+    return out
+
+
+def expert_gemm_grad_w(grad, x, plan: ExpertPlan, *, gather: bool = True, out=None):
+    """Gradient of expert_gemm for its weights (mpkExpertGemmGradW): out[e] = sum over
+    the expert's rows of grad[r] x[r]^T, experts x width x k; zero without rows."""
+    import torch
+    half = (torch.float16, torch.bfloat16)
+    address, ldx = _matrix("x", x, half, plan.n if gather else plan.rows)
+    pg, ldg = _matrix("grad", grad, (x.dtype,), plan.rows)
+    width, k = grad.shape[1], x.shape[1]
+    if out is None:
+        out = torch.empty((plan.experts, width, k), dtype=x.dtype, device=x.device)
+    po, ldo, so = _matrices("out", out, x.dtype, (plan.experts, width, k))
+    _run("mpkExpertGemmGradW", (grad, x, plan.offsets, plan.order, out), _types()[x.dtype], pg, ldg, address,
+         ldx, plan.offsets.data_ptr(), plan.order.data_ptr() if gather else None, plan.top_k, plan.rows, plan.experts,
+         width, k, po, ldo, so)
+    return out
+
+
+def expert_combine(y, plan: ExpertPlan, weights=None, *, out=None):
+    """Back to token order (mpkExpertCombine): out[t] = sum over slots of weights[t, s] *
+    y[pos[t, s]]; weights None: 1.  y: n * top_k x width, FP32, FP16 or BF16."""
+    import torch
+    address, ldy = _matrix("y", y, _types(), plan.rows)
+    width = y.shape[1]
+    if out is None:
+        out = torch.empty((plan.n, width), dtype=y.dtype, device=y.device)
+    po, ldo = _matrix("out", out, (y.dtype,), plan.n, width)
+    used = (y, plan.pos, out) if weights is None else (y, plan.pos, out, weights)
+    pweights = None if weights is None else _fp32("weights", weights, (plan.n, plan.top_k))
+    _run("mpkExpertCombine", used, _types()[y.dtype], address, ldy, plan.pos.data_ptr(), pweights, plan.n,
+         plan.top_k, width, po, ldo)
+    return out
+
+
+def expert_combine_grad(grad, y, plan: ExpertPlan, weights=None, *, out=None):
+    """Gradients of expert_combine (mpkExpertCombineGrad) from grad (n x width): (for y,
+    n * top_k x width with zero rows behind the last; for weights, n x top_k FP32).
+    y None: only the first, the other is None."""
+    import torch
+    address, ldgo = _matrix("grad", grad, _types(), plan.n)
+    width = grad.shape[1]
+    if out is None:
+        out = torch.empty((plan.rows, width), dtype=grad.dtype, device=grad.device)
+    po, ldo = _matrix("out", out, (grad.dtype,), plan.rows, width)
+    used = [grad, plan.pos, plan.offsets, out]
+    py, ldy, grad_weights, pgw, pweights = None, 0, None, None, None
+    if y is not None:
+        py, ldy = _matrix("y", y, (grad.dtype,), plan.rows, width)
+        grad_weights = torch.empty((plan.n, plan.top_k), dtype=torch.float32, device=grad.device)
+        pgw = grad_weights.data_ptr()
+        used.append(y)
+    if weights is not None:
+        pweights = _fp32("weights", weights, (plan.n, plan.top_k))
+        used.append(weights)
+    _run("mpkExpertCombineGrad", tuple(used), _types()[grad.dtype], address, ldgo, py, ldy,
+         plan.pos.data_ptr(), plan.offsets.data_ptr() + 4 * plan.experts, pweights, plan.n, plan.top_k, width, po, ldo,
+         pgw)
+    return out, grad_weights

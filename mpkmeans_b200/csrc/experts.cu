@@ -1,0 +1,454 @@
+/* experts.cu -- the experts' products and the combination of their rows: C ABI
+ * (include/mpkexperts.h), the kernel for layouts the tensor-core kernel
+ * (experts_tc.cu) does not take, and the two combine kernels.
+ */
+#include "experts.cuh"
+#include "mpkexperts.h"
+
+namespace mpk {
+namespace {
+
+constexpr unsigned FULL = 0xffffffffu;
+
+template <typename T>
+__device__ __forceinline__ float to_f(T v);
+template <>
+__device__ __forceinline__ float to_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+template <typename T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+/* ------------------------------------------------- products, any layout ---- */
+
+constexpr int GT = 64;                       /* output tile: 64 rows x 64 columns */
+constexpr int GC = 16;                       /* contraction step */
+constexpr int kAnyThreads = 256;
+
+/* Token row of sorted row r; -1 (read as zeros) where the plan names none. */
+__device__ __forceinline__ long long x_row(const ExpertArgs& a, long long r) {
+    if (!a.order) return r;
+    const int entry = a.order[r];
+    return (unsigned)entry < (unsigned long long)a.m ? entry / a.top_k : -1;
+}
+
+/* One 64 x 64 tile of one expert's output a block, operands staged in shared
+ * memory 16 deep, 4 x 4 sums a thread.  FWD and GRADX: blockIdx.x counts the row
+ * tiles of all experts (their number T is known on the device only; with D rows
+ * that no expert owns, T <= (m - D) / 64 + 63 experts / 64, so m / 64 + experts + 1
+ * blocks leave at least D / 64 past T, which set those rows to zero); GRADW: blockIdx.x = expert * column tiles + tile. */
+template <typename T, int MODE>
+__global__ void __launch_bounds__(kAnyThreads) k_experts_any(const ExpertArgs a) {
+    __shared__ float sa[GC][GT + 1], sb[GC][GT + 1];
+    __shared__ int where[2];
+    const int F = MODE == EXP_FWD ? a.width : a.k;
+    const int f0 = blockIdx.y * GT;
+    const int m = (int)a.m;
+    int e, tile;
+    if (MODE == EXP_GRADW) {
+        const int tiles = (a.width + GT - 1) / GT;
+        e = blockIdx.x / tiles;
+        tile = blockIdx.x - e * tiles;
+    } else {
+        if (threadIdx.x < 32) {              /* the expert whose row tiles hold tile blockIdx.x */
+            const int lane = threadIdx.x;
+            int run = 0, fe = -1, ft = 0;
+            for (int e0 = 0; e0 < a.experts && fe < 0; e0 += 32) {
+                const int q = e0 + lane;
+                const int t = q < a.experts
+                    ? (max(expert_start(a.offsets, q + 1, m) - expert_start(a.offsets, q, m), 0) + GT - 1) / GT : 0;
+                int incl = t;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int u = __shfl_up_sync(FULL, incl, o);
+                    if (lane >= o) incl += u;
+                }
+                const unsigned hit = __ballot_sync(FULL, run + incl > (int)blockIdx.x);
+                if (hit) {
+                    const int l = __ffs(hit) - 1;
+                    fe = e0 + l;
+                    ft = (int)blockIdx.x - run - __shfl_sync(FULL, incl - t, l);
+                }
+                run += __shfl_sync(FULL, incl, 31);
+            }
+            if (lane == 0) { where[0] = fe; where[1] = fe < 0 ? (int)blockIdx.x - run : ft; }
+        }
+        __syncthreads();
+        e = where[0];
+        tile = where[1];
+    }
+    T* out = static_cast<T*>(a.out);
+    if (MODE != EXP_GRADW && e < 0) {
+        const long long r0 = expert_start(a.offsets, a.experts, m) + (long long)tile * GT;
+        for (int i = threadIdx.x; i < GT * GT; i += kAnyThreads) {
+            const long long r = r0 + i / GT;
+            const int f = f0 + i % GT;
+            if (r < m && f < F) out[r * a.ldo + f] = from_f<T>(0.f);
+        }
+        return;
+    }
+    const int r0 = expert_start(a.offsets, e, m), r1 = expert_start(a.offsets, e + 1, m);
+    const int j0 = tile * GT;                                          /* first output row inside the expert */
+    const int J = MODE == EXP_GRADW ? a.width : r1 - r0;
+    const int C = MODE == EXP_FWD ? a.k : MODE == EXP_GRADX ? a.width : max(r1 - r0, 0);
+    const T* x = static_cast<const T*>(a.x);
+    const T* gy = static_cast<const T*>(a.gy);
+    const T* w = static_cast<const T*>(a.w) + (long long)e * a.stride_w;
+    float acc[4][4] = {};
+    const int tf = threadIdx.x & 15, tj = threadIdx.x >> 4;
+    for (int c0 = 0; c0 < C; c0 += GC) {
+        for (int i = threadIdx.x; i < GC * GT; i += kAnyThreads) {
+            /* neighbouring threads read along the operand's contiguous dimension */
+            const bool a_c = MODE == EXP_FWD, b_c = MODE != EXP_GRADW;
+            {
+                const int c = a_c ? i % GC : i / GT, f = a_c ? i / GC : i % GT;
+                float v = 0.f;
+                if (c0 + c < C && f0 + f < F) {
+                    if (MODE == EXP_FWD) v = to_f(w[(long long)(f0 + f) * a.ldw + c0 + c]);
+                    else if (MODE == EXP_GRADX) v = to_f(w[(long long)(c0 + c) * a.ldw + f0 + f]);
+                    else {
+                        const long long q = x_row(a, r0 + c0 + c);
+                        if (q >= 0) v = to_f(x[q * a.ldx + f0 + f]);
+                    }
+                }
+                sa[c][f] = v;
+            }
+            {
+                const int c = b_c ? i % GC : i / GT, j = b_c ? i / GC : i % GT;
+                float v = 0.f;
+                if (c0 + c < C && j0 + j < J) {
+                    if (MODE == EXP_FWD) {
+                        const long long q = x_row(a, r0 + j0 + j);
+                        if (q >= 0) v = to_f(x[q * a.ldx + c0 + c]);
+                    } else if (MODE == EXP_GRADX) {
+                        v = to_f(gy[(long long)(r0 + j0 + j) * a.ldgy + c0 + c]);
+                    } else {
+                        v = to_f(gy[(long long)(r0 + c0 + c) * a.ldgy + j0 + j]);
+                    }
+                }
+                sb[c][j] = v;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < GC; ++c) {
+            float va[4], vb[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { va[i] = sa[c][tf + 16 * i]; vb[i] = sb[c][tj + 16 * i]; }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) acc[i][q] = fmaf(va[q], vb[i], acc[i][q]);
+        }
+        __syncthreads();
+    }
+    T* base = MODE == EXP_GRADW ? out + (long long)e * a.stride_o : out + (long long)r0 * a.ldo;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int j = j0 + tj + 16 * i, f = f0 + tf + 16 * q;
+            if (j < J && f < F) base[(long long)j * a.ldo + f] = from_f<T>(acc[i][q]);
+        }
+}
+
+template <typename T>
+cudaError_t launch_any(const ExpertArgs& a, cudaStream_t s) {
+    const int F = a.mode == EXP_FWD ? a.width : a.k;
+    const unsigned ft = (unsigned)((F + GT - 1) / GT);
+    if (a.mode == EXP_GRADW) {
+        const dim3 g((unsigned)a.experts * (unsigned)((a.width + GT - 1) / GT), ft);
+        k_experts_any<T, EXP_GRADW><<<g, kAnyThreads, 0, s>>>(a);
+    } else {
+        const dim3 g((unsigned)(a.m / GT + a.experts + 1), ft);
+        if (a.mode == EXP_FWD) k_experts_any<T, EXP_FWD><<<g, kAnyThreads, 0, s>>>(a);
+        else k_experts_any<T, EXP_GRADX><<<g, kAnyThreads, 0, s>>>(a);
+    }
+    return cudaGetLastError();
+}
+
+/* --------------------------------------------------------------- combine ---- */
+
+/* V consecutive elements of a row, as floats. */
+template <typename T, int V>
+struct Pack {
+    __device__ static __forceinline__ void load(const T* p, float (&f)[V]) {
+        if constexpr (V == 1) {
+            f[0] = to_f(*p);
+        } else {
+            const uint4 u = *reinterpret_cast<const uint4*>(p);
+            const T* t = reinterpret_cast<const T*>(&u);
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[i] = to_f(t[i]);
+        }
+    }
+    __device__ static __forceinline__ void store(T* p, const float (&f)[V]) {
+        if constexpr (V == 1) {
+            *p = from_f<T>(f[0]);
+        } else {
+            uint4 u;
+            T* t = reinterpret_cast<T*>(&u);
+#pragma unroll
+            for (int i = 0; i < V; ++i) t[i] = from_f<T>(f[i]);
+            *reinterpret_cast<uint4*>(p) = u;
+        }
+    }
+};
+
+constexpr int kCombineThreads = 256;
+
+/* One thread a 16-byte piece (V elements) of one token's output row: the slots'
+ * rows are read once, added in slot order in FP32, written once. */
+template <typename T, int V>
+__global__ void __launch_bounds__(kCombineThreads)
+k_combine(const T* __restrict__ y, long long ldy, const int* __restrict__ pos, const float* __restrict__ weights,
+          long long n, int top_k, int width, T* __restrict__ out, long long ldo) {
+    const int pieces = (width + V - 1) / V;
+    const long long m = n * top_k, total = n * pieces, step = (long long)gridDim.x * kCombineThreads;
+    for (long long i = (long long)blockIdx.x * kCombineThreads + threadIdx.x; i < total; i += step) {
+        const long long t = i / pieces;
+        const int c = (int)(i - t * pieces) * V;
+        float acc[V] = {};
+        for (int s0 = 0; s0 < top_k; s0 += 8) {
+            float f[8][V], wt[8];
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                const long long q = t * top_k + s0 + s;
+                const long long p = s0 + s < top_k ? pos[q] : -1;
+                wt[s] = 0.f;
+                if (p >= 0 && p < m) {
+                    wt[s] = weights ? weights[q] : 1.f;
+                    Pack<T, V>::load(y + p * ldy + c, f[s]);
+                } else {
+#pragma unroll
+                    for (int u = 0; u < V; ++u) f[s][u] = 0.f;
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < 8; ++s)
+#pragma unroll
+                for (int u = 0; u < V; ++u) acc[u] = fmaf(wt[s], f[s][u], acc[u]);
+        }
+        Pack<T, V>::store(out + t * ldo + c, acc);
+    }
+}
+
+/* One block a token (grid-stride): the token's gradient row is read once per
+ * group of 8 slots (from L1/L2 after the first), every slot's row is read once
+ * for the weight's dot product and its gradient row written once.  The dots are
+ * summed per thread over its columns, then over the block in a fixed order. */
+template <typename T, int V>
+__global__ void __launch_bounds__(kCombineThreads)
+k_combine_grad(const T* __restrict__ go, long long ldgo, const T* __restrict__ y, long long ldy,
+               const int* __restrict__ pos, const int* __restrict__ rows, const float* __restrict__ weights,
+               long long n, int top_k, int width, T* __restrict__ gy, long long ldgy, float* __restrict__ gw) {
+    __shared__ float part[kCombineThreads / 32][8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long long m = n * top_k;
+    for (long long t = blockIdx.x; t < n; t += gridDim.x)
+        for (int s0 = 0; s0 < top_k; s0 += 8) {
+            long long p[8];
+            float wt[8], dot[8];
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                const long long q = t * top_k + s0 + s;
+                p[s] = s0 + s < top_k ? pos[q] : -1;
+                if (p[s] >= m) p[s] = -1;
+                wt[s] = p[s] >= 0 ? (weights ? weights[q] : 1.f) : 0.f;
+                dot[s] = 0.f;
+            }
+            for (int c = threadIdx.x * V; c < width; c += kCombineThreads * V) {
+                float g[V];
+                Pack<T, V>::load(go + t * ldgo + c, g);
+#pragma unroll
+                for (int s = 0; s < 8; ++s)
+                    if (p[s] >= 0) {
+                        float f[V];
+                        if (gw) {
+                            Pack<T, V>::load(y + p[s] * ldy + c, f);
+#pragma unroll
+                            for (int u = 0; u < V; ++u) dot[s] = fmaf(g[u], f[u], dot[s]);
+                        }
+#pragma unroll
+                        for (int u = 0; u < V; ++u) f[u] = wt[s] * g[u];
+                        Pack<T, V>::store(gy + p[s] * ldgy + c, f);
+                    }
+            }
+            if (gw) {
+#pragma unroll
+                for (int s = 0; s < 8; ++s) {
+                    float v = dot[s];
+                    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+                    if (lane == 0) part[warp][s] = v;
+                }
+                __syncthreads();
+                if (threadIdx.x < 8 && s0 + (int)threadIdx.x < top_k) {
+                    float v = 0.f;
+                    for (int q = 0; q < kCombineThreads / 32; ++q) v += part[q][threadIdx.x];
+                    gw[t * top_k + s0 + threadIdx.x] = v;
+                }
+                __syncthreads();
+            }
+        }
+    const int valid = *rows;
+    const int pieces = (width + V - 1) / V;
+    const float zero[V] = {};
+    for (long long r = (valid < 0 ? 0 : valid) + (long long)blockIdx.x; r < m; r += gridDim.x)
+        for (int c = threadIdx.x; c < pieces; c += kCombineThreads) Pack<T, V>::store(gy + r * ldgy + (long long)c * V, zero);
+}
+
+/* ------------------------------------------------------------- host side ---- */
+
+int sm_count() {
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    return sms;
+}
+
+bool half_type(int type) { return type == MPK_TYPE_FP16 || type == MPK_TYPE_BF16; }
+
+bool aligned16(const void* p, long long ld, size_t size) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * (long long)size % 16 == 0;
+}
+
+/* What every product needs of its sizes; the gathers' entry index and all row
+ * numbers fit 32 bits. */
+bool shape_ok(int type, long long m, int experts, int width, int k, bool gather, int top_k) {
+    return half_type(type) && m >= 0 && m < (1LL << 30) && experts >= 1 && experts <= MPK_MAX_EXPERTS && width >= 1 &&
+           width <= (1 << 20) && k >= 1 && k <= (1 << 20) && (!gather || (top_k >= 1 && m % top_k == 0));
+}
+
+mpkStatus run_product(ExpertArgs& a, cudaStream_t s) {
+    a.sms = sm_count();
+    if (!a.sms) return MPK_ERR_CUDA;
+    const cudaError_t e = a.bf16 ? launch_any<__nv_bfloat16>(a, s) : launch_any<__half>(a, s);
+    return e == cudaSuccess ? MPK_OK : MPK_ERR_CUDA;
+}
+
+template <typename T>
+cudaError_t run_combine(const void* y, long long ldy, const int* pos, const float* weights, long long n, int top_k,
+                        int width, void* out, long long ldo, int sms, cudaStream_t s) {
+    constexpr int V = 16 / sizeof(T);
+    const bool vec = width % V == 0 && aligned16(y, ldy, sizeof(T)) && aligned16(out, ldo, sizeof(T));
+    const long long pieces = n * (vec ? width / V : width);
+    const long long want = (pieces + kCombineThreads - 1) / kCombineThreads, most = (long long)sms * 64;
+    const int grid = (int)(want < most ? want : most);
+    const T *py = static_cast<const T*>(y);
+    T* po = static_cast<T*>(out);
+    if (vec) k_combine<T, V><<<grid, kCombineThreads, 0, s>>>(py, ldy, pos, weights, n, top_k, width, po, ldo);
+    else k_combine<T, 1><<<grid, kCombineThreads, 0, s>>>(py, ldy, pos, weights, n, top_k, width, po, ldo);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t run_combine_grad(const void* go, long long ldgo, const void* y, long long ldy, const int* pos,
+                             const int* rows, const float* weights, long long n, int top_k, int width, void* gy,
+                             long long ldgy, float* gw, int sms, cudaStream_t s) {
+    constexpr int V = 16 / sizeof(T);
+    const bool vec = width % V == 0 && aligned16(go, ldgo, sizeof(T)) && (!gw || aligned16(y, ldy, sizeof(T))) &&
+                     aligned16(gy, ldgy, sizeof(T));
+    const int grid = (int)(n < (long long)sms * 16 ? n : (long long)sms * 16);
+    const T *pg = static_cast<const T*>(go), *py = static_cast<const T*>(y);
+    T* po = static_cast<T*>(gy);
+    if (vec)
+        k_combine_grad<T, V><<<grid, kCombineThreads, 0, s>>>(pg, ldgo, py, ldy, pos, rows, weights, n, top_k, width,
+                                                              po, ldgy, gw);
+    else
+        k_combine_grad<T, 1><<<grid, kCombineThreads, 0, s>>>(pg, ldgo, py, ldy, pos, rows, weights, n, top_k, width,
+                                                              po, ldgy, gw);
+    return cudaGetLastError();
+}
+
+bool combine_ok(int type, long long n, int top_k, int width) {
+    return (type == MPK_TYPE_FP32 || half_type(type)) && n >= 0 && top_k >= 1 && top_k <= 1024 &&
+           n <= ((1LL << 30) - 1) / top_k && width >= 1 && width <= (1 << 20);
+}
+
+}  /* namespace */
+}  /* namespace mpk */
+
+using namespace mpk;
+
+extern "C" {
+
+mpkStatus mpkExpertGemm(cudaStream_t stream, int type, const void* dX, long long ldx, const void* dW, long long ldw,
+                        long long strideW, const int* dOffsets, const int* dOrder, int top_k, long long m,
+                        int experts, int width, int k, void* dY, long long ldy) {
+    if (!shape_ok(type, m, experts, width, k, dOrder != nullptr, top_k) || ldx < k || ldw < k || ldy < width ||
+        (experts > 1 && strideW < (long long)(width - 1) * ldw + k))
+        return MPK_ERR_INVALID;
+    if (m == 0) return MPK_OK;
+    if (!dX || !dW || !dOffsets || !dY) return MPK_ERR_INVALID;
+    ExpertArgs a{EXP_FWD, type == MPK_TYPE_BF16, dX, ldx, nullptr, 0, dW, ldw, strideW, dOffsets, dOrder, top_k,
+                 m, experts, width, k, dY, ldy, 0, 0};
+    return run_product(a, stream);
+}
+
+mpkStatus mpkExpertGemmGradX(cudaStream_t stream, int type, const void* dGY, long long ldgy, const void* dW,
+                             long long ldw, long long strideW, const int* dOffsets, long long m, int experts,
+                             int width, int k, void* dGX, long long ldgx) {
+    if (!shape_ok(type, m, experts, width, k, false, 1) || ldgy < width || ldw < k || ldgx < k ||
+        (experts > 1 && strideW < (long long)(width - 1) * ldw + k))
+        return MPK_ERR_INVALID;
+    if (m == 0) return MPK_OK;
+    if (!dGY || !dW || !dOffsets || !dGX) return MPK_ERR_INVALID;
+    ExpertArgs a{EXP_GRADX, type == MPK_TYPE_BF16, nullptr, 0, dGY, ldgy, dW, ldw, strideW, dOffsets, nullptr, 1,
+                 m, experts, width, k, dGX, ldgx, 0, 0};
+    return run_product(a, stream);
+}
+
+mpkStatus mpkExpertGemmGradW(cudaStream_t stream, int type, const void* dGY, long long ldgy, const void* dX,
+                             long long ldx, const int* dOffsets, const int* dOrder, int top_k, long long m,
+                             int experts, int width, int k, void* dGW, long long ldw, long long strideW) {
+    if (!shape_ok(type, m, experts, width, k, dOrder != nullptr, top_k) || ldgy < width || ldx < k || ldw < k ||
+        (experts > 1 && strideW < (long long)(width - 1) * ldw + k))
+        return MPK_ERR_INVALID;
+    if ((m > 0 && (!dGY || !dX)) || !dOffsets || !dGW) return MPK_ERR_INVALID;
+    ExpertArgs a{EXP_GRADW, type == MPK_TYPE_BF16, dX, ldx, dGY, ldgy, nullptr, 0, 0, dOffsets, dOrder, top_k,
+                 m, experts, width, k, dGW, ldw, strideW, 0};
+    return run_product(a, stream);
+}
+
+mpkStatus mpkExpertCombine(cudaStream_t stream, int type, const void* dY, long long ldy, const int* dPos,
+                           const float* dWeights, long long n, int top_k, int width, void* dOut, long long ldo) {
+    if (!combine_ok(type, n, top_k, width) || ldy < width || ldo < width) return MPK_ERR_INVALID;
+    if (n == 0) return MPK_OK;
+    if (!dY || !dPos || !dOut) return MPK_ERR_INVALID;
+    const int sms = sm_count();
+    if (!sms) return MPK_ERR_CUDA;
+    const cudaError_t e =
+        type == MPK_TYPE_FP32 ? run_combine<float>(dY, ldy, dPos, dWeights, n, top_k, width, dOut, ldo, sms, stream)
+        : type == MPK_TYPE_FP16 ? run_combine<__half>(dY, ldy, dPos, dWeights, n, top_k, width, dOut, ldo, sms, stream)
+        : run_combine<__nv_bfloat16>(dY, ldy, dPos, dWeights, n, top_k, width, dOut, ldo, sms, stream);
+    return e == cudaSuccess ? MPK_OK : MPK_ERR_CUDA;
+}
+
+mpkStatus mpkExpertCombineGrad(cudaStream_t stream, int type, const void* dGOut, long long ldgo, const void* dY,
+                               long long ldy, const int* dPos, const int* dRows, const float* dWeights, long long n,
+                               int top_k, int width, void* dGY, long long ldgy, float* dGWeights) {
+    if (!combine_ok(type, n, top_k, width) || ldgo < width || (dGWeights && ldy < width) || ldgy < width)
+        return MPK_ERR_INVALID;
+    if (n == 0) return MPK_OK;
+    if (!dGOut || (dGWeights && !dY) || !dPos || !dRows || !dGY) return MPK_ERR_INVALID;
+    const int sms = sm_count();
+    if (!sms) return MPK_ERR_CUDA;
+    const cudaError_t e =
+        type == MPK_TYPE_FP32 ? run_combine_grad<float>(dGOut, ldgo, dY, ldy, dPos, dRows, dWeights, n, top_k, width,
+                                                        dGY, ldgy, dGWeights, sms, stream)
+        : type == MPK_TYPE_FP16 ? run_combine_grad<__half>(dGOut, ldgo, dY, ldy, dPos, dRows, dWeights, n, top_k,
+                                                           width, dGY, ldgy, dGWeights, sms, stream)
+        : run_combine_grad<__nv_bfloat16>(dGOut, ldgo, dY, ldy, dPos, dRows, dWeights, n, top_k, width, dGY, ldgy,
+                                          dGWeights, sms, stream);
+    return e == cudaSuccess ? MPK_OK : MPK_ERR_CUDA;
+}
+
+}  /* extern "C" */

@@ -1,0 +1,682 @@
+/* route.cu -- tokens routed to experts: choice and weights, their gradient, and
+ * the plan that sorts the routed rows by expert (include/mpkexperts.h).
+ *
+ * mpkRoute, one warp a token.  With logits l, scores s (softmax or sigmoid) and
+ * choice values c = s + bias, the warp keeps the row in registers (expert 32 v +
+ * lane in register v), turns every choice value into an integer key of the same
+ * order (NaN highest, masked 0), drops the groups that lose, and takes the
+ * maximum top_k times with two warp reductions each: the key, then the lowest
+ * index that holds it.
+ *
+ * The choice is exact, as the assignment's is: without a bias, and with groups
+ * scored by their maximum, the order of c is the order of l and the keys are the
+ * logits themselves.  Otherwise c is an FP32 evaluation with a bounded error; a
+ * row in which two neighbours of the chosen sequence (the first loser included)
+ * or the groups on both sides of the cut come within twice that bound is
+ * decided again in FP64 (slow_choice), except where the two have the same logit
+ * and the same bias, which is an exact tie.  The scores of a 256-expert row lie
+ * some 1e-3 apart and the bound is about 1e-6, so few rows go there.
+ */
+#include "common.cuh"
+#include "mpkexperts.h"
+
+#include <climits>
+#include <cmath>
+
+namespace mpk {
+namespace {
+
+constexpr unsigned FULL = 0xffffffffu;
+constexpr int kRouteWarps = 4;
+
+template <typename T>
+__device__ __forceinline__ float to_f(T v);
+template <>
+__device__ __forceinline__ float to_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+template <typename T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+/* An unsigned key in the order of v: -inf (masked) 0, NaN the highest, the two
+ * zeros equal. */
+__device__ __forceinline__ unsigned key_of(float v) {
+    if (v != v) return 0xffffffffu;
+    const unsigned u = __float_as_uint(v + 0.0f);
+    const unsigned k = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+    return v == -INFINITY ? 0u : k;
+}
+__device__ __forceinline__ float of_key(unsigned k) {
+    if (k == 0xffffffffu) return NAN;
+    if (k == 0u) return -INFINITY;
+    return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+}
+__device__ __forceinline__ unsigned long long key_of(double v) {
+    if (v != v) return ~0ull;
+    const unsigned long long u = (unsigned long long)__double_as_longlong(v + 0.0);
+    const unsigned long long k = (u >> 63) ? ~u : (u | (1ull << 63));
+    return v == -(double)INFINITY ? 0ull : k;
+}
+__device__ __forceinline__ double of_key(unsigned long long k) {
+    if (k == ~0ull) return (double)NAN;
+    if (k == 0ull) return -(double)INFINITY;
+    return __longlong_as_double((long long)((k >> 63) ? (k & ~(1ull << 63)) : ~k));
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+    return v;
+}
+__device__ __forceinline__ double warp_sum(double v) {
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+    return v;
+}
+
+struct RouteShape {
+    int E, k, score, G, gs, top_groups, group_score, renorm;
+    unsigned gmul;            /* group of expert j: (j * gmul) >> 20, exact for j, gs < 1024 */
+    float scale;
+};
+
+/* The groups' keys (key of the maximum, or of the sum of the two best) from the
+ * experts' keys in shared memory: lanes [g * L, g * L + L) work on group g.  Every
+ * lane of a group's lanes returns its key; lanes past G * L return 0.  KEY is
+ * the 32-bit key of a float or the 64-bit key of a double. */
+template <typename KEY>
+__device__ __forceinline__ KEY group_key(const KEY* keys, const RouteShape& sh, int L, int lane) {
+    const int g = lane / L, sub = lane - g * L;
+    KEY a = 0, b = 0;
+    if (g < sh.G)
+        for (int i = sub; i < sh.gs; i += L) {
+            const KEY v = keys[g * sh.gs + i];
+            if (v > a) { b = a; a = v; }
+            else if (v > b) b = v;
+        }
+    for (int o = L >> 1; o > 0; o >>= 1) {
+        const KEY a2 = __shfl_xor_sync(FULL, a, o), b2 = __shfl_xor_sync(FULL, b, o);
+        if (a2 > a) { b = a > b2 ? a : b2; a = a2; }
+        else b = a2 > b ? a2 : b;
+    }
+    if (sh.group_score == MPK_GROUP_TOP2 && b != 0) a = key_of(of_key(a) + of_key(b));
+    return a;
+}
+
+/* Bit g * L of the result: group g is among the top_groups best (ties to the
+ * lowest index) and has an expert left. */
+template <typename KEY>
+__device__ __forceinline__ unsigned kept_groups(KEY gk, const RouteShape& sh, int L, int lane) {
+    const int g = lane / L;
+    int rank = 0;
+    for (int h = 0; h < sh.G; ++h) {
+        const KEY o = __shfl_sync(FULL, gk, h * L);
+        rank += (o > gk || (o == gk && h < g)) ? 1 : 0;
+    }
+    return __ballot_sync(FULL, lane == g * L && g < sh.G && gk != 0 && rank < sh.top_groups);
+}
+
+__device__ __forceinline__ int lanes_per_group(int G) {
+    int L = 1;
+    while (2 * L * G <= 32) L *= 2;
+    return L;
+}
+
+/* The whole choice of one row in FP64: slot `lane`'s expert, or -1.  keys: E
+ * 64-bit words of this warp's shared memory. */
+template <typename T>
+__device__ __noinline__ int slow_choice(const T* __restrict__ row, const float* __restrict__ bias, RouteShape sh,
+                                        unsigned long long* keys, int lane) {
+    double mx = 0.0, sum = 1.0;
+    if (sh.score == MPK_SCORE_SOFTMAX) {
+        float m = -INFINITY;
+        for (int j = lane; j < sh.E; j += 32) m = fmaxf(m, to_f(row[j]));
+        m = warp_max(m);
+        mx = m == -INFINITY ? 0.0 : (double)m;
+        sum = 0.0;
+        for (int j = lane; j < sh.E; j += 32) sum += exp((double)to_f(row[j]) - mx);
+        sum = warp_sum(sum);
+    }
+    for (int j = lane; j < sh.E; j += 32) {
+        const double x = (double)to_f(row[j]);
+        const double s = sh.score == MPK_SCORE_SOFTMAX ? exp(x - mx) / sum : 1.0 / (1.0 + exp(-x));
+        const double c = bias ? s + (double)bias[j] : s;
+        keys[j] = x == -(double)INFINITY ? 0ull : key_of(c);
+    }
+    __syncwarp();
+    if (sh.G > 1) {
+        const int L = lanes_per_group(sh.G);
+        const unsigned kept = kept_groups(group_key(keys, sh, L, lane), sh, L, lane);
+        __syncwarp();
+        for (int j = lane; j < sh.E; j += 32)
+            if (!((kept >> (((unsigned)j * sh.gmul >> 20) * L)) & 1u)) keys[j] = 0ull;
+        __syncwarp();
+    }
+    int mine = -1;
+    for (int i = 0; i < sh.k; ++i) {
+        unsigned long long b = 0ull;
+        int bj = INT_MAX;
+        for (int j = lane; j < sh.E; j += 32)
+            if (keys[j] > b) { b = keys[j]; bj = j; }
+        for (int o = 16; o > 0; o >>= 1) {
+            const unsigned long long b2 = __shfl_xor_sync(FULL, b, o);
+            const int j2 = __shfl_xor_sync(FULL, bj, o);
+            if (b2 > b || (b2 == b && j2 < bj)) { b = b2; bj = j2; }
+        }
+        if (b == 0ull) break;
+        if (lane == i) mine = bj;
+        if (lane == (bj & 31)) keys[bj] = 0ull;
+        __syncwarp();
+    }
+    __syncwarp();
+    return mine;
+}
+
+/* A chosen score up to a factor that the row's slots share, m being the largest
+ * chosen logit: e^(x - m) for softmax, and for sigmoids that are all below e^-60,
+ * where sigmoid(x) = e^x to the last bit.  As in FP64, a sigmoid below -745 is 0. */
+__device__ __forceinline__ float chosen_score(float x, float m, bool softmax) {
+    if (softmax) return expf(x - m);
+    if (m < -60.f) return x < -745.f ? 0.f : expf(x - m);
+    return 1.f / (1.f + expf(-x));
+}
+
+template <typename T, int VPL>
+__global__ void __launch_bounds__(32 * kRouteWarps)
+k_route(const T* __restrict__ logits, long long n, long long ld, const float* __restrict__ bias, RouteShape sh,
+        int* __restrict__ ids, float* __restrict__ weights) {
+    extern __shared__ unsigned long long route_sm[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    unsigned long long* keys64 = route_sm + (size_t)warp * sh.E;
+    unsigned* keys32 = reinterpret_cast<unsigned*>(keys64);
+    const bool softmax = sh.score == MPK_SCORE_SOFTMAX;
+    const bool grouped = sh.G > 1 && sh.top_groups < sh.G;
+    const bool top2 = grouped && sh.group_score == MPK_GROUP_TOP2;
+    const bool by_score = bias || top2;                       /* keys are choice values c, else logits */
+    const bool scores = by_score || (softmax && !sh.renorm);  /* some use of all experts' scores */
+    const int L = lanes_per_group(sh.G);
+    const long long step = (long long)gridDim.x * kRouteWarps;
+    for (long long t = (long long)blockIdx.x * kRouteWarps + warp; t < n; t += step) {
+        const T* row = logits + t * ld;
+        float x[VPL];
+        unsigned key[VPL];
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) x[v] = 32 * v + lane < sh.E ? to_f(row[32 * v + lane]) : -INFINITY;
+        float mx = 0.f, sum = 1.f, smax = 1.f;
+        if (scores) {
+            float c[VPL];
+            if (softmax) {
+                mx = x[0];
+#pragma unroll
+                for (int v = 1; v < VPL; ++v) mx = fmaxf(mx, x[v]);
+                mx = warp_max(mx);
+                if (mx == -INFINITY) mx = 0.f;
+                sum = 0.f;
+#pragma unroll
+                for (int v = 0; v < VPL; ++v) { c[v] = expf(x[v] - mx); sum += c[v]; }
+                sum = warp_sum(sum);
+                smax = 1.f / sum;
+#pragma unroll
+                for (int v = 0; v < VPL; ++v) c[v] *= smax;
+            } else {
+#pragma unroll
+                for (int v = 0; v < VPL; ++v) c[v] = 1.f / (1.f + expf(-x[v]));
+            }
+#pragma unroll
+            for (int v = 0; v < VPL; ++v) {
+                if (bias && 32 * v + lane < sh.E) c[v] += bias[32 * v + lane];
+                key[v] = x[v] == -INFINITY ? 0u : key_of(by_score ? c[v] : x[v]);
+            }
+        } else {
+#pragma unroll
+            for (int v = 0; v < VPL; ++v) key[v] = key_of(x[v]);
+        }
+        /* Error bounds of c.  expf and the sigmoid's division leave a few 2^-23
+         * of s; softmax adds |x - mx| 2^-24 s from the rounded argument, which is
+         * under 2^-17 s wherever s does not underflow and under 2^-19 of the
+         * row's largest score everywhere; adding the bias rounds by 2^-24 |c|. */
+        auto near = [&](float a, float b) {
+            const float tol = bias ? (softmax ? 0x1.0p-18f : 0x1.0p-20f) * smax + 0x1.0p-22f * (fabsf(a) + fabsf(b))
+                                   : 0x1.0p-16f * (fabsf(a) + fabsf(b)) + 1e-44f;
+            return !(a - b > tol);
+        };
+        bool slow = false;
+        if (grouped) {
+#pragma unroll
+            for (int v = 0; v < VPL; ++v)
+                if (32 * v + lane < sh.E) keys32[32 * v + lane] = key[v];
+            __syncwarp();
+            const unsigned gk = group_key(keys32, sh, L, lane);
+            const unsigned kept = kept_groups(gk, sh, L, lane);
+            if (by_score) {
+                const int g = lane / L;
+                const bool there = lane == g * L && g < sh.G, in = (kept >> lane) & 1u;
+                const unsigned lo = __reduce_min_sync(FULL, there && in ? gk : 0xffffffffu);
+                const unsigned hi = __reduce_max_sync(FULL, there && !in ? gk : 0u);
+                if (kept && hi) slow = near(of_key(lo), of_key(hi));
+            }
+#pragma unroll
+            for (int v = 0; v < VPL; ++v) {
+                const unsigned g = ((unsigned)(32 * v + lane) * sh.gmul >> 20) * L;
+                if (!(g < 32 && ((kept >> g) & 1u))) key[v] = 0u;
+                else if (top2 && !bias) key[v] = key_of(x[v]);      /* groups chosen: the logits' order again */
+            }
+            __syncwarp();
+        }
+        int mine = -1;
+        unsigned mykey = 0;
+        {
+            unsigned bk = 0;
+            int bv = 0;
+#pragma unroll
+            for (int v = 0; v < VPL; ++v)
+                if (key[v] > bk) { bk = key[v]; bv = v; }
+            const int takes = sh.k + (bias && sh.k < 32 ? 1 : 0);
+            for (int i = 0; i < takes; ++i) {
+                const unsigned top = __reduce_max_sync(FULL, bk);
+                if (top == 0u) break;
+                const unsigned j = __reduce_min_sync(FULL, bk == top ? (unsigned)(32 * bv + lane) : 0xffffffffu);
+                if (lane == i) { mine = (int)j; mykey = top; }
+                if (lane == (int)(j & 31u)) {
+#pragma unroll
+                    for (int v = 0; v < VPL; ++v)
+                        if (v == bv) key[v] = 0u;
+                    bk = 0u;
+                    bv = 0;
+#pragma unroll
+                    for (int v = 0; v < VPL; ++v)
+                        if (key[v] > bk) { bk = key[v]; bv = v; }
+                }
+            }
+        }
+        if (bias) {
+            const unsigned nk = __shfl_down_sync(FULL, mykey, 1);
+            const int nj = __shfl_down_sync(FULL, mine, 1);
+            if (lane < sh.k && lane < 31 && mine >= 0 && nj >= 0 && near(of_key(mykey), of_key(nk)))
+                slow = slow || !(to_f(row[mine]) == to_f(row[nj]) && bias[mine] == bias[nj]);
+            if (sh.k == 32) slow = true;                            /* no lane holds the first loser */
+        }
+        const bool again = __any_sync(FULL, slow);
+        if (again) mine = slow_choice(row, bias, sh, keys64, lane);
+        if (lane >= sh.k) mine = -1;
+        const bool valid = mine >= 0;
+        const float xi = !valid ? -INFINITY : (bias || again) ? to_f(row[mine]) : of_key(mykey);
+        float w;
+        if (sh.renorm) {
+            const float m = warp_max(xi);
+            const float e = valid ? chosen_score(xi, m, softmax) : 0.f;
+            const float total = warp_sum(e);
+            w = total == 0.f ? 0.f : e / total;
+            if (valid && sum != sum) w = NAN;
+        } else {
+            w = !valid ? 0.f : softmax ? expf(xi - mx) / sum : 1.f / (1.f + expf(-xi));
+        }
+        if (lane < sh.k) {
+            ids[t * sh.k + lane] = mine;
+            weights[t * sh.k + lane] = valid ? w * sh.scale : 0.f;
+        }
+    }
+}
+
+/* Gradient of the weights, one warp a token.  With w the weights at scale 1, g
+ * the incoming gradient times the scale and G = sum of g w over the slots:
+ *   renormalized:  softmax  dl_i = w_i (g_i - G)
+ *                  sigmoid  dl_i = w_i (1 - s_i) (g_i - G)      0 off the slots
+ *   otherwise:     sigmoid  dl_i = g_i s_i (1 - s_i)            0 off the slots
+ *                  softmax  dl_j = s_j ([j chosen] g_j - sum over slots of g s)
+ * so only the last form reads the whole row.  Slot i's term is formed by lane i;
+ * every lane then collects the terms of its own experts, so a row is written once. */
+template <typename T, int VPL>
+__global__ void __launch_bounds__(32 * kRouteWarps)
+k_route_grad(const T* __restrict__ logits, long long n, long long ld, RouteShape sh, const int* __restrict__ ids,
+             const float* __restrict__ gw, T* __restrict__ out, long long ldg) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const bool softmax = sh.score == MPK_SCORE_SOFTMAX;
+    const bool whole = softmax && !sh.renorm;
+    const long long step = (long long)gridDim.x * kRouteWarps;
+    for (long long t = (long long)blockIdx.x * kRouteWarps + warp; t < n; t += step) {
+        const T* row = logits + t * ld;
+        int id = lane < sh.k ? ids[t * sh.k + lane] : -1;
+        if ((unsigned)id >= (unsigned)sh.E) id = -1;
+        const bool valid = id >= 0;
+        const float g = valid ? gw[t * sh.k + lane] * sh.scale : 0.f;
+        const float xi = valid ? to_f(row[id]) : -INFINITY;
+        float s[VPL], acc[VPL];
+        float term, dot = 0.f;
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) acc[v] = 0.f;
+        if (whole) {
+            float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int v = 0; v < VPL; ++v) {
+                s[v] = 32 * v + lane < sh.E ? to_f(row[32 * v + lane]) : -INFINITY;
+                mx = fmaxf(mx, s[v]);
+            }
+            mx = warp_max(mx);
+            if (mx == -INFINITY) mx = 0.f;
+#pragma unroll
+            for (int v = 0; v < VPL; ++v) { s[v] = expf(s[v] - mx); sum += s[v]; }
+            sum = warp_sum(sum);
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;        /* every expert masked: no gradient */
+#pragma unroll
+            for (int v = 0; v < VPL; ++v) s[v] *= inv;
+            dot = warp_sum(valid ? g * (expf(xi - mx) * inv) : 0.f);
+            term = g;
+        } else {
+            const float si = valid ? 1.f / (1.f + expf(-xi)) : 0.f;
+            const float left = softmax ? 1.f : 1.f / (1.f + expf(xi));      /* 1 - s */
+            if (sh.renorm) {
+                const float m = warp_max(xi);
+                const float e = (!valid || m == -INFINITY) ? 0.f : chosen_score(xi, m, softmax);
+                const float total = warp_sum(e);
+                const float w = total == 0.f ? 0.f : e / total;
+                const float G = warp_sum(valid ? g * w : 0.f);
+                term = w * left * (g - G);
+            } else {
+                term = g * si * left;
+            }
+        }
+        for (int i = 0; i < sh.k; ++i) {
+            const int j = __shfl_sync(FULL, id, i);
+            const float d = __shfl_sync(FULL, term, i);
+            if (j >= 0 && (j & 31) == lane) {
+#pragma unroll
+                for (int v = 0; v < VPL; ++v)
+                    if (v == (j >> 5)) acc[v] += d;
+            }
+        }
+        T* dst = out + t * ldg;
+#pragma unroll
+        for (int v = 0; v < VPL; ++v)
+            if (32 * v + lane < sh.E) dst[32 * v + lane] = from_f<T>(whole ? s[v] * (acc[v] - dot) : acc[v]);
+    }
+}
+
+/* -------------------------------------------------------------- the plan ---- */
+/* A stable counting sort.  A block takes a chunk of the entries, each of its
+ * warps a contiguous piece; a warp counts 32 entries at a time with
+ * match_any (the lanes that share an expert), so an entry's rank among its
+ * expert's is (entries of earlier blocks) + (of earlier warps) + (of this warp so
+ * far) + (lower lanes of its match): no atomics, and the order is fixed. */
+constexpr int kPlanThreads = 512, kPlanWarps = kPlanThreads / 32;
+constexpr int kPlanChunk = 4096;             /* entries a block of the multi-block plan */
+constexpr int kPlanOne = 16384;              /* up to here one block does everything in one launch */
+
+__device__ __forceinline__ int plan_id(const int* ids, long long i, long long end, int E) {
+    const int a = i < end ? ids[i] : -1;
+    return (unsigned)a < (unsigned)E ? a : -1;
+}
+
+/* Counts of this warp's piece [lo, hi) into cnt (E ints of shared memory, zeroed). */
+__device__ __forceinline__ void plan_count(const int* ids, long long lo, long long hi, int E, int* cnt, int lane) {
+    for (long long i = lo; i < hi; i += 32) {
+        const int a = plan_id(ids, i + lane, hi, E);
+        const unsigned peers = __match_any_sync(FULL, a);
+        if (a >= 0 && lane == __ffs(peers) - 1) cnt[a] += __popc(peers);
+        __syncwarp();
+    }
+}
+
+/* Exclusive scan of one int per thread over the block; tot receives the total. */
+__device__ __forceinline__ int block_scan(int v, int* part, int& tot) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    int incl = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(FULL, incl, o);
+        if (lane >= o) incl += u;
+    }
+    if (lane == 31) part[w] = incl;
+    __syncthreads();
+    int run = 0;
+    tot = 0;
+    for (int q = 0; q < kPlanWarps; ++q) {
+        if (q < w) run += part[q];
+        tot += part[q];
+    }
+    __syncthreads();
+    return run + incl - v;
+}
+
+/* cnt[w * E + e] (counts of each warp) becomes the first sorted row of warp w's
+ * entries of expert e, given before[e] rows of e in earlier blocks (NULL: none)
+ * and the experts' totals (NULL: the block's own).  Returns the total of all;
+ * block 0 writes the offsets. */
+__device__ int plan_starts(int* cnt, int E, const int* before, long long before_stride, const int* totals,
+                           int* offsets, int* part) {
+    int carry = 0;
+    for (int e0 = 0; e0 < E; e0 += kPlanThreads) {
+        const int e = e0 + threadIdx.x;
+        int own = 0;
+        if (e < E)
+            for (int w = 0; w < kPlanWarps; ++w) {
+                const int c = cnt[w * E + e];
+                cnt[w * E + e] = own;
+                own += c;
+            }
+        int tot;
+        const int base = carry + block_scan(e < E ? (totals ? totals[e] : own) : 0, part, tot);
+        if (e < E) {
+            const int first = base + (before ? before[e * before_stride] : 0);
+            for (int w = 0; w < kPlanWarps; ++w) cnt[w * E + e] += first;
+            if (offsets) offsets[e] = base;
+        }
+        carry += tot;
+    }
+    if (offsets && threadIdx.x == 0) offsets[E] = carry;
+    __syncthreads();
+    return carry;
+}
+
+__device__ __forceinline__ void plan_place(const int* ids, long long lo, long long hi, int E, int* at, int* order,
+                                           int* pos, int lane) {
+    for (long long i = lo; i < hi; i += 32) {
+        const int a = plan_id(ids, i + lane, hi, E);
+        const unsigned peers = __match_any_sync(FULL, a);
+        const int r = a >= 0 ? at[a] + __popc(peers & ((1u << lane) - 1u)) : -1;
+        if (i + lane < hi) pos[i + lane] = r;
+        if (r >= 0) order[r] = (int)(i + lane);
+        __syncwarp();
+        if (a >= 0 && lane == __ffs(peers) - 1) at[a] += __popc(peers);
+        __syncwarp();
+    }
+}
+
+/* STAGE 0: the whole plan in one block.  STAGE 1: this block's counts to
+ * work[e * B + b].  STAGE 2: placement, with work scanned by k_plan_scan. */
+template <int STAGE>
+__global__ void __launch_bounds__(kPlanThreads)
+k_plan(const int* __restrict__ ids, long long m, int E, long long chunk, int* __restrict__ work,
+       int* __restrict__ offsets, int* __restrict__ order, int* __restrict__ pos) {
+    extern __shared__ int cnt[];                 /* kPlanWarps x E */
+    __shared__ int part[kPlanWarps];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const long long c0 = (long long)blockIdx.x * chunk, c1 = min(m, c0 + chunk);
+    const long long piece = ((chunk + kPlanWarps - 1) / kPlanWarps + 31) / 32 * 32;
+    const long long lo = min(c1, c0 + w * piece), hi = min(c1, lo + piece);
+    const long long B = gridDim.x;
+    for (int i = threadIdx.x; i < kPlanWarps * E; i += kPlanThreads) cnt[i] = 0;
+    __syncthreads();
+    plan_count(ids, lo, hi, E, cnt + w * E, lane);
+    __syncthreads();
+    if (STAGE == 1) {
+        for (int e = threadIdx.x; e < E; e += kPlanThreads) {
+            int s = 0;
+            for (int q = 0; q < kPlanWarps; ++q) s += cnt[q * E + e];
+            work[e * B + blockIdx.x] = s;
+        }
+        return;
+    }
+    const int total = STAGE == 0 ? plan_starts(cnt, E, nullptr, 0, nullptr, offsets, part)
+                                 : plan_starts(cnt, E, work + blockIdx.x, B, work + E * B,
+                                               blockIdx.x == 0 ? offsets : nullptr, part);
+    plan_place(ids, lo, hi, E, cnt + w * E, order, pos, lane);
+    for (long long r = total + (long long)blockIdx.x * kPlanThreads + threadIdx.x; r < m; r += B * kPlanThreads)
+        order[r] = -1;
+}
+
+/* One warp an expert: its counts over the blocks become their exclusive prefix,
+ * its total goes behind them. */
+__global__ void k_plan_scan(int* __restrict__ work, int E, int B) {
+    const int lane = threadIdx.x & 31, e = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    if (e >= E) return;
+    int* row = work + (size_t)e * B;
+    int run = 0;
+    for (int b0 = 0; b0 < B; b0 += 32) {
+        const int v = b0 + lane < B ? row[b0 + lane] : 0;
+        int incl = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(FULL, incl, o);
+            if (lane >= o) incl += u;
+        }
+        if (b0 + lane < B) row[b0 + lane] = run + incl - v;
+        run += __shfl_sync(FULL, incl, 31);
+    }
+    if (lane == 0) work[(size_t)E * B + e] = run;
+}
+
+/* ------------------------------------------------------------- host side ---- */
+
+bool route_shape(const mpkRouteParams* p, RouteShape& sh, bool choice) {
+    if (!p || p->experts < 1 || p->experts > MPK_MAX_EXPERTS || p->top_k < 1 || p->top_k > MPK_MAX_TOP_K ||
+        p->top_k > p->experts || (p->score != MPK_SCORE_SOFTMAX && p->score != MPK_SCORE_SIGMOID) ||
+        !std::isfinite(p->scale))
+        return false;
+    sh = RouteShape{p->experts, p->top_k, p->score, 1, p->experts, 1, MPK_GROUP_MAX, p->renormalize ? 1 : 0, 0, p->scale};
+    if (choice) {
+        if (p->groups < 1 || p->groups > MPK_MAX_GROUPS || p->experts % p->groups || p->top_groups < 1 ||
+            p->top_groups > p->groups || (p->group_score != MPK_GROUP_MAX && p->group_score != MPK_GROUP_TOP2))
+            return false;
+        sh.G = p->groups;
+        sh.gs = p->experts / p->groups;
+        sh.top_groups = p->top_groups;
+        sh.group_score = p->group_score;
+    }
+    /* j * gmul / 2^20 exceeds j / gs by less than j / 2^20 < 1 / gs */
+    sh.gmul = ((1u << 20) + sh.gs - 1) / sh.gs;
+    return true;
+}
+
+int sm_count() {
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    return sms;
+}
+
+/* one warp a token until every SM holds its 16 blocks of four warps */
+int route_grid(long long n, int sms) {
+    const long long b = (n + kRouteWarps - 1) / kRouteWarps;
+    return (int)(b < (long long)sms * 16 ? b : (long long)sms * 16);
+}
+
+template <typename T, int VPL>
+cudaError_t run_route(const RouteShape& sh, const void* logits, long long n, long long ld, const float* bias, int* ids,
+                      float* w, int sms, cudaStream_t s) {
+    const size_t smem = (bias || sh.G > 1) ? (size_t)kRouteWarps * sh.E * 8 : 0;
+    k_route<T, VPL><<<route_grid(n, sms), 32 * kRouteWarps, smem, s>>>(static_cast<const T*>(logits), n, ld, bias, sh,
+                                                                      ids, w);
+    return cudaGetLastError();
+}
+
+template <typename T, int VPL>
+cudaError_t run_route_grad(const RouteShape& sh, const void* logits, long long n, long long ld, const int* ids,
+                           const float* gw, void* out, long long ldg, int sms, cudaStream_t s) {
+    k_route_grad<T, VPL><<<route_grid(n, sms), 32 * kRouteWarps, 0, s>>>(static_cast<const T*>(logits), n, ld, sh, ids,
+                                                                        gw, static_cast<T*>(out), ldg);
+    return cudaGetLastError();
+}
+
+/* The registers a row takes: 32 * VPL >= experts. */
+#define MPK_BY_WIDTH(T, CALL)                                      \
+    (sh.E <= 32 ? CALL(T, 1) : sh.E <= 64 ? CALL(T, 2) : sh.E <= 128 ? CALL(T, 4) \
+     : sh.E <= 256 ? CALL(T, 8) : sh.E <= 512 ? CALL(T, 16) : CALL(T, 32))
+#define MPK_BY_TYPE(CALL)                                          \
+    (type == MPK_TYPE_FP32 ? MPK_BY_WIDTH(float, CALL)             \
+     : type == MPK_TYPE_FP16 ? MPK_BY_WIDTH(__half, CALL) : MPK_BY_WIDTH(__nv_bfloat16, CALL))
+
+bool type_ok(int type) { return type == MPK_TYPE_FP32 || type == MPK_TYPE_FP16 || type == MPK_TYPE_BF16; }
+
+long long plan_blocks(long long m) { return m <= kPlanOne ? 1 : (m + kPlanChunk - 1) / kPlanChunk; }
+
+}  /* namespace */
+}  /* namespace mpk */
+
+using namespace mpk;
+
+extern "C" {
+
+void mpkRouteParamsInit(mpkRouteParams* p) {
+    if (!p) return;
+    *p = mpkRouteParams{0, 0, MPK_SCORE_SOFTMAX, 1, 1, MPK_GROUP_MAX, 1, 1.0f};
+}
+
+mpkStatus mpkRoute(cudaStream_t stream, const mpkRouteParams* p, const void* dLogits, int type, long long n,
+                   long long ld, const float* dBias, int* dIds, float* dWeights) {
+    RouteShape sh;
+    if (!route_shape(p, sh, true) || !type_ok(type) || n < 0 || n > (1LL << 40) || ld < sh.E) return MPK_ERR_INVALID;
+    if (n == 0) return MPK_OK;
+    if (!dLogits || !dIds || !dWeights) return MPK_ERR_INVALID;
+    const int sms = sm_count();
+    if (!sms) return MPK_ERR_CUDA;
+#define MPK_ROUTE(T, V) run_route<T, V>(sh, dLogits, n, ld, dBias, dIds, dWeights, sms, stream)
+    return MPK_BY_TYPE(MPK_ROUTE) == cudaSuccess ? MPK_OK : MPK_ERR_CUDA;
+#undef MPK_ROUTE
+}
+
+mpkStatus mpkRouteGrad(cudaStream_t stream, const mpkRouteParams* p, const void* dLogits, int type, long long n,
+                       long long ld, const int* dIds, const float* dGradWeights, void* dGradLogits, long long ldg) {
+    RouteShape sh;
+    if (!route_shape(p, sh, false) || !type_ok(type) || n < 0 || n > (1LL << 40) || ld < sh.E || ldg < sh.E)
+        return MPK_ERR_INVALID;
+    if (n == 0) return MPK_OK;
+    if (!dLogits || !dIds || !dGradWeights || !dGradLogits) return MPK_ERR_INVALID;
+    const int sms = sm_count();
+    if (!sms) return MPK_ERR_CUDA;
+#define MPK_ROUTE(T, V) run_route_grad<T, V>(sh, dLogits, n, ld, dIds, dGradWeights, dGradLogits, ldg, sms, stream)
+    return MPK_BY_TYPE(MPK_ROUTE) == cudaSuccess ? MPK_OK : MPK_ERR_CUDA;
+#undef MPK_ROUTE
+}
+
+size_t mpkExpertPlanBytes(long long n, int top_k, int experts) {
+    if (n <= 0 || top_k < 1 || experts < 1 || experts > MPK_MAX_EXPERTS || n > (1LL << 30) / top_k) return 0;
+    const long long B = plan_blocks(n * top_k);
+    return B == 1 ? 0 : (size_t)(experts * B + experts) * sizeof(int);
+}
+
+mpkStatus mpkExpertPlan(cudaStream_t stream, const int* dIds, long long n, int top_k, int experts, int* dOffsets,
+                        int* dOrder, int* dPos, void* dWork, size_t work_bytes) {
+    if (n < 0 || top_k < 1 || experts < 1 || experts > MPK_MAX_EXPERTS || n > ((1LL << 30) - 1) / top_k || !dOffsets)
+        return MPK_ERR_INVALID;
+    const long long m = n * top_k;
+    if (m > 0 && (!dIds || !dOrder || !dPos)) return MPK_ERR_INVALID;
+    const size_t need = mpkExpertPlanBytes(n, top_k, experts);
+    if (need && (!dWork || work_bytes < need || reinterpret_cast<uintptr_t>(dWork) % sizeof(int))) return MPK_ERR_INVALID;
+    const int smem = kPlanWarps * experts * (int)sizeof(int);
+    const int B = (int)plan_blocks(m);
+    int* work = static_cast<int*>(dWork);
+    if (smem > 48 * 1024) {
+        if (cudaFuncSetAttribute(k_plan<0>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+            cudaFuncSetAttribute(k_plan<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+            cudaFuncSetAttribute(k_plan<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+            return MPK_ERR_CUDA;
+    }
+    if (B == 1) {
+        k_plan<0><<<1, kPlanThreads, smem, stream>>>(dIds, m, experts, m, nullptr, dOffsets, dOrder, dPos);
+    } else {
+        k_plan<1><<<B, kPlanThreads, smem, stream>>>(dIds, m, experts, kPlanChunk, work, nullptr, nullptr, nullptr);
+        k_plan_scan<<<(experts + 7) / 8, 256, 0, stream>>>(work, experts, B);
+        k_plan<2><<<B, kPlanThreads, smem, stream>>>(dIds, m, experts, kPlanChunk, work, dOffsets, dOrder, dPos);
+    }
+    return cudaGetLastError() == cudaSuccess ? MPK_OK : MPK_ERR_CUDA;
+}
+
+}  /* extern "C" */
