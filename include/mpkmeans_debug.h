@@ -72,6 +72,9 @@ mpkStatus mpkDebugMGFailNextWait(void);
  * Returns -1 when the word cannot be read.  No reference counterpart. */
 int mpkDebugGemmStatus(int clear);
 
+/* The same for the tensor-core products of mpkexperts.h. */
+int mpkDebugExpertStatus(int clear);
+
 /* Test hook: process the queued wide rows in rounds of at most `rows` (down
  * from the engine's capacity), to exercise several rounds on small inputs
  * (k >= 4096; with smaller k there is one round and the rows past it rescan

@@ -203,6 +203,7 @@ SIGNATURES = {
     "mpkDebugWideCounters": (_I, [_P, ctypes.POINTER(_LL), ctypes.POINTER(_LL), ctypes.POINTER(_LL)]),
     "mpkDebugWideRoundRows": (_I, [_P, _LL]),
     "mpkDebugGemmStatus": (_I, [_I]),
+    "mpkDebugExpertStatus": (_I, [_I]),
     "mpkDebugEngineLaunches": (_LL, [_P]),
     "mpkDebugSetWaitLimit": (_I, [_P, ctypes.c_ulonglong]),
     "mpkDebugInjectStall": (_I, [_P, _I]),

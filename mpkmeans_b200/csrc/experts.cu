@@ -330,7 +330,8 @@ bool shape_ok(int type, long long m, int experts, int width, int k, bool gather,
 mpkStatus run_product(ExpertArgs& a, cudaStream_t s) {
     a.sms = sm_count();
     if (!a.sms) return MPK_ERR_CUDA;
-    const cudaError_t e = a.bf16 ? launch_any<__nv_bfloat16>(a, s) : launch_any<__half>(a, s);
+    const cudaError_t e = experts_tc_ok(a) ? launch_experts_tc(a, s)
+                          : a.bf16 ? launch_any<__nv_bfloat16>(a, s) : launch_any<__half>(a, s);
     return e == cudaSuccess ? MPK_OK : MPK_ERR_CUDA;
 }
 

@@ -1,0 +1,616 @@
+/* experts_tc.cu -- the experts' products on tcgen05 (sm_100a).
+ *
+ * One persistent kernel for the product and its two gradients.  All three are
+ * out[j][f] = sum_c A[f][c] B[j][c] for one expert, with f the output's contiguous
+ * dimension (the 128 lanes of a TMEM accumulator) and j its rows (the columns):
+ *
+ *          f        j              c      A (128 f a CTA)        B (BN j)
+ *   FWD    width    expert's rows  k      W_e, K-major           X rows, K-major
+ *   GRADX  k        expert's rows  width  W_e, MN-major          GY rows, K-major
+ *   GRADW  k        width          rows   X rows, MN-major       GY rows, MN-major
+ *
+ * so weights are always the wide operand's source, a short segment of rows costs
+ * only a narrow tile (BN = 32 .. 128 for few rows an expert), and every store of
+ * a warp runs along f.  The experts' row counts are on the device only: each CTA
+ * scans them into shared memory and the grid walks the tiles of all experts.
+ *
+ *   warp 0      TMA producer: one 64-deep stage of A and B at a time.  Gathered
+ *               rows come by tile::gather4, four token rows a lane, so no sorted
+ *               copy of X is written; sorted rows come as plain boxes.
+ *   warp 1      MMA issuer, whole contraction into one FP32 TMEM accumulator, two
+ *               accumulators so that the next tile's MMAs overlap the epilogue.
+ *   warps 2-9   epilogue: round to the output type, swap halves between lane
+ *               pairs so that a lane holds two neighbouring f, store 4 bytes.
+ *
+ * PAIR: two CTAs on two SMs share each MMA (cta_group::2, 256 f x 256 j): every
+ * CTA stages its 128 f of A and 128 j of B, 32 KB for 256 x 256 x 64 products of
+ * the pair, half the operand traffic of one-CTA 128 x 256 tiles.
+ *
+ * Rows past a segment.  FWD and GRADX read whatever rows follow (a gather repeats
+ * the segment's first): a column of the accumulator depends on its own row only
+ * and those columns are not stored.  GRADW contracts over the rows, so the last
+ * stage of a segment fetches both operands by gather with an index past the
+ * tensor for the rows that are not the expert's, which TMA fills with zeros.
+ */
+#include "experts.cuh"
+#include "mpkexperts.h"
+#include "mpkmeans_debug.h"
+
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
+namespace mpk {
+namespace {
+
+/* Bounded waits that ran out in any product kernel of this device (MPK_DEV_* bits). */
+__device__ int g_experts_status;
+
+constexpr int BM = 128, BK = 64;
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr int A_STAGE = BM * BK * 2;             /* 16 KB */
+constexpr int BOX = 64 * 64 * 2;                 /* one 64 x 64 MN-major box */
+constexpr int kSmemMax = 232448;
+constexpr int kMisc = 1024 + 4 * (MPK_MAX_EXPERTS + 1);
+constexpr int kGroup = 8;                        /* row tiles that sweep the f tiles together */
+
+template <int BN, bool PAIR>
+struct Cfg {
+    static constexpr int BL = PAIR ? BN / 2 : BN;              /* j's this CTA stages */
+    static constexpr int FT = PAIR ? 2 * BM : BM;              /* f's of one tile */
+    static constexpr int B_STAGE = BL * BK * 2;
+    static constexpr int STAGE = A_STAGE + B_STAGE;
+    static constexpr int RAW = (kSmemMax - kMisc) / STAGE;
+    static constexpr int STAGES = RAW > 12 ? 12 : RAW;
+    static constexpr int SMEM_BYTES = STAGES * STAGE + kMisc;
+    static constexpr int TMEM_COLS = 2 * BN < 32 ? 32 : 2 * BN;
+    static constexpr int HALF = BN / 2;                        /* columns an epilogue warp */
+    static constexpr int CH = HALF < 32 ? HALF : 32;           /* columns of one TMEM load */
+    static_assert(BL <= 128, "one gather4 a lane");
+    static_assert(CH == 16 || CH == 32, "TMEM load width");
+    static_assert(TMEM_COLS <= 512, "TMEM columns");
+    static_assert(STAGE % 1024 == 0, "swizzle atoms");
+};
+
+template <int STAGES>
+struct EMisc {
+    uint64_t full[STAGES], empty[STAGES], t_full[2], t_empty[2], fin;
+    uint32_t tmem_slot;
+    int abort_flag;
+};
+
+struct Params {
+    const int* offsets;
+    const int* order;           /* gathered rows (NULL: sorted) */
+    int top_k, m, experts, xrows;
+    int F, J, C;                /* J: GRADW's rows of one expert's output; C: contraction (not GRADW) */
+    void* out;
+    long long ldo, stride_o;
+    int pairs;                  /* 4-byte stores are aligned */
+};
+
+/* Four rows of a 2-D tensor map with a one-row box, 64 elements from x each, to
+ * 4 x 128 bytes of shared memory (swizzled by address like any other box). */
+__device__ __forceinline__ void tma_gather4(const CUtensorMap* map, uint64_t* bar, void* smem, int x, const int (&r)[4]) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+        :: "r"(smem_u32(smem)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(r[0]), "r"(r[1]),
+           "r"(r[2]), "r"(r[3])
+        : "memory");
+}
+__device__ __forceinline__ void tma_gather4_pair(const CUtensorMap* map, uint32_t bar, void* smem, int x,
+                                                 const int (&r)[4]) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2"
+        " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+        :: "r"(smem_u32(smem)), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(r[0]), "r"(r[1]),
+           "r"(r[2]), "r"(r[3])
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_2d_pair(const CUtensorMap* map, uint32_t bar, void* smem, int x, int y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4}], [%2];"
+        :: "r"(smem_u32(smem)), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+        : "memory");
+}
+
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+    int ok = 0;
+    if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort_flag, &g_experts_status) ? 1 : 0;
+    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+
+__device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity) {
+    const unsigned long long t0 = globaltimer();
+    while (!mbar_try_wait(bar, parity))
+        if (globaltimer() - t0 > kWaitLimitNs) return;
+}
+
+/* One tile of one expert's output. */
+struct Tile {
+    int e;
+    int r0, rows;               /* the expert's sorted rows */
+    int j0, nj;                 /* first output row inside the expert, rows of this tile */
+    int f0;
+    int nk;                     /* 64-deep contraction steps */
+};
+
+/* The tiles of all experts in the order they are worked on: expert by expert,
+ * inside one kGroup row tiles at a time, their f tiles in turn, the row tiles
+ * innermost -- CTAs that run together then share a few tiles of W and of X, and
+ * a weight matrix larger than L2 is read once per kGroup row tiles.
+ * start[e] is the first row tile of expert e. */
+template <int MODE, int BN, int FTILE>
+struct Tiles {
+    const Params& p;
+    const int* start;
+    int ft;                     /* f tiles */
+    int e;
+    __device__ Tiles(const Params& p_, const int* start_) : p(p_), start(start_), ft((p_.F + FTILE - 1) / FTILE), e(0) {}
+    __device__ long long total() const { return (long long)start[p.experts] * ft; }
+    /* u ascends from call to call */
+    __device__ Tile at(long long u) {
+        while ((long long)start[e + 1] * ft <= u) ++e;
+        Tile t;
+        t.e = e;
+        const int l0 = start[e], count = start[e + 1] - l0;
+        const long long l = u - (long long)l0 * ft;
+        const int g = (int)(l / ((long long)kGroup * ft));
+        const int rem = (int)(l - (long long)g * kGroup * ft);
+        const int in = min(kGroup, count - g * kGroup);
+        const int jt = g * kGroup + rem % in;
+        t.f0 = rem / in * FTILE;
+        t.j0 = jt * BN;
+        t.r0 = expert_start(p.offsets, e, p.m);
+        t.rows = max(expert_start(p.offsets, e + 1, p.m) - t.r0, 0);
+        t.nj = min(BN, (MODE == EXP_GRADW ? p.J : t.rows) - t.j0);
+        t.nk = ((MODE == EXP_GRADW ? t.rows : p.C) + BK - 1) / BK;
+        return t;
+    }
+};
+
+__device__ __forceinline__ uint32_t pack2(float a, float b, bool bf16) {
+    uint32_t r;
+    if (bf16) asm("cvt.rn.bf16x2.f32 %0, %2, %1;" : "=r"(r) : "f"(a), "f"(b));
+    else asm("cvt.rn.f16x2.f32 %0, %2, %1;" : "=r"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+template <int MODE, int BN, bool PAIR, int FMT>
+__global__ void __launch_bounds__(kThreads, 1)
+k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+             const __grid_constant__ CUtensorMap tmAg, const __grid_constant__ CUtensorMap tmBg, const Params p) {
+    using K = Cfg<BN, PAIR>;
+    constexpr int STAGES = K::STAGES, STAGE = K::STAGE, BL = K::BL;
+    constexpr bool A_MN = MODE != EXP_FWD, B_MN = MODE == EXP_GRADW;
+    static_assert(sizeof(EMisc<STAGES>) <= 1024, "misc");
+    extern __shared__ __align__(1024) uint8_t smem[];
+    EMisc<STAGES>& ms = *reinterpret_cast<EMisc<STAGES>*>(smem + STAGES * STAGE);
+    int* start = reinterpret_cast<int*>(smem + STAGES * STAGE + 1024);
+    volatile int* abort_flag = &ms.abort_flag;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = PAIR ? (int)cluster_rank() : 0;
+    const long long u0 = PAIR ? blockIdx.x >> 1 : blockIdx.x, ustep = PAIR ? gridDim.x >> 1 : gridDim.x;
+
+    if (smem_u32(smem) & 1023u) {
+        if (threadIdx.x == 0) atomicOr(&g_experts_status, MPK_DEV_TIMEOUT);
+        return;
+    }
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < STAGES; ++i) { mbar_init(&ms.full[i], 1); mbar_init(&ms.empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&ms.t_full[i], 1); mbar_init(&ms.t_empty[i], (PAIR ? 2 : 1) * kEpiWarps); }
+        mbar_init(&ms.fin, 1);
+        ms.abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 0 && lane == 0) { tma_prefetch_desc(&tmA); tma_prefetch_desc(&tmB); }
+    if (warp == 1) {
+        if (PAIR) tmem_alloc_pair(&ms.tmem_slot, K::TMEM_COLS);
+        else tmem_alloc(&ms.tmem_slot, K::TMEM_COLS);
+    }
+    if (warp == 2) {                             /* first row tile of every expert */
+        int run = 0;
+        for (int e0 = 0; e0 < p.experts; e0 += 32) {
+            const int e = e0 + lane;
+            int t = 0;
+            if (e < p.experts) {
+                const int rows = MODE == EXP_GRADW ? p.J
+                    : max(expert_start(p.offsets, e + 1, p.m) - expert_start(p.offsets, e, p.m), 0);
+                t = (rows + BN - 1) / BN;
+            }
+            int incl = t;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += v;
+            }
+            if (e < p.experts) start[e] = run + incl - t;
+            run += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        if (lane == 0) start[p.experts] = run;
+    }
+    tc_fence_before();
+    if (PAIR) cluster_sync();
+    else __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = ms.tmem_slot;
+    Tiles<MODE, BN, K::FT> tiles(p, start);
+    const long long total = tiles.total();
+
+    if (warp == 0) {
+        /* ------------------------------------------------- producer ---- */
+        uint32_t last[STAGES];
+#pragma unroll
+        for (int i = 0; i < STAGES; ++i) last[i] = 0xffffffffu;
+        uint32_t it = 0;
+        bool ok = true;
+        auto rows_of = [&](int r, int end, int (&idx)[4], int past, bool gather) {
+            /* token rows (or the sorted rows themselves) of sorted rows r .. r + 3; past where there is none */
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                idx[i] = past;
+                if (r + i < end) {
+                    if (gather) {
+                        const int entry = p.order[r + i];
+                        if ((unsigned)entry < (unsigned)p.m) idx[i] = entry / p.top_k;
+                    } else {
+                        idx[i] = r + i;
+                    }
+                }
+            }
+        };
+        for (long long u = u0; u < total && ok; u += ustep) {
+            const Tile t = tiles.at(u);
+            const int f0 = t.f0 + rank * BM;                     /* this CTA's f's */
+            const int jl = t.j0 + rank * BL;                     /* and j's */
+            const int end = t.r0 + t.rows;
+            int idx[4];
+            if (MODE == EXP_FWD && p.order && lane < BL / 4) {
+                /* the rows past the segment repeat its first: any row will do */
+                rows_of(t.r0 + jl + 4 * lane, end, idx, -1, true);
+                const int first = p.order[t.r0];
+                const int some = (unsigned)first < (unsigned)p.m ? first / p.top_k : p.xrows;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (idx[i] < 0) idx[i] = some;
+            }
+            /* GRADW: lane l fetches rows 4 (l mod 16) .. of the 64-element chunk l / 16 */
+            const int q4 = 4 * (lane & 15), ch = lane >> 4;
+            if (MODE == EXP_GRADW && t.nk > 0) rows_of(t.r0 + q4, end, idx, p.xrows, p.order != nullptr);
+            for (int kc = 0; kc < t.nk; ++kc, ++it) {
+                const int st = (int)(it % STAGES);
+                const uint32_t use = it / STAGES;
+                if (!wait_warp(&ms.empty[st], (use & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+                uint8_t* sa = smem + st * STAGE;
+                uint8_t* sb = sa + A_STAGE;
+                uint64_t* bar = &ms.full[st];
+                const uint32_t pbar = PAIR ? peer_addr(bar, 0) : 0u;
+                if (lane == 0) {
+                    if (!PAIR) mbar_expect_tx(bar, STAGE);
+                    else if (rank == 0) mbar_expect_tx(bar, 2 * STAGE);
+#pragma unroll
+                    for (int i = 0; i < STAGES; ++i)
+                        if (i == st) last[i] = use;
+                }
+                __syncwarp();
+                auto load3 = [&](const CUtensorMap* map, void* dst, int x, int y, int z) {
+                    if (PAIR) tma_load_3d_pair(map, pbar, dst, x, y, z);
+                    else tma_load_3d(map, bar, dst, x, y, z);
+                };
+                auto load2 = [&](const CUtensorMap* map, void* dst, int x, int y) {
+                    if (PAIR) tma_load_2d_pair(map, pbar, dst, x, y);
+                    else tma_load_2d(map, bar, dst, x, y);
+                };
+                auto gather = [&](const CUtensorMap* map, void* dst, int x, const int (&r)[4]) {
+                    if (PAIR) tma_gather4_pair(map, pbar, dst, x, r);
+                    else tma_gather4(map, bar, dst, x, r);
+                };
+                if (MODE == EXP_FWD) {
+                    if (lane == 0) load3(&tmA, sa, kc * BK, f0, t.e);
+                    if (p.order) {
+                        if (lane < BL / 4) gather(&tmBg, sb + 512 * lane, kc * BK, idx);
+                    } else if (lane == 0) {
+                        load2(&tmB, sb, kc * BK, t.r0 + jl);
+                    }
+                } else if (MODE == EXP_GRADX) {
+                    if (lane == 0) {
+                        load3(&tmA, sa, f0, kc * BK, t.e);
+                        load3(&tmA, sa + BOX, f0 + 64, kc * BK, t.e);
+                        load2(&tmB, sb, kc * BK, t.r0 + jl);
+                    }
+                } else {
+                    const int r = t.r0 + kc * BK;
+                    const bool whole = r + BK <= end;
+                    if (whole && !p.order) {
+                        if (lane < 2) load2(&tmA, sa + lane * BOX, f0 + 64 * lane, r);
+                    } else {
+                        gather(&tmAg, sa + ch * BOX + q4 * 128, f0 + 64 * ch, idx);
+                    }
+                    if (whole) {
+                        if (lane < BL / 64) load2(&tmB, sb + lane * BOX, jl + 64 * lane, r);
+                    } else {
+                        int own[4];
+                        rows_of(r + q4, end, own, p.m, false);
+                        if (ch < BL / 64) gather(&tmBg, sb + ch * BOX + q4 * 128, jl + 64 * ch, own);
+                    }
+                    rows_of(r + BK + q4, end, idx, p.xrows, p.order != nullptr);
+                }
+            }
+        }
+        if (!ok && lane == 0) {
+            if (!PAIR) {
+#pragma unroll
+                for (int i = 0; i < STAGES; ++i)
+                    if (last[i] != 0xffffffffu) drain_wait(&ms.full[i], last[i] & 1u);
+            } else {
+                /* a pair's loads complete on CTA 0's barriers, and a phase that was never armed does not
+                 * complete: give every load in flight a fixed time (each takes microseconds) */
+                const unsigned long long t_end = globaltimer() + 20000000ull;
+                while (globaltimer() < t_end) {
+                }
+            }
+        }
+    } else if (warp == 1) {
+        /* ------------------------------------------------- MMA issuer --- */
+        if (lane == 0 && rank == 0) {
+            constexpr uint32_t idesc = idesc_f16(PAIR ? 2 * BM : BM, BN, FMT, A_MN ? 1 : 0, B_MN ? 1 : 0);
+            auto commit = [&](uint64_t* bar) {
+                if (PAIR) {
+                    umma_commit_pair(peer_addr(bar, 0));
+                    umma_commit_pair(peer_addr(bar, 1));
+                } else {
+                    umma_commit(bar);
+                }
+            };
+            uint32_t it = 0, ts = 0;
+            bool ok = true;
+            for (long long u = u0; u < total && ok; u += ustep) {
+                const Tile t = tiles.at(u);
+                if (t.nk == 0) continue;
+                const int tb = (int)(ts & 1u);
+                if (!mbar_wait(&ms.t_empty[tb], ((ts >> 1) & 1u) ^ 1u, abort_flag, &g_experts_status)) { ok = false; break; }
+                tc_fence_after();
+                const uint32_t d_tmem = tmem_base + (uint32_t)(tb * BN);
+                for (int kc = 0; kc < t.nk; ++kc, ++it) {
+                    const int st = (int)(it % STAGES);
+                    if (!mbar_wait(&ms.full[st], (it / STAGES) & 1u, abort_flag, &g_experts_status)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t sa = smem_u32(smem + st * STAGE);
+                    const uint32_t sb = sa + A_STAGE;
+#pragma unroll
+                    for (int ks = 0; ks < BK / 16; ++ks) {
+                        const uint64_t ad = A_MN ? sw128_desc(sa + ks * 2048, BOX, 1024) : sw128_desc(sa + ks * 32, 16, 1024);
+                        const uint64_t bd = B_MN ? sw128_desc(sb + ks * 2048, BOX, 1024) : sw128_desc(sb + ks * 32, 16, 1024);
+                        const uint32_t acc = (kc > 0 || ks > 0) ? 1u : 0u;
+                        if (PAIR) umma_f16_pair(d_tmem, ad, bd, idesc, acc);
+                        else umma_f16(d_tmem, ad, bd, idesc, acc);
+                    }
+                    commit(&ms.empty[st]);
+                }
+                if (ok) commit(&ms.t_full[tb]);
+                ++ts;
+            }
+            if (PAIR) umma_commit_pair(peer_addr(&ms.fin, 0));
+            else umma_commit(&ms.fin);
+            drain_wait(&ms.fin, 0);
+        }
+    } else {
+        /* --------------------------------------------------- epilogue --- */
+        constexpr int CH = K::CH;
+        const int half = (warp - 2) >> 2;         /* which columns of the tile */
+        const int q = warp & 3;                   /* TMEM lane quarter */
+        const uint32_t t_lane = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * K::HALF);
+        const bool odd = lane & 1;
+        const uint32_t sel = odd ? 0x3276u : 0x5410u;
+        uint16_t* out = static_cast<uint16_t*>(p.out);
+        bool ok = true;
+        uint32_t ts = 0;
+        for (long long u = u0; u < total; u += ustep) {
+            const Tile t = tiles.at(u);
+            const int tb = (int)(ts & 1u);
+            if (t.nk > 0) {
+                if (ok) ok = wait_warp(&ms.t_full[tb], (ts >> 1) & 1u, abort_flag);
+                ++ts;
+                if (!ok) continue;
+                tc_fence_after();
+            }
+            const int f = t.f0 + rank * BM + q * 32 + lane;
+            uint16_t* base = MODE == EXP_GRADW ? out + (long long)t.e * p.stride_o + (long long)t.j0 * p.ldo
+                                               : out + (long long)(t.r0 + t.j0) * p.ldo;
+            const int nj = t.nj - half * K::HALF;                /* columns of this warp that exist */
+            base += (long long)(half * K::HALF) * p.ldo;
+#pragma unroll 1
+            for (int c = 0; c < K::HALF; c += CH) {
+                if (c >= nj) break;
+                uint32_t r[CH];
+                if (t.nk > 0) {
+                    if constexpr (CH == 32) tmem_ld32(t_lane + (uint32_t)(tb * BN + c), r);
+                    else tmem_ld16(t_lane + (uint32_t)(tb * BN + c), r);
+                    tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int e = 0; e < CH; ++e) r[e] = 0u;
+                }
+                if (p.pairs) {
+                    const int fe = f - (odd ? 1 : 0);
+                    uint16_t* dst = base + (long long)(c + (odd ? 1 : 0)) * p.ldo + fe;
+#pragma unroll
+                    for (int e = 0; e < CH; e += 2) {
+                        const uint32_t own = pack2(__uint_as_float(r[e]), __uint_as_float(r[e + 1]), FMT == 1);
+                        const uint32_t other = __shfl_xor_sync(0xffffffffu, own, 1);
+                        const uint32_t v = __byte_perm(own, other, sel);
+                        if (c + e + (odd ? 1 : 0) < nj) {
+                            if (fe + 1 < p.F) *reinterpret_cast<uint32_t*>(dst) = v;
+                            else if (fe < p.F) *dst = (uint16_t)v;
+                        }
+                        dst += 2 * p.ldo;
+                    }
+                } else {
+                    uint16_t* dst = base + (long long)c * p.ldo + f;
+#pragma unroll
+                    for (int e = 0; e < CH; ++e) {
+                        if (c + e < nj && f < p.F) *dst = (uint16_t)pack2(__uint_as_float(r[e]), 0.f, FMT == 1);
+                        dst += p.ldo;
+                    }
+                }
+            }
+            if (t.nk > 0) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (PAIR) mbar_arrive_cluster(peer_addr(&ms.t_empty[tb], 0));
+                    else mbar_arrive(&ms.t_empty[tb]);
+                }
+            }
+        }
+        if (MODE != EXP_GRADW) {                  /* rows that no expert owns */
+            const int valid = expert_start(p.offsets, p.experts, p.m);
+            const int tid = threadIdx.x - 64;
+            for (long long r = valid + (long long)blockIdx.x; r < p.m; r += gridDim.x)
+                for (int f = tid; f < p.F; f += 32 * kEpiWarps) out[r * p.ldo + f] = 0;
+        }
+    }
+
+    tc_fence_before();
+    if (PAIR) cluster_sync();
+    else __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        if (PAIR) tmem_dealloc_pair(tmem_base, K::TMEM_COLS);
+        else tmem_dealloc(tmem_base, K::TMEM_COLS);
+    }
+}
+
+/* ------------------------------------------------------------- host side ---- */
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* q = nullptr;
+        cudaDriverEntryPointQueryResult res;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &q, 12000, cudaEnableDefault, &res) == cudaSuccess &&
+            res == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(q);
+    });
+    return fn;
+}
+
+/* rows x cols (x planes) with row stride ld and plane stride, 64-element boxes of box_rows rows. */
+bool row_map(CUtensorMap* map, const void* base, bool bf16, long long cols, long long rows, long long planes, long long ld,
+             long long stride, int box_rows) {
+    auto fn = encode_fn();
+    if (!fn) return false;
+    if (rows <= 1) ld = (cols + 7) / 8 * 8;
+    if (planes <= 1) stride = ld;                /* no step is ever taken along it */
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
+    const cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)stride * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
+    const cuuint32_t es[3] = {1, 1, 1};
+    return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, planes ? 3 : 2,
+              const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int MODE, int BN, bool PAIR, int FMT>
+cudaError_t launch_t(const ExpertArgs& a, cudaStream_t s) {
+    using K = Cfg<BN, PAIR>;
+    auto kern = k_experts_tc<MODE, BN, PAIR, FMT>;
+    const bool gather = a.order != nullptr;
+    const long long xrows = gather ? a.m / a.top_k : a.m;
+    CUtensorMap tmA{}, tmB{}, tmAg{}, tmBg{};
+    bool ok;
+    if (MODE == EXP_FWD) {
+        ok = row_map(&tmA, a.w, a.bf16, a.k, a.width, a.experts, a.ldw, a.stride_w, BM);
+        ok = ok && (gather ? row_map(&tmBg, a.x, a.bf16, a.k, xrows, 0, a.ldx, 0, 1)
+                           : row_map(&tmB, a.x, a.bf16, a.k, xrows, 0, a.ldx, 0, K::BL));
+    } else if (MODE == EXP_GRADX) {
+        ok = row_map(&tmA, a.w, a.bf16, a.k, a.width, a.experts, a.ldw, a.stride_w, BK) &&
+             row_map(&tmB, a.gy, a.bf16, a.width, a.m, 0, a.ldgy, 0, K::BL);
+    } else {
+        ok = row_map(&tmA, a.x, a.bf16, a.k, xrows, 0, a.ldx, 0, BK) && row_map(&tmAg, a.x, a.bf16, a.k, xrows, 0, a.ldx, 0, 1) &&
+             row_map(&tmB, a.gy, a.bf16, a.width, a.m, 0, a.ldgy, 0, BK) &&
+             row_map(&tmBg, a.gy, a.bf16, a.width, a.m, 0, a.ldgy, 0, 1);
+    }
+    if (!ok) return cudaErrorInvalidValue;
+    Params p{a.offsets, a.order, a.top_k, (int)a.m, a.experts, (int)xrows, MODE == EXP_FWD ? a.width : a.k, a.width,
+             MODE == EXP_FWD ? a.k : a.width, a.out, a.ldo, a.stride_o,
+             reinterpret_cast<uintptr_t>(a.out) % 4 == 0 && a.ldo % 2 == 0 && (MODE != EXP_GRADW || a.stride_o % 2 == 0)};
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, K::SMEM_BYTES);
+    if (e != cudaSuccess) return e;
+    /* the most tiles there can be: every expert with rows rounds up by one */
+    const long long ft = (p.F + K::FT - 1) / K::FT;
+    const long long some = a.m < a.experts ? a.m : a.experts;
+    const long long jt = MODE == EXP_GRADW ? (long long)a.experts * ((a.width + BN - 1) / BN) : a.m / BN + some;
+    const long long units = ft * jt;
+    const long long fit = PAIR ? a.sms / 2 : a.sms;
+    const int n = (int)(units < fit ? units : fit);
+    if (n == 0) return cudaSuccess;
+    if (!PAIR) {
+        kern<<<n, kThreads, K::SMEM_BYTES, s>>>(tmA, tmB, tmAg, tmBg, p);
+        return cudaGetLastError();
+    }
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(2 * n, 1, 1);
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = K::SMEM_BYTES;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, kern, tmA, tmB, tmAg, tmBg, p);
+    return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+template <int MODE, int FMT>
+cudaError_t launch_mode(const ExpertArgs& a, cudaStream_t s) {
+    if (MODE == EXP_GRADW) {
+        if (a.width <= 128 || a.k <= 128) return launch_t<EXP_GRADW, 128, false, FMT>(a, s);
+        return launch_t<EXP_GRADW, 256, true, FMT>(a, s);
+    }
+    const long long rows = a.m / a.experts;      /* of an average expert */
+    if (rows <= 24) return launch_t<MODE, 32, false, FMT>(a, s);
+    if (rows <= 96) return launch_t<MODE, 128, false, FMT>(a, s);
+    return launch_t<MODE, 256, true, FMT>(a, s);
+}
+
+bool rows16(const void* q, long long ld) { return reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld % 8 == 0; }
+
+}  /* namespace */
+
+bool experts_tc_ok(const ExpertArgs& a) {
+    const long long xrows = a.order ? a.m / a.top_k : a.m;
+    const bool x = a.mode == EXP_GRADX || rows16(a.x, xrows > 1 ? a.ldx : 8);
+    const bool gy = a.mode == EXP_FWD || rows16(a.gy, a.m > 1 ? a.ldgy : 8);
+    const bool w = a.mode == EXP_GRADW ||
+                   (rows16(a.w, a.width > 1 ? a.ldw : 8) && (a.experts == 1 || a.stride_w % 8 == 0));
+    /* TMA strides stay below 2^40 bytes */
+    const bool small = a.ldx < (1LL << 38) && a.ldgy < (1LL << 38) && a.ldw < (1LL << 38) && a.stride_w < (1LL << 38);
+    return x && gy && w && small && a.m > 0;
+}
+
+cudaError_t launch_experts_tc(const ExpertArgs& a, cudaStream_t s) {
+    switch (a.mode) {
+        case EXP_FWD: return a.bf16 ? launch_mode<EXP_FWD, 1>(a, s) : launch_mode<EXP_FWD, 0>(a, s);
+        case EXP_GRADX: return a.bf16 ? launch_mode<EXP_GRADX, 1>(a, s) : launch_mode<EXP_GRADX, 0>(a, s);
+        default: return a.bf16 ? launch_mode<EXP_GRADW, 1>(a, s) : launch_mode<EXP_GRADW, 0>(a, s);
+    }
+}
+
+}  /* namespace mpk */
+
+extern "C" int mpkDebugExpertStatus(int clear) {
+    int v = -1;
+    if (cudaMemcpyFromSymbol(&v, mpk::g_experts_status, sizeof(int)) != cudaSuccess) return -1;
+    if (clear) {
+        const int zero = 0;
+        if (cudaMemcpyToSymbol(mpk::g_experts_status, &zero, sizeof(int)) != cudaSuccess) return -1;
+    }
+    return v;
+}

@@ -258,6 +258,13 @@ def product_tolerance(want, magnitude, length, dtype):
     return half_step(dtype) * (np.abs(want) + length * 2 * U32 * magnitude) + length * 2 * U32 * magnitude + least(dtype)
 
 
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    """Every test ends with the products' device status clear."""
+    yield
+    assert M.lib().mpkDebugExpertStatus(1) == 0
+
+
 def setup_products(seed, n, top_k, experts, k, width, dtype, gather, dropped, skew):
     ids = random_ids(seed, n, top_k, experts, dropped, skew)
     plan = M.expert_plan(ids, experts)
