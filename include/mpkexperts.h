@@ -122,17 +122,23 @@ mpkStatus mpkExpertPlan(cudaStream_t stream, const int* dIds, long long n, int t
  * otherwise.  Rows of dY and dGX that no expert owns ([dOffsets[experts], m)) are
  * set to zero; an expert without rows gets a zero gradient.  Nothing past row m
  * and nothing between a row's end and its stride is written.
+ * With dOrder, dWork is scratch of mpkExpertGemmBytes(0 for Gemm, 1 for GradW, ...)
+ * bytes on a 16-byte boundary (a sorted copy of the rows of X; 0 where the
+ * experts have few rows and the product gathers them itself); without, it is not
+ * looked at.
  * width and k in 1 .. 2^20; any alignment of the element type: rows that start
  * on 16-byte boundaries (addresses and strides) run on the tensor cores. */
+size_t mpkExpertGemmBytes(int grad_w, long long m, int experts, int k);
 mpkStatus mpkExpertGemm(cudaStream_t stream, int type, const void* dX, long long ldx, const void* dW, long long ldw,
                         long long strideW, const int* dOffsets, const int* dOrder, int top_k, long long m,
-                        int experts, int width, int k, void* dY, long long ldy);
+                        int experts, int width, int k, void* dY, long long ldy, void* dWork, size_t work_bytes);
 mpkStatus mpkExpertGemmGradX(cudaStream_t stream, int type, const void* dGY, long long ldgy, const void* dW,
                              long long ldw, long long strideW, const int* dOffsets, long long m, int experts,
                              int width, int k, void* dGX, long long ldgx);
 mpkStatus mpkExpertGemmGradW(cudaStream_t stream, int type, const void* dGY, long long ldgy, const void* dX,
                              long long ldx, const int* dOffsets, const int* dOrder, int top_k, long long m,
-                             int experts, int width, int k, void* dGW, long long ldw, long long strideW);
+                             int experts, int width, int k, void* dGW, long long ldw, long long strideW, void* dWork,
+                             size_t work_bytes);
 
 /* dOut[t] = sum over slots s of dWeights[t, s] * dY[dPos[t, s]] (n x width of
  * `type`, FP32 sums in slot order); dWeights NULL: weights of 1 (the gradient of

@@ -216,9 +216,11 @@ SIGNATURES = {
     "mpkRouteGrad": (_I, [_P, _ROUTE, _P, _I, _LL, _LL, _P, _P, _P, _LL]),
     "mpkExpertPlanBytes": (ctypes.c_size_t, [_LL, _I, _I]),
     "mpkExpertPlan": (_I, [_P, _P, _LL, _I, _I, _P, _P, _P, _P, ctypes.c_size_t]),
-    "mpkExpertGemm": (_I, [_P, _I, _P, _LL, _P, _LL, _LL, _P, _P, _I, _LL, _I, _I, _I, _P, _LL]),
+    "mpkExpertGemmBytes": (ctypes.c_size_t, [_I, _LL, _I, _I]),
+    "mpkExpertGemm": (_I, [_P, _I, _P, _LL, _P, _LL, _LL, _P, _P, _I, _LL, _I, _I, _I, _P, _LL, _P, ctypes.c_size_t]),
     "mpkExpertGemmGradX": (_I, [_P, _I, _P, _LL, _P, _LL, _LL, _P, _LL, _I, _I, _I, _P, _LL]),
-    "mpkExpertGemmGradW": (_I, [_P, _I, _P, _LL, _P, _LL, _P, _P, _I, _LL, _I, _I, _I, _P, _LL, _LL]),
+    "mpkExpertGemmGradW": (_I, [_P, _I, _P, _LL, _P, _LL, _P, _P, _I, _LL, _I, _I, _I, _P, _LL, _LL, _P,
+                                ctypes.c_size_t]),
     "mpkExpertCombine": (_I, [_P, _I, _P, _LL, _P, _P, _LL, _I, _I, _P, _LL]),
     "mpkExpertCombineGrad": (_I, [_P, _I, _P, _LL, _P, _LL, _P, _P, _P, _LL, _I, _I, _P, _LL, _P]),
 }
@@ -681,6 +683,15 @@ def expert_plan(ids, experts: int) -> ExpertPlan:
     return ExpertPlan(offsets, order, pos.view(n, top_k))
 
 
+def _sorted_copy(grad_w: int, x, plan: "ExpertPlan", gather: bool) -> tuple:
+    """(scratch tensor or None, its address, its bytes) of a product that gathers x."""
+    need = int(lib().mpkExpertGemmBytes(grad_w, plan.rows, plan.experts, x.shape[1])) if gather else 0
+    if not need:
+        return None, None, 0
+    work = x.new_empty(need // 2)
+    return work, work.data_ptr(), need
+
+
 def expert_gemm(x, w, plan: ExpertPlan, *, gather: bool = True, out=None):
     """Every routed row times its expert's matrix (mpkExpertGemm): out[r] = w[e] x[r].
     w: experts x width x k, FP16 or BF16.  x: n x k token rows (gather) or n * top_k
@@ -693,9 +704,10 @@ def expert_gemm(x, w, plan: ExpertPlan, *, gather: bool = True, out=None):
     if out is None:
         out = torch.empty((plan.rows, width), dtype=x.dtype, device=x.device)
     po, ldo = _matrix("out", out, (x.dtype,), plan.rows, width)
+    work, pwork, need = _sorted_copy(0, x, plan, gather)
     _run("mpkExpertGemm", (x, w, plan.offsets, plan.order, out), _types()[x.dtype], address, ldx, pw, ldw, sw,
          plan.offsets.data_ptr(), plan.order.data_ptr() if gather else None, plan.top_k, plan.rows, plan.experts,
-         width, k, po, ldo)
+         width, k, po, ldo, pwork, need)
     return out
 
 
@@ -727,9 +739,10 @@ def expert_gemm_grad_w(grad, x, plan: ExpertPlan, *, gather: bool = True, out=No
     if out is None:
         out = torch.empty((plan.experts, width, k), dtype=x.dtype, device=x.device)
     po, ldo, so = _matrices("out", out, x.dtype, (plan.experts, width, k))
+    work, pwork, need = _sorted_copy(1, x, plan, gather)
     _run("mpkExpertGemmGradW", (grad, x, plan.offsets, plan.order, out), _types()[x.dtype], pg, ldg, address,
          ldx, plan.offsets.data_ptr(), plan.order.data_ptr() if gather else None, plan.top_k, plan.rows, plan.experts,
-         width, k, po, ldo, so)
+         width, k, po, ldo, so, pwork, need)
     return out
 
 

@@ -5,6 +5,8 @@
 #include "experts.cuh"
 #include "mpkexperts.h"
 
+#include <type_traits>
+
 namespace mpk {
 namespace {
 
@@ -175,6 +177,37 @@ cudaError_t launch_any(const ExpertArgs& a, cudaStream_t s) {
     return cudaGetLastError();
 }
 
+/* ------------------------------------------------------ sorted copy of X ---- */
+
+constexpr int kCopyThreads = 256;
+
+/* out[r] = x[order[r] / top_k] for the sorted rows there are, V elements a copy: a
+ * warp a row, eight copies in flight a lane. */
+template <int V>
+__global__ void __launch_bounds__(kCopyThreads)
+k_sort_rows(const uint16_t* __restrict__ x, long long ldx, const int* __restrict__ order, int top_k, int m, int k,
+            uint16_t* __restrict__ out, long long ldo) {
+    using W = typename std::conditional<V == 8, uint4, uint16_t>::type;
+    const int lane = threadIdx.x & 31;
+    const long long warps = (long long)gridDim.x * (kCopyThreads / 32);
+    const int pieces = (k + V - 1) / V;
+    for (long long r = (long long)blockIdx.x * (kCopyThreads / 32) + (threadIdx.x >> 5); r < m; r += warps) {
+        const int entry = order[r];
+        if ((unsigned)entry >= (unsigned)m) continue;          /* behind the last routed row */
+        const W* src = reinterpret_cast<const W*>(x + (long long)(entry / top_k) * ldx);
+        W* dst = reinterpret_cast<W*>(out + r * ldo);
+        int c = lane;
+        for (; c + 7 * 32 < pieces; c += 8 * 32) {
+            W v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = src[c + 32 * i];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) dst[c + 32 * i] = v[i];
+        }
+        for (; c < pieces; c += 32) dst[c] = src[c];
+    }
+}
+
 /* --------------------------------------------------------------- combine ---- */
 
 /* V consecutive elements of a row, as floats. */
@@ -327,12 +360,44 @@ bool shape_ok(int type, long long m, int experts, int width, int k, bool gather,
            width <= (1 << 20) && k >= 1 && k <= (1 << 20) && (!gather || (top_k >= 1 && m % top_k == 0));
 }
 
-mpkStatus run_product(ExpertArgs& a, cudaStream_t s) {
+/* Row stride of the sorted copy of gathered rows: 16-byte steps. */
+long long copy_ld(int k) { return ((long long)k + 7) / 8 * 8; }
+
+size_t copy_bytes(int mode, long long m, int experts, int k) {
+    return mode == EXP_FWD && experts_few_rows(m, experts) ? 0 : (size_t)m * copy_ld(k) * 2;
+}
+
+/* With a sorted copy the product sees plain sorted rows; the tiled kernel gathers
+ * for itself and takes none. */
+mpkStatus run_product(ExpertArgs& a, void* work, cudaStream_t s) {
     a.sms = sm_count();
     if (!a.sms) return MPK_ERR_CUDA;
-    const cudaError_t e = experts_tc_ok(a) ? launch_experts_tc(a, s)
-                          : a.bf16 ? launch_any<__nv_bfloat16>(a, s) : launch_any<__half>(a, s);
-    return e == cudaSuccess ? MPK_OK : MPK_ERR_CUDA;
+    ExpertArgs sorted = a;
+    if (a.order && copy_bytes(a.mode, a.m, a.experts, a.k)) {
+        sorted.x = work;
+        sorted.ldx = copy_ld(a.k);
+        sorted.order = nullptr;
+    }
+    if (!experts_tc_ok(sorted))
+        return (a.bf16 ? launch_any<__nv_bfloat16>(a, s) : launch_any<__half>(a, s)) == cudaSuccess ? MPK_OK : MPK_ERR_CUDA;
+    if (a.order && !sorted.order) {
+        const long long rows8 = (a.m + kCopyThreads / 32 - 1) / (kCopyThreads / 32), most = (long long)a.sms * 8;
+        const int grid = (int)(rows8 < most ? rows8 : most);
+        const uint16_t* x = static_cast<const uint16_t*>(a.x);
+        uint16_t* out = static_cast<uint16_t*>(work);
+        const long long xrows = a.m / a.top_k;
+        if (a.k % 8 == 0 && aligned16(x, xrows > 1 ? a.ldx : 8, 2))
+            k_sort_rows<8><<<grid, kCopyThreads, 0, s>>>(x, a.ldx, a.order, a.top_k, (int)a.m, a.k, out, sorted.ldx);
+        else
+            k_sort_rows<1><<<grid, kCopyThreads, 0, s>>>(x, a.ldx, a.order, a.top_k, (int)a.m, a.k, out, sorted.ldx);
+        if (cudaGetLastError() != cudaSuccess) return MPK_ERR_CUDA;
+    }
+    return launch_experts_tc(sorted, s) == cudaSuccess ? MPK_OK : MPK_ERR_CUDA;
+}
+
+/* A call's scratch: none asked for, or enough of it on a 16-byte boundary. */
+bool work_ok(size_t need, const void* work, size_t bytes) {
+    return need == 0 || (work && bytes >= need && reinterpret_cast<uintptr_t>(work) % 16 == 0);
 }
 
 template <typename T>
@@ -381,17 +446,24 @@ using namespace mpk;
 
 extern "C" {
 
+size_t mpkExpertGemmBytes(int grad_w, long long m, int experts, int k) {
+    if (m <= 0 || m >= (1LL << 30) || experts < 1 || k < 1 || k > (1 << 20)) return 0;
+    return copy_bytes(grad_w ? EXP_GRADW : EXP_FWD, m, experts, k);
+}
+
 mpkStatus mpkExpertGemm(cudaStream_t stream, int type, const void* dX, long long ldx, const void* dW, long long ldw,
                         long long strideW, const int* dOffsets, const int* dOrder, int top_k, long long m,
-                        int experts, int width, int k, void* dY, long long ldy) {
+                        int experts, int width, int k, void* dY, long long ldy, void* dWork, size_t work_bytes) {
     if (!shape_ok(type, m, experts, width, k, dOrder != nullptr, top_k) || ldx < k || ldw < k || ldy < width ||
         (experts > 1 && strideW < (long long)(width - 1) * ldw + k))
         return MPK_ERR_INVALID;
     if (m == 0) return MPK_OK;
-    if (!dX || !dW || !dOffsets || !dY) return MPK_ERR_INVALID;
+    if (!dX || !dW || !dOffsets || !dY ||
+        (dOrder && !work_ok(copy_bytes(EXP_FWD, m, experts, k), dWork, work_bytes)))
+        return MPK_ERR_INVALID;
     ExpertArgs a{EXP_FWD, type == MPK_TYPE_BF16, dX, ldx, nullptr, 0, dW, ldw, strideW, dOffsets, dOrder, top_k,
                  m, experts, width, k, dY, ldy, 0, 0};
-    return run_product(a, stream);
+    return run_product(a, dWork, stream);
 }
 
 mpkStatus mpkExpertGemmGradX(cudaStream_t stream, int type, const void* dGY, long long ldgy, const void* dW,
@@ -404,19 +476,22 @@ mpkStatus mpkExpertGemmGradX(cudaStream_t stream, int type, const void* dGY, lon
     if (!dGY || !dW || !dOffsets || !dGX) return MPK_ERR_INVALID;
     ExpertArgs a{EXP_GRADX, type == MPK_TYPE_BF16, nullptr, 0, dGY, ldgy, dW, ldw, strideW, dOffsets, nullptr, 1,
                  m, experts, width, k, dGX, ldgx, 0, 0};
-    return run_product(a, stream);
+    return run_product(a, nullptr, stream);
 }
 
 mpkStatus mpkExpertGemmGradW(cudaStream_t stream, int type, const void* dGY, long long ldgy, const void* dX,
                              long long ldx, const int* dOffsets, const int* dOrder, int top_k, long long m,
-                             int experts, int width, int k, void* dGW, long long ldw, long long strideW) {
+                             int experts, int width, int k, void* dGW, long long ldw, long long strideW, void* dWork,
+                             size_t work_bytes) {
     if (!shape_ok(type, m, experts, width, k, dOrder != nullptr, top_k) || ldgy < width || ldx < k || ldw < k ||
         (experts > 1 && strideW < (long long)(width - 1) * ldw + k))
         return MPK_ERR_INVALID;
-    if ((m > 0 && (!dGY || !dX)) || !dOffsets || !dGW) return MPK_ERR_INVALID;
+    if ((m > 0 && (!dGY || !dX)) || !dOffsets || !dGW ||
+        (dOrder && !work_ok(copy_bytes(EXP_GRADW, m, experts, k), dWork, work_bytes)))
+        return MPK_ERR_INVALID;
     ExpertArgs a{EXP_GRADW, type == MPK_TYPE_BF16, dX, ldx, dGY, ldgy, nullptr, 0, 0, dOffsets, dOrder, top_k,
                  m, experts, width, k, dGW, ldw, strideW, 0};
-    return run_product(a, stream);
+    return run_product(a, dWork, stream);
 }
 
 mpkStatus mpkExpertCombine(cudaStream_t stream, int type, const void* dY, long long ldy, const int* dPos,

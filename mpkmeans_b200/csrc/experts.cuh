@@ -30,7 +30,11 @@ struct ExpertArgs {
     int sms;
 };
 
-/* Whether the operands and the output have the layout the tensor-core kernel takes. */
+/* Whether the average expert has so few rows that reading W bounds the product:
+ * such calls gather rows in the product's kernel; all others, and every gradient
+ * of the weights, take X sorted. */
+bool experts_few_rows(long long m, int experts);
+/* Whether the operands have the layout the tensor-core kernel takes. */
 bool experts_tc_ok(const ExpertArgs& a);
 cudaError_t launch_experts_tc(const ExpertArgs& a, cudaStream_t s);
 

@@ -10,27 +10,39 @@
  *   GRADW  k        width          rows   X rows, MN-major       GY rows, MN-major
  *
  * so weights are always the wide operand's source, a short segment of rows costs
- * only a narrow tile (BN = 32 .. 128 for few rows an expert), and every store of
- * a warp runs along f.  The experts' row counts are on the device only: each CTA
- * scans them into shared memory and the grid walks the tiles of all experts.
+ * only a narrow tile, and every store of a warp runs along f.  The experts' row
+ * counts are on the device only: each CTA scans them into shared memory and the
+ * grid walks the tiles of all experts.
  *
- *   warp 0      TMA producer: one 64-deep stage of A and B at a time.  Gathered
- *               rows come by tile::gather4, four token rows a lane, so no sorted
- *               copy of X is written; sorted rows come as plain boxes.
+ *   warp 0      TMA producer: one 64-deep stage of A and B at a time.
  *   warp 1      MMA issuer, whole contraction into one FP32 TMEM accumulator, two
  *               accumulators so that the next tile's MMAs overlap the epilogue.
  *   warps 2-9   epilogue: round to the output type, swap halves between lane
  *               pairs so that a lane holds two neighbouring f, store 4 bytes.
  *
- * PAIR: two CTAs on two SMs share each MMA (cta_group::2, 256 f x 256 j): every
- * CTA stages its 128 f of A and 128 j of B, 32 KB for 256 x 256 x 64 products of
- * the pair, half the operand traffic of one-CTA 128 x 256 tiles.
+ * Many rows an expert (PAIR): two CTAs on two SMs share each MMA (cta_group::2,
+ * 256 f x up to 256 j).  Every CTA stages its 128 f of A and its half of the j's,
+ * 32 KB for 256 x 256 x 64 products of the pair, half the operand traffic of
+ * one-CTA 128 x 256 tiles.  The MMA is only as wide as the tile has rows (rounded
+ * up to 32), so the last tile of a segment costs its share.  X comes sorted: the
+ * caller copies gathered rows first.  (Gathering 128-byte pieces of rows inside
+ * this kernel held 32768 x 4096 by 2048 at 0.80 ms with cp.async and 1.45 ms with
+ * TMA's gather4, 45 ns an instruction; sorted rows take 0.47 ms and the copy
+ * 0.06 ms.)
  *
- * Rows past a segment.  FWD and GRADX read whatever rows follow (a gather repeats
- * the segment's first): a column of the accumulator depends on its own row only
- * and those columns are not stored.  GRADW contracts over the rows, so the last
- * stage of a segment fetches both operands by gather with an index past the
- * tensor for the rows that are not the expert's, which TMA fills with zeros.
+ * Few rows an expert: one CTA, 128 f x 32 j, bound by reading W once, eleven
+ * stages of 20 KB in flight.  Gathered rows come by cp.async in warps 10-15, 16
+ * bytes a copy, into the same swizzled layout.  Warp w fills ring slots w, w + 6,
+ * ...: handing a stage to the tensor cores (proxy fence, arrive) waits for all
+ * copies its warp has in flight, so stages overlap between warps, not within one;
+ * and one warp sees every use of a slot, so it cannot be two phases behind the
+ * slot's barrier, whose parity would then look like the next.
+ *
+ * Rows past a segment.  FWD and GRADX read whatever rows follow (the gather
+ * writes zeros): a column of the accumulator depends on its own row only and those
+ * columns are not stored.  GRADW contracts over the rows, so the last stage of a
+ * segment fetches its rows by gather4 with an index past the tensor for the rows
+ * that are not the expert's, which TMA fills with zeros.
  */
 #include "experts.cuh"
 #include "mpkexperts.h"
@@ -48,15 +60,18 @@ __device__ int g_experts_status;
 
 constexpr int BM = 128, BK = 64;
 constexpr int kEpiWarps = 8;
-constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr int kGatherWarps = 6;
+constexpr int kFewRows = 32;                     /* j's of a tile where experts have few rows */
+constexpr int BROWS = 32;                        /* rows of one K-major box of B */
 constexpr int A_STAGE = BM * BK * 2;             /* 16 KB */
 constexpr int BOX = 64 * 64 * 2;                 /* one 64 x 64 MN-major box */
 constexpr int kSmemMax = 232448;
 constexpr int kMisc = 1024 + 4 * (MPK_MAX_EXPERTS + 1);
 constexpr int kGroup = 8;                        /* row tiles that sweep the f tiles together */
 
-template <int BN, bool PAIR>
+template <bool PAIR>
 struct Cfg {
+    static constexpr int BN = PAIR ? 256 : kFewRows;           /* j's of a tile, at most */
     static constexpr int BL = PAIR ? BN / 2 : BN;              /* j's this CTA stages */
     static constexpr int FT = PAIR ? 2 * BM : BM;              /* f's of one tile */
     static constexpr int B_STAGE = BL * BK * 2;
@@ -64,12 +79,12 @@ struct Cfg {
     static constexpr int RAW = (kSmemMax - kMisc) / STAGE;
     static constexpr int STAGES = RAW > 12 ? 12 : RAW;
     static constexpr int SMEM_BYTES = STAGES * STAGE + kMisc;
-    static constexpr int TMEM_COLS = 2 * BN < 32 ? 32 : 2 * BN;
+    static constexpr int TMEM_COLS = 2 * BN;
     static constexpr int HALF = BN / 2;                        /* columns an epilogue warp */
     static constexpr int CH = HALF < 32 ? HALF : 32;           /* columns of one TMEM load */
-    static_assert(BL <= 128, "one gather4 a lane");
+    static constexpr int THREADS = 64 + 32 * kEpiWarps + (PAIR ? 0 : 32 * kGatherWarps);
     static_assert(CH == 16 || CH == 32, "TMEM load width");
-    static_assert(TMEM_COLS <= 512, "TMEM columns");
+    static_assert(TMEM_COLS >= 32 && TMEM_COLS <= 512, "TMEM columns");
     static_assert(STAGE % 1024 == 0, "swizzle atoms");
 };
 
@@ -83,7 +98,10 @@ struct EMisc {
 struct Params {
     const int* offsets;
     const int* order;           /* gathered rows (NULL: sorted) */
-    int top_k, m, experts, xrows;
+    int top_k, m, experts;
+    const void* x;              /* gathered rows: xcols elements, ldx apart */
+    long long ldx;
+    int xcols;
     int F, J, C;                /* J: GRADW's rows of one expert's output; C: contraction (not GRADW) */
     void* out;
     long long ldo, stride_o;
@@ -92,14 +110,6 @@ struct Params {
 
 /* Four rows of a 2-D tensor map with a one-row box, 64 elements from x each, to
  * 4 x 128 bytes of shared memory (swizzled by address like any other box). */
-__device__ __forceinline__ void tma_gather4(const CUtensorMap* map, uint64_t* bar, void* smem, int x, const int (&r)[4]) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
-        :: "r"(smem_u32(smem)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(r[0]), "r"(r[1]),
-           "r"(r[2]), "r"(r[3])
-        : "memory");
-}
 __device__ __forceinline__ void tma_gather4_pair(const CUtensorMap* map, uint32_t bar, void* smem, int x,
                                                  const int (&r)[4]) {
     asm volatile(
@@ -109,6 +119,13 @@ __device__ __forceinline__ void tma_gather4_pair(const CUtensorMap* map, uint32_
            "r"(r[2]), "r"(r[3])
         : "memory");
 }
+/* 16 bytes of global memory to shared memory, the bytes past `bytes` as zeros (none is read at 0). */
+__device__ __forceinline__ void cp_async16(void* smem, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(smem_u32(smem)), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+/* Orders this thread's writes to shared memory before later reads by TMA and the tensor cores. */
+__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tma_load_2d_pair(const CUtensorMap* map, uint32_t bar, void* smem, int x, int y) {
     asm volatile(
         "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
@@ -134,6 +151,7 @@ struct Tile {
     int e;
     int r0, rows;               /* the expert's sorted rows */
     int j0, nj;                 /* first output row inside the expert, rows of this tile */
+    int wide;                   /* columns of the MMA */
     int f0;
     int nk;                     /* 64-deep contraction steps */
 };
@@ -167,6 +185,7 @@ struct Tiles {
         t.r0 = expert_start(p.offsets, e, p.m);
         t.rows = max(expert_start(p.offsets, e + 1, p.m) - t.r0, 0);
         t.nj = min(BN, (MODE == EXP_GRADW ? p.J : t.rows) - t.j0);
+        t.wide = min(BN, (t.nj + 31) & ~31);
         t.nk = ((MODE == EXP_GRADW ? t.rows : p.C) + BK - 1) / BK;
         return t;
     }
@@ -179,13 +198,15 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, bool bf16) {
     return r;
 }
 
-template <int MODE, int BN, bool PAIR, int FMT>
-__global__ void __launch_bounds__(kThreads, 1)
+template <int MODE, bool PAIR, int FMT>
+__global__ void __launch_bounds__(Cfg<PAIR>::THREADS, 1)
 k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
              const __grid_constant__ CUtensorMap tmAg, const __grid_constant__ CUtensorMap tmBg, const Params p) {
-    using K = Cfg<BN, PAIR>;
-    constexpr int STAGES = K::STAGES, STAGE = K::STAGE, BL = K::BL;
+    static_assert(PAIR || MODE != EXP_GRADW, "the weights' gradient runs on pairs");
+    using K = Cfg<PAIR>;
+    constexpr int STAGES = K::STAGES, STAGE = K::STAGE, BN = K::BN, BL = K::BL;
     constexpr bool A_MN = MODE != EXP_FWD, B_MN = MODE == EXP_GRADW;
+    const bool gathers = !PAIR && p.order != nullptr;
     static_assert(sizeof(EMisc<STAGES>) <= 1024, "misc");
     extern __shared__ __align__(1024) uint8_t smem[];
     EMisc<STAGES>& ms = *reinterpret_cast<EMisc<STAGES>*>(smem + STAGES * STAGE);
@@ -200,7 +221,9 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
         return;
     }
     if (threadIdx.x == 0) {
-        for (int i = 0; i < STAGES; ++i) { mbar_init(&ms.full[i], 1); mbar_init(&ms.empty[i], 1); }
+        /* a stage is full with the TMA bytes and, where rows are gathered, the gather warp's arrival */
+        const int arrivals = gathers ? 2 : 1;
+        for (int i = 0; i < STAGES; ++i) { mbar_init(&ms.full[i], arrivals); mbar_init(&ms.empty[i], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&ms.t_full[i], 1); mbar_init(&ms.t_empty[i], (PAIR ? 2 : 1) * kEpiWarps); }
         mbar_init(&ms.fin, 1);
         ms.abort_flag = 0;
@@ -246,39 +269,16 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
         for (int i = 0; i < STAGES; ++i) last[i] = 0xffffffffu;
         uint32_t it = 0;
         bool ok = true;
-        auto rows_of = [&](int r, int end, int (&idx)[4], int past, bool gather) {
-            /* token rows (or the sorted rows themselves) of sorted rows r .. r + 3; past where there is none */
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                idx[i] = past;
-                if (r + i < end) {
-                    if (gather) {
-                        const int entry = p.order[r + i];
-                        if ((unsigned)entry < (unsigned)p.m) idx[i] = entry / p.top_k;
-                    } else {
-                        idx[i] = r + i;
-                    }
-                }
-            }
-        };
         for (long long u = u0; u < total && ok; u += ustep) {
             const Tile t = tiles.at(u);
             const int f0 = t.f0 + rank * BM;                     /* this CTA's f's */
-            const int jl = t.j0 + rank * BL;                     /* and j's */
+            const int jn = PAIR ? t.wide / 2 : BN;               /* and j's */
+            const int jl = t.j0 + rank * jn;
             const int end = t.r0 + t.rows;
-            int idx[4];
-            if (MODE == EXP_FWD && p.order && lane < BL / 4) {
-                /* the rows past the segment repeat its first: any row will do */
-                rows_of(t.r0 + jl + 4 * lane, end, idx, -1, true);
-                const int first = p.order[t.r0];
-                const int some = (unsigned)first < (unsigned)p.m ? first / p.top_k : p.xrows;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (idx[i] < 0) idx[i] = some;
-            }
-            /* GRADW: lane l fetches rows 4 (l mod 16) .. of the 64-element chunk l / 16 */
+            const int boxes = MODE == EXP_GRADW ? (jn + 63) / 64 : (jn + BROWS - 1) / BROWS;
+            uint32_t bytes = A_STAGE + (gathers ? 0 : boxes * (MODE == EXP_GRADW ? BOX : BROWS * BK * 2));
+            /* GRADW's last stage: lane l fetches rows 4 (l mod 16) .. of the 64-element chunk l / 16 */
             const int q4 = 4 * (lane & 15), ch = lane >> 4;
-            if (MODE == EXP_GRADW && t.nk > 0) rows_of(t.r0 + q4, end, idx, p.xrows, p.order != nullptr);
             for (int kc = 0; kc < t.nk; ++kc, ++it) {
                 const int st = (int)(it % STAGES);
                 const uint32_t use = it / STAGES;
@@ -288,8 +288,8 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
                 uint64_t* bar = &ms.full[st];
                 const uint32_t pbar = PAIR ? peer_addr(bar, 0) : 0u;
                 if (lane == 0) {
-                    if (!PAIR) mbar_expect_tx(bar, STAGE);
-                    else if (rank == 0) mbar_expect_tx(bar, 2 * STAGE);
+                    if (!PAIR) mbar_expect_tx(bar, bytes);
+                    else if (rank == 0) mbar_expect_tx(bar, 2 * bytes);
 #pragma unroll
                     for (int i = 0; i < STAGES; ++i)
                         if (i == st) last[i] = use;
@@ -303,39 +303,29 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
                     if (PAIR) tma_load_2d_pair(map, pbar, dst, x, y);
                     else tma_load_2d(map, bar, dst, x, y);
                 };
-                auto gather = [&](const CUtensorMap* map, void* dst, int x, const int (&r)[4]) {
-                    if (PAIR) tma_gather4_pair(map, pbar, dst, x, r);
-                    else tma_gather4(map, bar, dst, x, r);
-                };
-                if (MODE == EXP_FWD) {
-                    if (lane == 0) load3(&tmA, sa, kc * BK, f0, t.e);
-                    if (p.order) {
-                        if (lane < BL / 4) gather(&tmBg, sb + 512 * lane, kc * BK, idx);
-                    } else if (lane == 0) {
-                        load2(&tmB, sb, kc * BK, t.r0 + jl);
-                    }
-                } else if (MODE == EXP_GRADX) {
+                if (MODE != EXP_GRADW) {
                     if (lane == 0) {
-                        load3(&tmA, sa, f0, kc * BK, t.e);
-                        load3(&tmA, sa + BOX, f0 + 64, kc * BK, t.e);
-                        load2(&tmB, sb, kc * BK, t.r0 + jl);
+                        if (MODE == EXP_FWD) {
+                            load3(&tmA, sa, kc * BK, f0, t.e);
+                        } else {
+                            load3(&tmA, sa, f0, kc * BK, t.e);
+                            load3(&tmA, sa + BOX, f0 + 64, kc * BK, t.e);
+                        }
                     }
+                    if (!gathers && lane < boxes)
+                        load2(&tmB, sb + lane * (BROWS * BK * 2), kc * BK, t.r0 + jl + BROWS * lane);
                 } else {
                     const int r = t.r0 + kc * BK;
-                    const bool whole = r + BK <= end;
-                    if (whole && !p.order) {
+                    if (r + BK <= end) {
                         if (lane < 2) load2(&tmA, sa + lane * BOX, f0 + 64 * lane, r);
-                    } else {
-                        gather(&tmAg, sa + ch * BOX + q4 * 128, f0 + 64 * ch, idx);
-                    }
-                    if (whole) {
-                        if (lane < BL / 64) load2(&tmB, sb + lane * BOX, jl + 64 * lane, r);
+                        if (lane < boxes) load2(&tmB, sb + lane * BOX, jl + 64 * lane, r);
                     } else {
                         int own[4];
-                        rows_of(r + q4, end, own, p.m, false);
-                        if (ch < BL / 64) gather(&tmBg, sb + ch * BOX + q4 * 128, jl + 64 * ch, own);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) own[i] = r + q4 + i < end ? r + q4 + i : p.m;
+                        tma_gather4_pair(&tmAg, pbar, sa + ch * BOX + q4 * 128, f0 + 64 * ch, own);
+                        if (ch < boxes) tma_gather4_pair(&tmBg, pbar, sb + ch * BOX + q4 * 128, jl + 64 * ch, own);
                     }
-                    rows_of(r + BK + q4, end, idx, p.xrows, p.order != nullptr);
                 }
             }
         }
@@ -355,7 +345,6 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
     } else if (warp == 1) {
         /* ------------------------------------------------- MMA issuer --- */
         if (lane == 0 && rank == 0) {
-            constexpr uint32_t idesc = idesc_f16(PAIR ? 2 * BM : BM, BN, FMT, A_MN ? 1 : 0, B_MN ? 1 : 0);
             auto commit = [&](uint64_t* bar) {
                 if (PAIR) {
                     umma_commit_pair(peer_addr(bar, 0));
@@ -373,6 +362,7 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
                 if (!mbar_wait(&ms.t_empty[tb], ((ts >> 1) & 1u) ^ 1u, abort_flag, &g_experts_status)) { ok = false; break; }
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + (uint32_t)(tb * BN);
+                const uint32_t idesc = idesc_f16(PAIR ? 2 * BM : BM, t.wide, FMT, A_MN ? 1 : 0, B_MN ? 1 : 0);
                 for (int kc = 0; kc < t.nk; ++kc, ++it) {
                     const int st = (int)(it % STAGES);
                     if (!mbar_wait(&ms.full[st], (it / STAGES) & 1u, abort_flag, &g_experts_status)) { ok = false; break; }
@@ -395,6 +385,60 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
             if (PAIR) umma_commit_pair(peer_addr(&ms.fin, 0));
             else umma_commit(&ms.fin);
             drain_wait(&ms.fin, 0);
+        }
+    } else if (warp >= 2 + kEpiWarps) {
+        /* ----------------------------------------------------- gather --- */
+        /* Warp w copies the stages of its ring slots on its own.  Lane l copies the 16-byte piece c = l mod
+         * 8 of rows l / 8, l / 8 + 4, ...: eight pieces make the 128 bytes a row has in a stage, at place c ^
+         * (row mod 8) of them. */
+        if constexpr (MODE == EXP_FWD && !PAIR) if (gathers) {
+            constexpr int N = BL / 4;                            /* rows a lane */
+            static_assert(BL == 32, "a lane looks one row up");
+            const int w = warp - (2 + kEpiWarps);
+            static_assert(STAGES >= kGatherWarps, "every gather warp has a slot");
+            /* the next stage in one of this warp's slots */
+            auto after = [&](uint32_t it) {
+                const int st = (int)(it % STAGES);
+                return it + (uint32_t)(st + kGatherWarps < STAGES ? kGatherWarps : STAGES - st + w);
+            };
+            const int c = lane & 7, row = lane >> 3;
+            const uint16_t* x = static_cast<const uint16_t*>(p.x);
+            uint32_t it0 = 0, it = (uint32_t)w;                  /* first stage of the tile; this warp's next */
+            bool ok = true;
+            int idx[N];
+            for (long long u = u0; u < total && ok; u += ustep) {
+                const Tile t = tiles.at(u);
+                const int end = t.r0 + t.rows;
+                const uint32_t it1 = it0 + (uint32_t)t.nk;
+                if (it < it1) {                                  /* token rows, -1 past the segment */
+                    const int at = t.r0 + t.j0 + lane;
+                    const int entry = at < end ? p.order[at] : -1;
+                    const int own = (unsigned)entry < (unsigned)p.m ? entry / p.top_k : -1;
+#pragma unroll
+                    for (int i = 0; i < N; ++i) idx[i] = __shfl_sync(0xffffffffu, own, 4 * i + row);
+                }
+                for (; it < it1; it = after(it)) {
+                    const int kc = (int)(it - it0);
+                    const int st = (int)(it % STAGES);
+                    if (!wait_warp(&ms.empty[st], ((it / STAGES) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+                    uint8_t* dst = smem + st * STAGE + A_STAGE;
+                    const int col = kc * BK + 8 * c;
+                    const int bytes = min(16, max(0, 2 * (p.xcols - col)));
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        const int r = row + 4 * i;
+                        const bool there = idx[i] >= 0 && bytes > 0;
+                        cp_async16(dst + r * 128 + ((c ^ (r & 7)) << 4),
+                                   there ? x + (long long)idx[i] * p.ldx + col : x, there ? bytes : 0);
+                    }
+                    cp_async_wait_all();
+                    fence_async_proxy();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&ms.full[st]);
+                }
+                it0 = it1;
+            }
+            cp_async_wait_all();
         }
     } else {
         /* --------------------------------------------------- epilogue --- */
@@ -514,28 +558,26 @@ bool row_map(CUtensorMap* map, const void* base, bool bf16, long long cols, long
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int MODE, int BN, bool PAIR, int FMT>
+template <int MODE, bool PAIR, int FMT>
 cudaError_t launch_t(const ExpertArgs& a, cudaStream_t s) {
-    using K = Cfg<BN, PAIR>;
-    auto kern = k_experts_tc<MODE, BN, PAIR, FMT>;
-    const bool gather = a.order != nullptr;
-    const long long xrows = gather ? a.m / a.top_k : a.m;
+    using K = Cfg<PAIR>;
+    constexpr int BN = K::BN;
+    auto kern = k_experts_tc<MODE, PAIR, FMT>;
     CUtensorMap tmA{}, tmB{}, tmAg{}, tmBg{};
     bool ok;
     if (MODE == EXP_FWD) {
-        ok = row_map(&tmA, a.w, a.bf16, a.k, a.width, a.experts, a.ldw, a.stride_w, BM);
-        ok = ok && (gather ? row_map(&tmBg, a.x, a.bf16, a.k, xrows, 0, a.ldx, 0, 1)
-                           : row_map(&tmB, a.x, a.bf16, a.k, xrows, 0, a.ldx, 0, K::BL));
+        ok = row_map(&tmA, a.w, a.bf16, a.k, a.width, a.experts, a.ldw, a.stride_w, BM) &&
+             (a.order || row_map(&tmB, a.x, a.bf16, a.k, a.m, 0, a.ldx, 0, BROWS));
     } else if (MODE == EXP_GRADX) {
         ok = row_map(&tmA, a.w, a.bf16, a.k, a.width, a.experts, a.ldw, a.stride_w, BK) &&
-             row_map(&tmB, a.gy, a.bf16, a.width, a.m, 0, a.ldgy, 0, K::BL);
+             row_map(&tmB, a.gy, a.bf16, a.width, a.m, 0, a.ldgy, 0, BROWS);
     } else {
-        ok = row_map(&tmA, a.x, a.bf16, a.k, xrows, 0, a.ldx, 0, BK) && row_map(&tmAg, a.x, a.bf16, a.k, xrows, 0, a.ldx, 0, 1) &&
+        ok = row_map(&tmA, a.x, a.bf16, a.k, a.m, 0, a.ldx, 0, BK) && row_map(&tmAg, a.x, a.bf16, a.k, a.m, 0, a.ldx, 0, 1) &&
              row_map(&tmB, a.gy, a.bf16, a.width, a.m, 0, a.ldgy, 0, BK) &&
              row_map(&tmBg, a.gy, a.bf16, a.width, a.m, 0, a.ldgy, 0, 1);
     }
     if (!ok) return cudaErrorInvalidValue;
-    Params p{a.offsets, a.order, a.top_k, (int)a.m, a.experts, (int)xrows, MODE == EXP_FWD ? a.width : a.k, a.width,
+    Params p{a.offsets, a.order, a.top_k, (int)a.m, a.experts, a.x, a.ldx, a.k, MODE == EXP_FWD ? a.width : a.k, a.width,
              MODE == EXP_FWD ? a.k : a.width, a.out, a.ldo, a.stride_o,
              reinterpret_cast<uintptr_t>(a.out) % 4 == 0 && a.ldo % 2 == 0 && (MODE != EXP_GRADW || a.stride_o % 2 == 0)};
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, K::SMEM_BYTES);
@@ -549,7 +591,7 @@ cudaError_t launch_t(const ExpertArgs& a, cudaStream_t s) {
     const int n = (int)(units < fit ? units : fit);
     if (n == 0) return cudaSuccess;
     if (!PAIR) {
-        kern<<<n, kThreads, K::SMEM_BYTES, s>>>(tmA, tmB, tmAg, tmBg, p);
+        kern<<<n, K::THREADS, K::SMEM_BYTES, s>>>(tmA, tmB, tmAg, tmBg, p);
         return cudaGetLastError();
     }
     cudaLaunchConfig_t cfg = {};
@@ -559,7 +601,7 @@ cudaError_t launch_t(const ExpertArgs& a, cudaStream_t s) {
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3(2 * n, 1, 1);
-    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.blockDim = dim3(K::THREADS, 1, 1);
     cfg.dynamicSmemBytes = K::SMEM_BYTES;
     cfg.stream = s;
     cfg.attrs = attr;
@@ -568,39 +610,33 @@ cudaError_t launch_t(const ExpertArgs& a, cudaStream_t s) {
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 
-template <int MODE, int FMT>
-cudaError_t launch_mode(const ExpertArgs& a, cudaStream_t s) {
-    if (MODE == EXP_GRADW) {
-        if (a.width <= 128 || a.k <= 128) return launch_t<EXP_GRADW, 128, false, FMT>(a, s);
-        return launch_t<EXP_GRADW, 256, true, FMT>(a, s);
-    }
-    const long long rows = a.m / a.experts;      /* of an average expert */
-    if (rows <= 24) return launch_t<MODE, 32, false, FMT>(a, s);
-    if (rows <= 96) return launch_t<MODE, 128, false, FMT>(a, s);
-    return launch_t<MODE, 256, true, FMT>(a, s);
+template <int FMT>
+cudaError_t launch_fmt(const ExpertArgs& a, cudaStream_t s) {
+    if (a.mode == EXP_GRADW) return launch_t<EXP_GRADW, true, FMT>(a, s);
+    if (experts_few_rows(a.m, a.experts))
+        return a.mode == EXP_FWD ? launch_t<EXP_FWD, false, FMT>(a, s) : launch_t<EXP_GRADX, false, FMT>(a, s);
+    return a.mode == EXP_FWD ? launch_t<EXP_FWD, true, FMT>(a, s) : launch_t<EXP_GRADX, true, FMT>(a, s);
 }
 
 bool rows16(const void* q, long long ld) { return reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld % 8 == 0; }
 
 }  /* namespace */
 
+bool experts_few_rows(long long m, int experts) { return m / experts <= 24; }
+
 bool experts_tc_ok(const ExpertArgs& a) {
+    /* TMA addresses and strides: 16-byte steps, strides below 2^40 bytes; one row has no stride */
+    const long long most = 1LL << 38;
     const long long xrows = a.order ? a.m / a.top_k : a.m;
     const bool x = a.mode == EXP_GRADX || rows16(a.x, xrows > 1 ? a.ldx : 8);
     const bool gy = a.mode == EXP_FWD || rows16(a.gy, a.m > 1 ? a.ldgy : 8);
     const bool w = a.mode == EXP_GRADW ||
                    (rows16(a.w, a.width > 1 ? a.ldw : 8) && (a.experts == 1 || a.stride_w % 8 == 0));
-    /* TMA strides stay below 2^40 bytes */
-    const bool small = a.ldx < (1LL << 38) && a.ldgy < (1LL << 38) && a.ldw < (1LL << 38) && a.stride_w < (1LL << 38);
-    return x && gy && w && small && a.m > 0;
+    return x && gy && w && a.ldx < most && a.ldgy < most && a.ldw < most && a.stride_w < most && a.m > 0;
 }
 
 cudaError_t launch_experts_tc(const ExpertArgs& a, cudaStream_t s) {
-    switch (a.mode) {
-        case EXP_FWD: return a.bf16 ? launch_mode<EXP_FWD, 1>(a, s) : launch_mode<EXP_FWD, 0>(a, s);
-        case EXP_GRADX: return a.bf16 ? launch_mode<EXP_GRADX, 1>(a, s) : launch_mode<EXP_GRADX, 0>(a, s);
-        default: return a.bf16 ? launch_mode<EXP_GRADW, 1>(a, s) : launch_mode<EXP_GRADW, 0>(a, s);
-    }
+    return a.bf16 ? launch_fmt<1>(a, s) : launch_fmt<0>(a, s);
 }
 
 }  /* namespace mpk */

@@ -79,18 +79,19 @@ def refused(fn, good, changes):
 
 
 def test_products_refuse():
-    # stream, type, X, ldx, W, ldw, strideW, offsets, order, top_k, m, experts, width, k, Y, ldy
-    refused("mpkExpertGemm", [None, 2, FAKE, 64, FAKE, 64, 64 * 32, FAKE, FAKE, 2, 8, 4, 32, 64, FAKE, 32],
+    # stream, type, X, ldx, W, ldw, strideW, offsets, order, top_k, m, experts, width, k, Y, ldy, work, bytes
+    refused("mpkExpertGemm", [None, 2, FAKE, 64, FAKE, 64, 64 * 32, FAKE, FAKE, 2, 800, 4, 32, 64, FAKE, 32, FAKE, 1 << 30],
             [(1, 0), (1, 3), (2, None), (3, 63), (4, None), (5, 63), (6, 64 * 32 - 1), (7, None), (9, 0), (9, 3),
-             (10, -1), (10, 1 << 30), (11, 0), (11, 1025), (12, 0), (12, (1 << 20) + 1), (13, 0), (14, None), (15, 31)])
+             (10, -1), (10, 1 << 30), (11, 0), (11, 1025), (12, 0), (12, (1 << 20) + 1), (13, 0), (14, None), (15, 31), (16, None), (16, 4104), (17, 800 * 64 * 2 - 1)])
     # stream, type, GY, ldgy, W, ldw, strideW, offsets, m, experts, width, k, GX, ldgx
     refused("mpkExpertGemmGradX", [None, 1, FAKE, 32, FAKE, 64, 64 * 32, FAKE, 8, 4, 32, 64, FAKE, 64],
             [(1, 0), (2, None), (3, 31), (4, None), (5, 63), (6, 64 * 32 - 1), (7, None), (8, -1), (9, 0), (10, 0),
              (11, 0), (12, None), (13, 63)])
-    # stream, type, GY, ldgy, X, ldx, offsets, order, top_k, m, experts, width, k, GW, ldw, strideW
-    refused("mpkExpertGemmGradW", [None, 1, FAKE, 32, FAKE, 64, FAKE, FAKE, 2, 8, 4, 32, 64, FAKE, 64, 64 * 32],
+    # stream, type, GY, ldgy, X, ldx, offsets, order, top_k, m, experts, width, k, GW, ldw, strideW, work, bytes
+    refused("mpkExpertGemmGradW", [None, 1, FAKE, 32, FAKE, 64, FAKE, FAKE, 2, 8, 4, 32, 64, FAKE, 64, 64 * 32, FAKE, 1 << 30],
             [(1, 0), (2, None), (3, 31), (4, None), (5, 63), (6, None), (8, 0), (8, 3), (9, -1), (10, 0), (11, 0),
-             (12, 0), (13, None), (14, 63), (15, 64 * 32 - 1)])
+             (12, 0), (13, None), (14, 63), (15, 64 * 32 - 1), (16, None), (16, 4104), (17, 8 * 64 * 2 - 1)])
+    assert M.lib().mpkExpertGemmBytes(0, 8, 4, 64) == 0 and M.lib().mpkExpertGemmBytes(0, 800, 4, 64) == 800 * 64 * 2
 
 
 def test_combine_refuses():
