@@ -513,35 +513,46 @@ class Engine:
 _SCORES = {"softmax": 0, "sigmoid": 1}
 _GROUP_SCORES = {"max": 0, "top2": 1}
 _type_codes = None
+torch = None
 
 
 def _types() -> dict:
-    """torch dtype -> mpkType."""
-    global _type_codes
+    """torch dtype -> mpkType; binds torch on the first call."""
+    global _type_codes, torch
     if _type_codes is None:
         import torch
         _type_codes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
     return _type_codes
 
 
-def _matrix(name: str, t, dtypes=None, rows: int | None = None, cols: int | None = None) -> tuple[int, int]:
+def _matrix(name: str, t, rows: int | None = None, cols: int | None = None, dtype=None) -> tuple[int, int]:
     """(address, row stride) of a 2-D CUDA tensor whose rows are contiguous."""
-    if t.dim() != 2 or (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[1] != cols):
-        want = f"{'n' if rows is None else rows} x {'m' if cols is None else cols}"
-        raise ValueError(f"{name}: expected a {want} tensor, got {tuple(t.shape)}")
-    if dtypes is not None and t.dtype not in dtypes:
-        raise ValueError(f"{name}: dtype {t.dtype} is not one of {', '.join(map(str, dtypes))}")
+    if t.dim() != 2:
+        raise ValueError(f"{name}: expected a matrix, got {tuple(t.shape)}")
+    n, c = t.shape
+    if (rows is not None and n != rows) or (cols is not None and c != cols):
+        raise ValueError(f"{name}: expected {'n' if rows is None else rows} x {'m' if cols is None else cols}, got {n} x {c}")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{name}: dtype {t.dtype}, expected {dtype}")
     if not t.is_cuda:
         raise ValueError(f"{name}: expected a CUDA tensor")
-    n, c = t.shape
     ld, inner = t.stride()
-    if c > 1 and inner != 1:
+    if inner != 1 and c > 1:
         raise ValueError(f"{name}: rows must be contiguous")
     if n <= 1:
         ld = c
     elif ld < c:
         raise ValueError(f"{name}: rows overlap (row stride {ld} under {c} columns)")
     return t.data_ptr(), ld
+
+
+def _type_of(name: str, t, least: int = 0) -> int:
+    """mpkType of a tensor; least 1 leaves FP32 out."""
+    code = _types().get(t.dtype, -1)
+    if code < least:
+        raise ValueError(f"{name}: dtype {t.dtype} is not one of "
+                         f"{', '.join(str(d) for d, v in _types().items() if v >= least)}")
+    return code
 
 
 def _matrices(name: str, t, dtype, shape: tuple) -> tuple[int, int, int]:
@@ -567,35 +578,29 @@ def _matrices(name: str, t, dtype, shape: tuple) -> tuple[int, int, int]:
     return t.data_ptr(), sr, se
 
 
-def _int32(name: str, t, shape: tuple) -> int:
-    import torch
-    if tuple(t.shape) != shape or t.dtype != torch.int32:
-        raise ValueError(f"{name}: expected int32 of shape {shape}, got {t.dtype} of {tuple(t.shape)}")
-    return _ptr(t)
-
-
-def _fp32(name: str, t, shape: tuple) -> int:
-    import torch
-    if tuple(t.shape) != shape or t.dtype != torch.float32:
-        raise ValueError(f"{name}: expected float32 of shape {shape}, got {t.dtype} of {tuple(t.shape)}")
+def _array(name: str, t, dtype, *shape: int) -> int:
+    """Address of a contiguous CUDA tensor of this dtype and shape."""
+    if t.shape != shape or t.dtype != dtype:
+        raise ValueError(f"{name}: expected {dtype} of shape {shape}, got {t.dtype} of {tuple(t.shape)}")
     return _ptr(t)
 
 
 def _run(fn_name: str, tensors: tuple, *args) -> None:
     """Call fn_name(stream, *args) on the tensors' device (all on one) and torch's
     current stream there, the stream that outputs and scratch are allocated on."""
-    import torch
-    device = tensors[0].device
+    device = tensors[0].get_device()
     for t in tensors:
-        if t.device != device:
-            raise ValueError(f"{fn_name}: tensors on {device} and {t.device}")
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if device.index == torch.cuda.current_device():
-        status = getattr(lib(), fn_name)(stream, *args)
+        if t.get_device() != device:
+            raise ValueError(f"{fn_name}: tensors on {tensors[0].device} and {t.device}")
+    stream = torch._C._cuda_getCurrentRawStream(device)
+    fn = getattr(_lib or lib(), fn_name)
+    if device == torch.cuda.current_device():
+        status = fn(stream, *args)
     else:
         with torch.cuda.device(device):
-            status = getattr(lib(), fn_name)(stream, *args)
-    check(fn_name, status)
+            status = fn(stream, *args)
+    if status != MPK_OK:
+        raise MpkError(fn_name, status)
 
 
 def _route_params(experts, top_k, score, groups, top_groups, group_score, renormalize, scale) -> mpkRouteParams:
@@ -613,15 +618,15 @@ def route(logits, top_k: int, *, score: str = "softmax", bias=None, groups: int 
     FP16 or BF16; bias: one FP32 value an expert, added to the scores for the
     choice only.  Returns (ids, weights), n x top_k int32 and FP32, best first;
     id -1 with weight 0 where no expert is left (logits or bias of -inf mask)."""
-    import torch
-    address, ld = _matrix("logits", logits, _types())
+    code = _type_of("logits", logits)
+    address, ld = _matrix("logits", logits)
     n, experts = logits.shape
     params = _route_params(experts, top_k, score, groups, top_groups, group_score, renormalize, scale)
     used = (logits,) if bias is None else (logits, bias)
-    pbias = None if bias is None else _fp32("bias", bias, (experts,))
+    pbias = None if bias is None else _array("bias", bias, torch.float32, experts)
     ids = torch.empty((n, max(top_k, 0)), dtype=torch.int32, device=logits.device)
     weights = torch.empty((n, max(top_k, 0)), dtype=torch.float32, device=logits.device)
-    _run("mpkRoute", used, ctypes.byref(params), address, _types()[logits.dtype], n, ld, pbias, ids.data_ptr(),
+    _run("mpkRoute", used, ctypes.byref(params), address, code, n, ld, pbias, ids.data_ptr(),
          weights.data_ptr())
     return ids, weights
 
@@ -630,8 +635,8 @@ def route_grad(grad_weights, logits, ids, *, score: str = "softmax", renormalize
                out=None):
     """Gradient of route's weights with respect to its logits (mpkRouteGrad), of the
     logits' type; the choice (ids, as route returned them) is a constant."""
-    import torch
-    address, ld = _matrix("logits", logits, _types())
+    code = _type_of("logits", logits)
+    address, ld = _matrix("logits", logits)
     n, experts = logits.shape
     if ids.dim() != 2:
         raise ValueError(f"ids: expected n x top_k, got {tuple(ids.shape)}")
@@ -639,10 +644,10 @@ def route_grad(grad_weights, logits, ids, *, score: str = "softmax", renormalize
     params = _route_params(experts, top_k, score, 1, 1, "max", renormalize, scale)
     if out is None:
         out = torch.empty((n, experts), dtype=logits.dtype, device=logits.device)
-    address_out, ldg = _matrix("out", out, (logits.dtype,), n, experts)
+    address_out, ldg = _matrix("out", out, n, experts, logits.dtype)
     _run("mpkRouteGrad", (logits, ids, grad_weights, out), ctypes.byref(params), address,
-         _types()[logits.dtype], n, ld, _int32("ids", ids, (n, top_k)),
-         _fp32("grad_weights", grad_weights, (n, top_k)), address_out, ldg)
+         code, n, ld, _array("ids", ids, torch.int32, n, top_k),
+         _array("grad_weights", grad_weights, torch.float32, n, top_k), address_out, ldg)
     return out
 
 
@@ -660,20 +665,20 @@ class ExpertPlan:
         self.n, self.top_k = pos.shape
         self.rows = self.n * self.top_k
         self.experts = offsets.shape[0] - 1
-        _int32("offsets", offsets, (self.experts + 1,))
-        _int32("order", order, (self.rows,))
-        _int32("pos", pos, (self.n, self.top_k))
+        int32 = _types() and torch.int32
+        _array("offsets", offsets, int32, self.experts + 1)
+        _array("order", order, int32, self.rows)
+        _array("pos", pos, int32, self.n, self.top_k)
         self.offsets, self.order, self.pos = offsets, order, pos
 
 
 def expert_plan(ids, experts: int) -> ExpertPlan:
     """Sort the entries of ids (n x top_k int32) by expert, stably (mpkExpertPlan);
     ids outside [0, experts) are dropped."""
-    import torch
     if ids.dim() != 2:
         raise ValueError(f"ids: expected n x top_k, got {tuple(ids.shape)}")
     n, top_k = ids.shape
-    address = _int32("ids", ids, (n, top_k))
+    address = _array("ids", ids, _types() and torch.int32, n, top_k)
     need = int(lib().mpkExpertPlanBytes(n, top_k, experts))
     buf = torch.empty(max(experts, 0) + 1 + 2 * n * top_k, dtype=torch.int32, device=ids.device)
     offsets, order, pos = buf.split([max(experts, 0) + 1, n * top_k, n * top_k])
@@ -696,16 +701,15 @@ def expert_gemm(x, w, plan: ExpertPlan, *, gather: bool = True, out=None):
     """Every routed row times its expert's matrix (mpkExpertGemm): out[r] = w[e] x[r].
     w: experts x width x k, FP16 or BF16.  x: n x k token rows (gather) or n * top_k
     rows already sorted.  Returns n * top_k x width, rows without an expert zero."""
-    import torch
-    half = (torch.float16, torch.bfloat16)
-    address, ldx = _matrix("x", x, half, plan.n if gather else plan.rows)
+    code = _type_of("x", x, 1)
+    address, ldx = _matrix("x", x, plan.n if gather else plan.rows)
     pw, ldw, sw = _matrices("w", w, x.dtype, (plan.experts, None, x.shape[1]))
     width, k = w.shape[1], w.shape[2]
     if out is None:
         out = torch.empty((plan.rows, width), dtype=x.dtype, device=x.device)
-    po, ldo = _matrix("out", out, (x.dtype,), plan.rows, width)
+    po, ldo = _matrix("out", out, plan.rows, width, x.dtype)
     work, pwork, need = _sorted_copy(0, x, plan, gather)
-    _run("mpkExpertGemm", (x, w, plan.offsets, plan.order, out), _types()[x.dtype], address, ldx, pw, ldw, sw,
+    _run("mpkExpertGemm", (x, w, plan.offsets, plan.order, out), code, address, ldx, pw, ldw, sw,
          plan.offsets.data_ptr(), plan.order.data_ptr() if gather else None, plan.top_k, plan.rows, plan.experts,
          width, k, po, ldo, pwork, need)
     return out
@@ -715,15 +719,14 @@ def expert_gemm_grad_x(grad, w, plan: ExpertPlan, *, out=None):
     """Gradient of expert_gemm for its sorted rows (mpkExpertGemmGradX): out[r] = w[e]^T
     grad[r], n * top_k x k.  For gathered tokens, expert_combine(out, plan) adds a
     token's rows up.  Also the product for weights stored experts x k x width."""
-    import torch
-    half = (torch.float16, torch.bfloat16)
-    address, ldg = _matrix("grad", grad, half, plan.rows)
+    code = _type_of("grad", grad, 1)
+    address, ldg = _matrix("grad", grad, plan.rows)
     pw, ldw, sw = _matrices("w", w, grad.dtype, (plan.experts, grad.shape[1], None))
     width, k = w.shape[1], w.shape[2]
     if out is None:
         out = torch.empty((plan.rows, k), dtype=grad.dtype, device=grad.device)
-    po, ldo = _matrix("out", out, (grad.dtype,), plan.rows, k)
-    _run("mpkExpertGemmGradX", (grad, w, plan.offsets, out), _types()[grad.dtype], address, ldg, pw, ldw, sw,
+    po, ldo = _matrix("out", out, plan.rows, k, grad.dtype)
+    _run("mpkExpertGemmGradX", (grad, w, plan.offsets, out), code, address, ldg, pw, ldw, sw,
          plan.offsets.data_ptr(), plan.rows, plan.experts, width, k, po, ldo)
     return out
 
@@ -731,16 +734,15 @@ def expert_gemm_grad_x(grad, w, plan: ExpertPlan, *, out=None):
 def expert_gemm_grad_w(grad, x, plan: ExpertPlan, *, gather: bool = True, out=None):
     """Gradient of expert_gemm for its weights (mpkExpertGemmGradW): out[e] = sum over
     the expert's rows of grad[r] x[r]^T, experts x width x k; zero without rows."""
-    import torch
-    half = (torch.float16, torch.bfloat16)
-    address, ldx = _matrix("x", x, half, plan.n if gather else plan.rows)
-    pg, ldg = _matrix("grad", grad, (x.dtype,), plan.rows)
+    code = _type_of("x", x, 1)
+    address, ldx = _matrix("x", x, plan.n if gather else plan.rows)
+    pg, ldg = _matrix("grad", grad, plan.rows, None, x.dtype)
     width, k = grad.shape[1], x.shape[1]
     if out is None:
         out = torch.empty((plan.experts, width, k), dtype=x.dtype, device=x.device)
     po, ldo, so = _matrices("out", out, x.dtype, (plan.experts, width, k))
     work, pwork, need = _sorted_copy(1, x, plan, gather)
-    _run("mpkExpertGemmGradW", (grad, x, plan.offsets, plan.order, out), _types()[x.dtype], pg, ldg, address,
+    _run("mpkExpertGemmGradW", (grad, x, plan.offsets, plan.order, out), code, pg, ldg, address,
          ldx, plan.offsets.data_ptr(), plan.order.data_ptr() if gather else None, plan.top_k, plan.rows, plan.experts,
          width, k, po, ldo, so, pwork, need)
     return out
@@ -749,15 +751,15 @@ def expert_gemm_grad_w(grad, x, plan: ExpertPlan, *, gather: bool = True, out=No
 def expert_combine(y, plan: ExpertPlan, weights=None, *, out=None):
     """Back to token order (mpkExpertCombine): out[t] = sum over slots of weights[t, s] *
     y[pos[t, s]]; weights None: 1.  y: n * top_k x width, FP32, FP16 or BF16."""
-    import torch
-    address, ldy = _matrix("y", y, _types(), plan.rows)
+    code = _type_of("y", y)
+    address, ldy = _matrix("y", y, plan.rows)
     width = y.shape[1]
     if out is None:
         out = torch.empty((plan.n, width), dtype=y.dtype, device=y.device)
-    po, ldo = _matrix("out", out, (y.dtype,), plan.n, width)
+    po, ldo = _matrix("out", out, plan.n, width, y.dtype)
     used = (y, plan.pos, out) if weights is None else (y, plan.pos, out, weights)
-    pweights = None if weights is None else _fp32("weights", weights, (plan.n, plan.top_k))
-    _run("mpkExpertCombine", used, _types()[y.dtype], address, ldy, plan.pos.data_ptr(), pweights, plan.n,
+    pweights = None if weights is None else _array("weights", weights, torch.float32, plan.n, plan.top_k)
+    _run("mpkExpertCombine", used, code, address, ldy, plan.pos.data_ptr(), pweights, plan.n,
          plan.top_k, width, po, ldo)
     return out
 
@@ -766,23 +768,23 @@ def expert_combine_grad(grad, y, plan: ExpertPlan, weights=None, *, out=None):
     """Gradients of expert_combine (mpkExpertCombineGrad) from grad (n x width): (for y,
     n * top_k x width with zero rows behind the last; for weights, n x top_k FP32).
     y None: only the first, the other is None."""
-    import torch
-    address, ldgo = _matrix("grad", grad, _types(), plan.n)
+    code = _type_of("grad", grad)
+    address, ldgo = _matrix("grad", grad, plan.n)
     width = grad.shape[1]
     if out is None:
         out = torch.empty((plan.rows, width), dtype=grad.dtype, device=grad.device)
-    po, ldo = _matrix("out", out, (grad.dtype,), plan.rows, width)
+    po, ldo = _matrix("out", out, plan.rows, width, grad.dtype)
     used = [grad, plan.pos, plan.offsets, out]
     py, ldy, grad_weights, pgw, pweights = None, 0, None, None, None
     if y is not None:
-        py, ldy = _matrix("y", y, (grad.dtype,), plan.rows, width)
+        py, ldy = _matrix("y", y, plan.rows, width, grad.dtype)
         grad_weights = torch.empty((plan.n, plan.top_k), dtype=torch.float32, device=grad.device)
         pgw = grad_weights.data_ptr()
         used.append(y)
     if weights is not None:
-        pweights = _fp32("weights", weights, (plan.n, plan.top_k))
+        pweights = _array("weights", weights, torch.float32, plan.n, plan.top_k)
         used.append(weights)
-    _run("mpkExpertCombineGrad", tuple(used), _types()[grad.dtype], address, ldgo, py, ldy,
+    _run("mpkExpertCombineGrad", tuple(used), code, address, ldgo, py, ldy,
          plan.pos.data_ptr(), plan.offsets.data_ptr() + 4 * plan.experts, pweights, plan.n, plan.top_k, width, po, ldo,
          pgw)
     return out, grad_weights

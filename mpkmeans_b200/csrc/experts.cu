@@ -210,127 +210,132 @@ k_sort_rows(const uint16_t* __restrict__ x, long long ldx, const int* __restrict
 
 /* --------------------------------------------------------------- combine ---- */
 
-/* V consecutive elements of a row, as floats. */
+/* V consecutive elements of a row: as they are loaded, and as floats. */
 template <typename T, int V>
 struct Pack {
-    __device__ static __forceinline__ void load(const T* p, float (&f)[V]) {
-        if constexpr (V == 1) {
-            f[0] = to_f(*p);
-        } else {
-            const uint4 u = *reinterpret_cast<const uint4*>(p);
-            const T* t = reinterpret_cast<const T*>(&u);
+    using Raw = typename std::conditional<V == 1, T, uint4>::type;
+    __device__ static __forceinline__ Raw raw(const T* p) { return *reinterpret_cast<const Raw*>(p); }
+    __device__ static __forceinline__ void open(const Raw& r, float (&f)[V]) {
+        const T* t = reinterpret_cast<const T*>(&r);
 #pragma unroll
-            for (int i = 0; i < V; ++i) f[i] = to_f(t[i]);
-        }
+        for (int i = 0; i < V; ++i) f[i] = to_f(t[i]);
     }
     __device__ static __forceinline__ void store(T* p, const float (&f)[V]) {
-        if constexpr (V == 1) {
-            *p = from_f<T>(f[0]);
-        } else {
-            uint4 u;
-            T* t = reinterpret_cast<T*>(&u);
+        Raw r;
+        T* t = reinterpret_cast<T*>(&r);
 #pragma unroll
-            for (int i = 0; i < V; ++i) t[i] = from_f<T>(f[i]);
-            *reinterpret_cast<uint4*>(p) = u;
-        }
+        for (int i = 0; i < V; ++i) t[i] = from_f<T>(f[i]);
+        *reinterpret_cast<Raw*>(p) = r;
     }
 };
 
 constexpr int kCombineThreads = 256;
 
-/* One thread a 16-byte piece (V elements) of one token's output row: the slots'
- * rows are read once, added in slot order in FP32, written once. */
-template <typename T, int V>
+/* TPR threads (a power of two) share a token's row, kCombineThreads / TPR tokens a
+ * block, blockIdx.y the TPR-piece span of the row: one thread a 16-byte piece (V
+ * elements).  S slots' pieces are in flight at once and are added in slot order in
+ * FP32; every row is read once, every output written once. */
+template <typename T, int V, int S>
 __global__ void __launch_bounds__(kCombineThreads)
 k_combine(const T* __restrict__ y, long long ldy, const int* __restrict__ pos, const float* __restrict__ weights,
-          long long n, int top_k, int width, T* __restrict__ out, long long ldo) {
-    const int pieces = (width + V - 1) / V;
-    const long long m = n * top_k, total = n * pieces, step = (long long)gridDim.x * kCombineThreads;
-    for (long long i = (long long)blockIdx.x * kCombineThreads + threadIdx.x; i < total; i += step) {
-        const long long t = i / pieces;
-        const int c = (int)(i - t * pieces) * V;
-        float acc[V] = {};
-        for (int s0 = 0; s0 < top_k; s0 += 8) {
-            float f[8][V], wt[8];
+          long long n, int top_k, int width, int log_tpr, T* __restrict__ out, long long ldo) {
+    const long long t = ((long long)blockIdx.x << (8 - log_tpr)) + (threadIdx.x >> log_tpr);
+    const int c = (int)(((blockIdx.y << log_tpr) + (threadIdx.x & ((1u << log_tpr) - 1u))) * V);
+    if (t >= n || c >= width) return;
+    const long long m = n * top_k;
+    float acc[V] = {};
+    for (int s0 = 0; s0 < top_k; s0 += S) {
+        typename Pack<T, V>::Raw f[S];
+        float wt[S];
 #pragma unroll
-            for (int s = 0; s < 8; ++s) {
-                const long long q = t * top_k + s0 + s;
-                const long long p = s0 + s < top_k ? pos[q] : -1;
-                wt[s] = 0.f;
-                if (p >= 0 && p < m) {
-                    wt[s] = weights ? weights[q] : 1.f;
-                    Pack<T, V>::load(y + p * ldy + c, f[s]);
-                } else {
-#pragma unroll
-                    for (int u = 0; u < V; ++u) f[s][u] = 0.f;
-                }
-            }
-#pragma unroll
-            for (int s = 0; s < 8; ++s)
-#pragma unroll
-                for (int u = 0; u < V; ++u) acc[u] = fmaf(wt[s], f[s][u], acc[u]);
+        for (int s = 0; s < S; ++s) {
+            const long long q = t * top_k + s0 + s;
+            const int p = s0 + s < top_k ? pos[q] : -1;
+            const bool there = p >= 0 && p < m;
+            wt[s] = !there ? 0.f : weights ? weights[q] : 1.f;
+            f[s] = there ? Pack<T, V>::raw(y + (long long)p * ldy + c) : typename Pack<T, V>::Raw{};
         }
-        Pack<T, V>::store(out + t * ldo + c, acc);
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            float v[V];
+            Pack<T, V>::open(f[s], v);
+#pragma unroll
+            for (int u = 0; u < V; ++u) acc[u] = fmaf(wt[s], v[u], acc[u]);
+        }
     }
+    Pack<T, V>::store(out + t * ldo + c, acc);
 }
 
-/* One block a token (grid-stride): the token's gradient row is read once per
- * group of 8 slots (from L1/L2 after the first), every slot's row is read once
- * for the weight's dot product and its gradient row written once.  The dots are
- * summed per thread over its columns, then over the block in a fixed order. */
-template <typename T, int V>
+/* TPR threads (32 .. 256) a token: for every piece of the token's gradient row the
+ * S slots' pieces are read together for the weights' dot products and their
+ * gradient pieces written.  The dots are summed per thread over its columns, then
+ * over the token's threads in a fixed order. */
+template <typename T, int V, int S>
 __global__ void __launch_bounds__(kCombineThreads)
 k_combine_grad(const T* __restrict__ go, long long ldgo, const T* __restrict__ y, long long ldy,
                const int* __restrict__ pos, const int* __restrict__ rows, const float* __restrict__ weights,
-               long long n, int top_k, int width, T* __restrict__ gy, long long ldgy, float* __restrict__ gw) {
-    __shared__ float part[kCombineThreads / 32][8];
+               long long n, int top_k, int width, int log_tpr, T* __restrict__ gy, long long ldgy,
+               float* __restrict__ gw) {
+    __shared__ float part[kCombineThreads / 32][S];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const long long m = n * top_k;
-    for (long long t = blockIdx.x; t < n; t += gridDim.x)
-        for (int s0 = 0; s0 < top_k; s0 += 8) {
-            long long p[8];
-            float wt[8], dot[8];
+    const long long t = ((long long)blockIdx.x << (8 - log_tpr)) + (threadIdx.x >> log_tpr);
+    const int tpr = 1 << log_tpr, own = threadIdx.x & (tpr - 1);
+    for (int s0 = 0; s0 < top_k; s0 += S) {
+        int p[S];
+        float wt[S], dot[S];
 #pragma unroll
-            for (int s = 0; s < 8; ++s) {
-                const long long q = t * top_k + s0 + s;
-                p[s] = s0 + s < top_k ? pos[q] : -1;
-                if (p[s] >= m) p[s] = -1;
-                wt[s] = p[s] >= 0 ? (weights ? weights[q] : 1.f) : 0.f;
-                dot[s] = 0.f;
-            }
-            for (int c = threadIdx.x * V; c < width; c += kCombineThreads * V) {
+        for (int s = 0; s < S; ++s) {
+            const long long q = t * top_k + s0 + s;
+            p[s] = t < n && s0 + s < top_k ? pos[q] : -1;
+            if (p[s] >= m) p[s] = -1;
+            wt[s] = p[s] < 0 ? 0.f : weights ? weights[q] : 1.f;
+            dot[s] = 0.f;
+        }
+        if (t < n)
+            for (int c = own * V; c < width; c += tpr * V) {
                 float g[V];
-                Pack<T, V>::load(go + t * ldgo + c, g);
+                Pack<T, V>::open(Pack<T, V>::raw(go + t * ldgo + c), g);
+                if (gw) {
+                    typename Pack<T, V>::Raw f[S];
 #pragma unroll
-                for (int s = 0; s < 8; ++s)
+                    for (int s = 0; s < S; ++s)
+                        f[s] = p[s] >= 0 ? Pack<T, V>::raw(y + (long long)p[s] * ldy + c) : typename Pack<T, V>::Raw{};
+#pragma unroll
+                    for (int s = 0; s < S; ++s) {
+                        float v[V];
+                        Pack<T, V>::open(f[s], v);
+                        /* a dropped slot stays 0 whatever the gradient holds */
+#pragma unroll
+                        for (int u = 0; u < V; ++u) dot[s] = p[s] >= 0 ? fmaf(g[u], v[u], dot[s]) : 0.f;
+                    }
+                }
+#pragma unroll
+                for (int s = 0; s < S; ++s)
                     if (p[s] >= 0) {
-                        float f[V];
-                        if (gw) {
-                            Pack<T, V>::load(y + p[s] * ldy + c, f);
+                        float v[V];
 #pragma unroll
-                            for (int u = 0; u < V; ++u) dot[s] = fmaf(g[u], f[u], dot[s]);
-                        }
-#pragma unroll
-                        for (int u = 0; u < V; ++u) f[u] = wt[s] * g[u];
-                        Pack<T, V>::store(gy + p[s] * ldgy + c, f);
+                        for (int u = 0; u < V; ++u) v[u] = wt[s] * g[u];
+                        Pack<T, V>::store(gy + (long long)p[s] * ldgy + c, v);
                     }
             }
-            if (gw) {
+        if (gw) {
 #pragma unroll
-                for (int s = 0; s < 8; ++s) {
-                    float v = dot[s];
-                    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
-                    if (lane == 0) part[warp][s] = v;
-                }
-                __syncthreads();
-                if (threadIdx.x < 8 && s0 + (int)threadIdx.x < top_k) {
-                    float v = 0.f;
-                    for (int q = 0; q < kCombineThreads / 32; ++q) v += part[q][threadIdx.x];
-                    gw[t * top_k + s0 + threadIdx.x] = v;
-                }
-                __syncthreads();
+            for (int s = 0; s < S; ++s) {
+                float v = dot[s];
+                for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+                if (lane == 0) part[warp][s] = v;
             }
+            __syncthreads();
+            if (own < S && s0 + own < top_k && t < n) {
+                float v = 0.f;
+                for (int q = 0; q < (tpr >> 5); ++q) v += part[warp + q][own];
+                gw[t * top_k + s0 + own] = v;
+            }
+            __syncthreads();
         }
+    }
+    /* rows that no expert owns */
     const int valid = *rows;
     const int pieces = (width + V - 1) / V;
     const float zero[V] = {};
@@ -400,38 +405,60 @@ bool work_ok(size_t need, const void* work, size_t bytes) {
     return need == 0 || (work && bytes >= need && reinterpret_cast<uintptr_t>(work) % 16 == 0);
 }
 
+/* Threads a row (log2): a power of two up to the block that covers the row's pieces. */
+int log_threads(int pieces, int least) {
+    int l = least;
+    while (l < 8 && (1 << l) < pieces) ++l;
+    return l;
+}
+
+template <typename T, int V, int S>
+cudaError_t start_combine(const T* y, long long ldy, const int* pos, const float* weights, long long n, int top_k,
+                          int width, T* out, long long ldo, cudaStream_t s) {
+    const int pieces = (width + V - 1) / V, l = log_threads(pieces, 0);
+    const long long tokens = kCombineThreads >> l;
+    const dim3 grid((unsigned)((n + tokens - 1) / tokens), (unsigned)((pieces + (1 << l) - 1) >> l));
+    k_combine<T, V, S><<<grid, kCombineThreads, 0, s>>>(y, ldy, pos, weights, n, top_k, width, l, out, ldo);
+    return cudaGetLastError();
+}
+
 template <typename T>
 cudaError_t run_combine(const void* y, long long ldy, const int* pos, const float* weights, long long n, int top_k,
-                        int width, void* out, long long ldo, int sms, cudaStream_t s) {
+                        int width, void* out, long long ldo, cudaStream_t s) {
     constexpr int V = 16 / sizeof(T);
     const bool vec = width % V == 0 && aligned16(y, ldy, sizeof(T)) && aligned16(out, ldo, sizeof(T));
-    const long long pieces = n * (vec ? width / V : width);
-    const long long want = (pieces + kCombineThreads - 1) / kCombineThreads, most = (long long)sms * 64;
-    const int grid = (int)(want < most ? want : most);
-    const T *py = static_cast<const T*>(y);
+    const T* py = static_cast<const T*>(y);
     T* po = static_cast<T*>(out);
-    if (vec) k_combine<T, V><<<grid, kCombineThreads, 0, s>>>(py, ldy, pos, weights, n, top_k, width, po, ldo);
-    else k_combine<T, 1><<<grid, kCombineThreads, 0, s>>>(py, ldy, pos, weights, n, top_k, width, po, ldo);
+    if (!vec) return start_combine<T, 1, 8>(py, ldy, pos, weights, n, top_k, width, po, ldo, s);
+    return top_k <= 4 ? start_combine<T, V, 4>(py, ldy, pos, weights, n, top_k, width, po, ldo, s)
+                      : start_combine<T, V, 8>(py, ldy, pos, weights, n, top_k, width, po, ldo, s);
+}
+
+template <typename T, int V, int S>
+cudaError_t start_combine_grad(const T* go, long long ldgo, const T* y, long long ldy, const int* pos, const int* rows,
+                               const float* weights, long long n, int top_k, int width, T* gy, long long ldgy,
+                               float* gw, cudaStream_t s) {
+    const int l = log_threads((width + V - 1) / V, 5);
+    const long long tokens = kCombineThreads >> l;
+    k_combine_grad<T, V, S><<<(unsigned)((n + tokens - 1) / tokens), kCombineThreads, 0, s>>>(
+        go, ldgo, y, ldy, pos, rows, weights, n, top_k, width, l, gy, ldgy, gw);
     return cudaGetLastError();
 }
 
 template <typename T>
 cudaError_t run_combine_grad(const void* go, long long ldgo, const void* y, long long ldy, const int* pos,
                              const int* rows, const float* weights, long long n, int top_k, int width, void* gy,
-                             long long ldgy, float* gw, int sms, cudaStream_t s) {
+                             long long ldgy, float* gw, cudaStream_t s) {
     constexpr int V = 16 / sizeof(T);
     const bool vec = width % V == 0 && aligned16(go, ldgo, sizeof(T)) && (!gw || aligned16(y, ldy, sizeof(T))) &&
                      aligned16(gy, ldgy, sizeof(T));
-    const int grid = (int)(n < (long long)sms * 16 ? n : (long long)sms * 16);
     const T *pg = static_cast<const T*>(go), *py = static_cast<const T*>(y);
     T* po = static_cast<T*>(gy);
-    if (vec)
-        k_combine_grad<T, V><<<grid, kCombineThreads, 0, s>>>(pg, ldgo, py, ldy, pos, rows, weights, n, top_k, width,
-                                                              po, ldgy, gw);
-    else
-        k_combine_grad<T, 1><<<grid, kCombineThreads, 0, s>>>(pg, ldgo, py, ldy, pos, rows, weights, n, top_k, width,
-                                                              po, ldgy, gw);
-    return cudaGetLastError();
+    if (!vec)
+        return start_combine_grad<T, 1, 8>(pg, ldgo, py, ldy, pos, rows, weights, n, top_k, width, po, ldgy, gw, s);
+    return top_k <= 4
+        ? start_combine_grad<T, V, 4>(pg, ldgo, py, ldy, pos, rows, weights, n, top_k, width, po, ldgy, gw, s)
+        : start_combine_grad<T, V, 8>(pg, ldgo, py, ldy, pos, rows, weights, n, top_k, width, po, ldgy, gw, s);
 }
 
 bool combine_ok(int type, long long n, int top_k, int width) {
@@ -499,12 +526,10 @@ mpkStatus mpkExpertCombine(cudaStream_t stream, int type, const void* dY, long l
     if (!combine_ok(type, n, top_k, width) || ldy < width || ldo < width) return MPK_ERR_INVALID;
     if (n == 0) return MPK_OK;
     if (!dY || !dPos || !dOut) return MPK_ERR_INVALID;
-    const int sms = sm_count();
-    if (!sms) return MPK_ERR_CUDA;
     const cudaError_t e =
-        type == MPK_TYPE_FP32 ? run_combine<float>(dY, ldy, dPos, dWeights, n, top_k, width, dOut, ldo, sms, stream)
-        : type == MPK_TYPE_FP16 ? run_combine<__half>(dY, ldy, dPos, dWeights, n, top_k, width, dOut, ldo, sms, stream)
-        : run_combine<__nv_bfloat16>(dY, ldy, dPos, dWeights, n, top_k, width, dOut, ldo, sms, stream);
+        type == MPK_TYPE_FP32 ? run_combine<float>(dY, ldy, dPos, dWeights, n, top_k, width, dOut, ldo, stream)
+        : type == MPK_TYPE_FP16 ? run_combine<__half>(dY, ldy, dPos, dWeights, n, top_k, width, dOut, ldo, stream)
+        : run_combine<__nv_bfloat16>(dY, ldy, dPos, dWeights, n, top_k, width, dOut, ldo, stream);
     return e == cudaSuccess ? MPK_OK : MPK_ERR_CUDA;
 }
 
@@ -515,15 +540,13 @@ mpkStatus mpkExpertCombineGrad(cudaStream_t stream, int type, const void* dGOut,
         return MPK_ERR_INVALID;
     if (n == 0) return MPK_OK;
     if (!dGOut || (dGWeights && !dY) || !dPos || !dRows || !dGY) return MPK_ERR_INVALID;
-    const int sms = sm_count();
-    if (!sms) return MPK_ERR_CUDA;
     const cudaError_t e =
         type == MPK_TYPE_FP32 ? run_combine_grad<float>(dGOut, ldgo, dY, ldy, dPos, dRows, dWeights, n, top_k, width,
-                                                        dGY, ldgy, dGWeights, sms, stream)
+                                                        dGY, ldgy, dGWeights, stream)
         : type == MPK_TYPE_FP16 ? run_combine_grad<__half>(dGOut, ldgo, dY, ldy, dPos, dRows, dWeights, n, top_k,
-                                                           width, dGY, ldgy, dGWeights, sms, stream)
+                                                           width, dGY, ldgy, dGWeights, stream)
         : run_combine_grad<__nv_bfloat16>(dGOut, ldgo, dY, ldy, dPos, dRows, dWeights, n, top_k, width, dGY, ldgy,
-                                          dGWeights, sms, stream);
+                                          dGWeights, stream);
     return e == cudaSuccess ? MPK_OK : MPK_ERR_CUDA;
 }
 

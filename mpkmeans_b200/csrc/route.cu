@@ -4,9 +4,11 @@
  * mpkRoute, one warp a token.  With logits l, scores s (softmax or sigmoid) and
  * choice values c = s + bias, the warp keeps the row in registers (expert 32 v +
  * lane in register v), turns every choice value into an integer key of the same
- * order (NaN highest, masked 0), drops the groups that lose, and takes the
- * maximum top_k times with two warp reductions each: the key, then the lowest
- * index that holds it.
+ * order (NaN highest, masked lowest) and drops the groups that lose.  The top_k
+ * largest of the 32 lanes' maxima give a bound that at least top_k experts reach
+ * and few others do: about ten of 256 for top_k = 8.  Those are packed one a lane
+ * and ranked against each other.  (Taking the maximum top_k times, rescanning the
+ * registers of the lane that held it, was a third of 1800 instructions a row.)
  *
  * The choice is exact, as the assignment's is: without a bias, and with groups
  * scored by their maximum, the order of c is the order of l and the keys are the
@@ -47,19 +49,17 @@ __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-/* An unsigned key in the order of v: -inf (masked) 0, NaN the highest, the two
- * zeros equal. */
+/* An unsigned key in the order of v: the two zeros equal, NaN the highest (the
+ * addition makes every NaN the positive one), -inf below kLive. */
+constexpr unsigned kLive = 0x00800000u;
 __device__ __forceinline__ unsigned key_of(float v) {
-    if (v != v) return 0xffffffffu;
     const unsigned u = __float_as_uint(v + 0.0f);
-    const unsigned k = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-    return v == -INFINITY ? 0u : k;
+    return u ^ (0x80000000u | (unsigned)((int)u >> 31));
 }
 __device__ __forceinline__ float of_key(unsigned k) {
-    if (k == 0xffffffffu) return NAN;
-    if (k == 0u) return -INFINITY;
     return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
+/* The same in FP64, -inf as 0. */
 __device__ __forceinline__ unsigned long long key_of(double v) {
     if (v != v) return ~0ull;
     const unsigned long long u = (unsigned long long)__double_as_longlong(v + 0.0);
@@ -71,6 +71,9 @@ __device__ __forceinline__ double of_key(unsigned long long k) {
     if (k == 0ull) return -(double)INFINITY;
     return __longlong_as_double((long long)((k >> 63) ? (k & ~(1ull << 63)) : ~k));
 }
+
+__device__ __forceinline__ bool live(unsigned k) { return k >= kLive; }
+__device__ __forceinline__ bool live(unsigned long long k) { return k != 0; }
 
 __device__ __forceinline__ float warp_sum(float v) {
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
@@ -106,7 +109,7 @@ __device__ __forceinline__ KEY group_key(const KEY* keys, const RouteShape& sh, 
         if (a2 > a) { b = a > b2 ? a : b2; a = a2; }
         else b = a2 > b ? a2 : b;
     }
-    if (sh.group_score == MPK_GROUP_TOP2 && b != 0) a = key_of(of_key(a) + of_key(b));
+    if (sh.group_score == MPK_GROUP_TOP2 && live(b)) a = key_of(of_key(a) + of_key(b));
     return a;
 }
 
@@ -120,7 +123,7 @@ __device__ __forceinline__ unsigned kept_groups(KEY gk, const RouteShape& sh, in
         const KEY o = __shfl_sync(FULL, gk, h * L);
         rank += (o > gk || (o == gk && h < g)) ? 1 : 0;
     }
-    return __ballot_sync(FULL, lane == g * L && g < sh.G && gk != 0 && rank < sh.top_groups);
+    return __ballot_sync(FULL, lane == g * L && g < sh.G && live(gk) && rank < sh.top_groups);
 }
 
 __device__ __forceinline__ int lanes_per_group(int G) {
@@ -188,11 +191,78 @@ __device__ __forceinline__ float chosen_score(float x, float m, bool softmax) {
     return 1.f / (1.f + expf(-x));
 }
 
+/* The `takes` largest of a warp's keys in descending order, the lowest index first
+ * among equals: lane i returns the i-th in (key, index), index -1 where there are
+ * fewer.  cand: 32 words of this warp's shared memory. */
+template <int VPL>
+__device__ __forceinline__ void top_keys(unsigned (&key)[VPL], int takes, unsigned long long* cand, int lane,
+                                         unsigned& mykey, int& mine) {
+    mykey = 0u;
+    mine = -1;
+    /* bound: the takes-th largest of the lanes' maxima, or any live key */
+    unsigned lm = key[0], bound = kLive;
+#pragma unroll
+    for (int v = 1; v < VPL; ++v) lm = max(lm, key[v]);
+    for (int seen = 0;;) {
+        const unsigned m = __reduce_max_sync(FULL, lm);
+        if (m < kLive) break;
+        seen += __popc(__ballot_sync(FULL, lm == m));
+        if (seen >= takes) { bound = m; break; }
+        if (lm == m) lm = 0u;
+    }
+    int count = 0;
+    const unsigned below = (1u << lane) - 1u;
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) {
+        const bool in = key[v] >= bound;
+        const unsigned who = __ballot_sync(FULL, in);
+        const int at = count + __popc(who & below);
+        if (in && at < 32) cand[at] = (unsigned long long)key[v] << 32 | (unsigned)(32 * v + lane);
+        count += __popc(who);
+    }
+    __syncwarp();
+    if (count <= 32) {
+        /* candidate `lane`, in ascending order of index; its rank among them */
+        const unsigned long long c = lane < count ? cand[lane] : 0ull;
+        const unsigned k = (unsigned)(c >> 32);
+        int rank = 0;
+        for (int q = 0; q < count; ++q) {
+            const unsigned o = __shfl_sync(FULL, k, q);
+            rank += (o > k || (o == k && q < lane)) ? 1 : 0;
+        }
+        __syncwarp();
+        if (lane < count && rank < takes) cand[rank] = c;
+        __syncwarp();
+        if (lane < min(count, takes)) {
+            mykey = (unsigned)(cand[lane] >> 32);
+            mine = (int)(unsigned)cand[lane];
+        }
+    } else {
+        /* many equal maxima: the maximum, takes times */
+        for (int i = 0; i < takes; ++i) {
+            unsigned bk = 0u;
+            int bj = INT_MAX;
+#pragma unroll
+            for (int v = 0; v < VPL; ++v)
+                if (key[v] > bk) { bk = key[v]; bj = 32 * v + lane; }
+            const unsigned top = __reduce_max_sync(FULL, bk);
+            if (top < kLive) break;
+            const int j = __reduce_min_sync(FULL, bk == top ? bj : INT_MAX);
+            if (lane == i) { mykey = top; mine = j; }
+#pragma unroll
+            for (int v = 0; v < VPL; ++v)
+                if (32 * v + lane == j) key[v] = 0u;
+        }
+    }
+    __syncwarp();
+}
+
 template <typename T, int VPL>
 __global__ void __launch_bounds__(32 * kRouteWarps)
 k_route(const T* __restrict__ logits, long long n, long long ld, const float* __restrict__ bias, RouteShape sh,
         int* __restrict__ ids, float* __restrict__ weights) {
     extern __shared__ unsigned long long route_sm[];
+    __shared__ unsigned long long route_cand[kRouteWarps][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     unsigned long long* keys64 = route_sm + (size_t)warp * sh.E;
     unsigned* keys32 = reinterpret_cast<unsigned*>(keys64);
@@ -202,6 +272,19 @@ k_route(const T* __restrict__ logits, long long n, long long ld, const float* __
     const bool by_score = bias || top2;                       /* keys are choice values c, else logits */
     const bool scores = by_score || (softmax && !sh.renorm);  /* some use of all experts' scores */
     const int L = lanes_per_group(sh.G);
+    /* the bias and the groups of this lane's experts, kept over the rows where registers allow */
+    constexpr bool KEEP = VPL <= 8;
+    float bv[KEEP ? VPL : 1];
+    unsigned char gv[KEEP ? VPL : 1];
+    auto bias_of = [&](int v) { return 32 * v + lane < sh.E ? bias[32 * v + lane] : 0.f; };
+    auto group_of = [&](int v) { return (unsigned char)min(31u, ((unsigned)(32 * v + lane) * sh.gmul >> 20) * L); };
+    if constexpr (KEEP) {
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) {
+            bv[v] = bias ? bias_of(v) : 0.f;
+            gv[v] = group_of(v);
+        }
+    }
     const long long step = (long long)gridDim.x * kRouteWarps;
     for (long long t = (long long)blockIdx.x * kRouteWarps + warp; t < n; t += step) {
         const T* row = logits + t * ld;
@@ -227,19 +310,19 @@ k_route(const T* __restrict__ logits, long long n, long long ld, const float* __
                 for (int v = 0; v < VPL; ++v) c[v] *= smax;
             } else {
 #pragma unroll
-                for (int v = 0; v < VPL; ++v) c[v] = 1.f / (1.f + expf(-x[v]));
+                for (int v = 0; v < VPL; ++v) c[v] = __fdividef(1.f, 1.f + expf(-x[v]));
             }
 #pragma unroll
             for (int v = 0; v < VPL; ++v) {
-                if (bias && 32 * v + lane < sh.E) c[v] += bias[32 * v + lane];
+                if (bias) c[v] += KEEP ? bv[KEEP ? v : 0] : bias_of(v);
                 key[v] = x[v] == -INFINITY ? 0u : key_of(by_score ? c[v] : x[v]);
             }
         } else {
 #pragma unroll
             for (int v = 0; v < VPL; ++v) key[v] = key_of(x[v]);
         }
-        /* Error bounds of c.  expf and the sigmoid's division leave a few 2^-23
-         * of s; softmax adds |x - mx| 2^-24 s from the rounded argument, which is
+        /* Error bounds of c.  expf (2 ulp) and the sigmoid's division (2 ulp) leave 1.5 2^-22
+         * of 1; softmax adds |x - mx| 2^-24 s from the rounded argument, which is
          * under 2^-17 s wherever s does not underflow and under 2^-19 of the
          * row's largest score everywhere; adding the bias rounds by 2^-24 |c|. */
         auto near = [&](float a, float b) {
@@ -260,42 +343,19 @@ k_route(const T* __restrict__ logits, long long n, long long ld, const float* __
                 const bool there = lane == g * L && g < sh.G, in = (kept >> lane) & 1u;
                 const unsigned lo = __reduce_min_sync(FULL, there && in ? gk : 0xffffffffu);
                 const unsigned hi = __reduce_max_sync(FULL, there && !in ? gk : 0u);
-                if (kept && hi) slow = near(of_key(lo), of_key(hi));
+                if (kept && live(hi)) slow = near(of_key(lo), of_key(hi));
             }
 #pragma unroll
             for (int v = 0; v < VPL; ++v) {
-                const unsigned g = ((unsigned)(32 * v + lane) * sh.gmul >> 20) * L;
-                if (!(g < 32 && ((kept >> g) & 1u))) key[v] = 0u;
+                const unsigned g = KEEP ? gv[KEEP ? v : 0] : group_of(v);
+                if (!((kept >> g) & 1u) || 32 * v + lane >= sh.E) key[v] = 0u;
                 else if (top2 && !bias) key[v] = key_of(x[v]);      /* groups chosen: the logits' order again */
             }
             __syncwarp();
         }
-        int mine = -1;
-        unsigned mykey = 0;
-        {
-            unsigned bk = 0;
-            int bv = 0;
-#pragma unroll
-            for (int v = 0; v < VPL; ++v)
-                if (key[v] > bk) { bk = key[v]; bv = v; }
-            const int takes = sh.k + (bias && sh.k < 32 ? 1 : 0);
-            for (int i = 0; i < takes; ++i) {
-                const unsigned top = __reduce_max_sync(FULL, bk);
-                if (top == 0u) break;
-                const unsigned j = __reduce_min_sync(FULL, bk == top ? (unsigned)(32 * bv + lane) : 0xffffffffu);
-                if (lane == i) { mine = (int)j; mykey = top; }
-                if (lane == (int)(j & 31u)) {
-#pragma unroll
-                    for (int v = 0; v < VPL; ++v)
-                        if (v == bv) key[v] = 0u;
-                    bk = 0u;
-                    bv = 0;
-#pragma unroll
-                    for (int v = 0; v < VPL; ++v)
-                        if (key[v] > bk) { bk = key[v]; bv = v; }
-                }
-            }
-        }
+        int mine;
+        unsigned mykey;
+        top_keys(key, sh.k + (bias && sh.k < 32 ? 1 : 0), route_cand[warp], lane, mykey, mine);
         if (bias) {
             const unsigned nk = __shfl_down_sync(FULL, mykey, 1);
             const int nj = __shfl_down_sync(FULL, mine, 1);
@@ -401,27 +461,22 @@ k_route_grad(const T* __restrict__ logits, long long n, long long ld, RouteShape
 
 /* -------------------------------------------------------------- the plan ---- */
 /* A stable counting sort.  A block takes a chunk of the entries, each of its
- * warps a contiguous piece; a warp counts 32 entries at a time with
- * match_any (the lanes that share an expert), so an entry's rank among its
- * expert's is (entries of earlier blocks) + (of earlier warps) + (of this warp so
- * far) + (lower lanes of its match): no atomics, and the order is fixed. */
+ * warps a contiguous piece, 32 at a time: match_any gives the lanes that share an
+ * expert, so an entry's rank among its expert's is (entries of earlier blocks) +
+ * (of earlier warps) + (of this warp so far) + (lower lanes of its match): no
+ * atomics decide an order.  The block sorts its entries in shared memory first and
+ * writes each expert's run in one piece.
+ *
+ * Up to kPlanOne entries one block does everything; above, the blocks' counts
+ * (k_plan_count), their prefixes (k_plan_scan) and the placement are three launches. */
 constexpr int kPlanThreads = 512, kPlanWarps = kPlanThreads / 32;
-constexpr int kPlanChunk = 4096;             /* entries a block of the multi-block plan */
-constexpr int kPlanOne = 16384;              /* up to here one block does everything in one launch */
+constexpr int kPlanPer = 8;                                 /* entries a lane */
+constexpr int kPlanChunk = kPlanThreads * kPlanPer;         /* and a block of the multi-block plan */
+constexpr int kPlanOne = 2 * kPlanChunk;
 
 __device__ __forceinline__ int plan_id(const int* ids, long long i, long long end, int E) {
     const int a = i < end ? ids[i] : -1;
     return (unsigned)a < (unsigned)E ? a : -1;
-}
-
-/* Counts of this warp's piece [lo, hi) into cnt (E ints of shared memory, zeroed). */
-__device__ __forceinline__ void plan_count(const int* ids, long long lo, long long hi, int E, int* cnt, int lane) {
-    for (long long i = lo; i < hi; i += 32) {
-        const int a = plan_id(ids, i + lane, hi, E);
-        const unsigned peers = __match_any_sync(FULL, a);
-        if (a >= 0 && lane == __ffs(peers) - 1) cnt[a] += __popc(peers);
-        __syncwarp();
-    }
 }
 
 /* Exclusive scan of one int per thread over the block; tot receives the total. */
@@ -437,6 +492,7 @@ __device__ __forceinline__ int block_scan(int v, int* part, int& tot) {
     __syncthreads();
     int run = 0;
     tot = 0;
+#pragma unroll
     for (int q = 0; q < kPlanWarps; ++q) {
         if (q < w) run += part[q];
         tot += part[q];
@@ -445,81 +501,105 @@ __device__ __forceinline__ int block_scan(int v, int* part, int& tot) {
     return run + incl - v;
 }
 
-/* cnt[w * E + e] (counts of each warp) becomes the first sorted row of warp w's
- * entries of expert e, given before[e] rows of e in earlier blocks (NULL: none)
- * and the experts' totals (NULL: the block's own).  Returns the total of all;
- * block 0 writes the offsets. */
-__device__ int plan_starts(int* cnt, int E, const int* before, long long before_stride, const int* totals,
-                           int* offsets, int* part) {
-    int carry = 0;
+/* Placement of one chunk.  work: NULL when the chunk is everything, else the
+ * scanned counts, work[e * B + b] rows of expert e before block b and totals
+ * behind them. */
+template <int PER>
+__global__ void __launch_bounds__(kPlanThreads)
+k_plan(const int* __restrict__ ids, long long m, int E, const int* __restrict__ work, int* __restrict__ offsets,
+       int* __restrict__ order, int* __restrict__ pos) {
+    constexpr int CHUNK = kPlanThreads * PER;
+    extern __shared__ int plan_sm[];
+    __shared__ int part[kPlanWarps];
+    int* cnt = plan_sm;                          /* kPlanWarps x E: counts, then prefixes over the warps */
+    int* first = cnt + kPlanWarps * E;           /* E: sorted row of the chunk's first entry of each expert */
+    int* local = first + E;                      /* E: the same inside the chunk */
+    int* entry = local + E;                      /* CHUNK: the chunk's entries, sorted */
+    unsigned short* owner = reinterpret_cast<unsigned short*>(entry + CHUNK);
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int B = gridDim.x;
+    const long long lo = (long long)blockIdx.x * CHUNK + w * (32 * PER);
+    int a[PER], rank[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) a[i] = plan_id(ids, lo + 32 * i + lane, m, E);
+    for (int i = threadIdx.x; i < kPlanWarps * E; i += kPlanThreads) cnt[i] = 0;
+    __syncthreads();
+    int* mine = cnt + w * E;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const unsigned peers = __match_any_sync(FULL, a[i]);
+        const int old = a[i] >= 0 ? mine[a[i]] : 0;
+        rank[i] = old + __popc(peers & ((1u << lane) - 1u));
+        __syncwarp();
+        if (a[i] >= 0 && lane == __ffs(peers) - 1) mine[a[i]] = old + __popc(peers);
+        __syncwarp();
+    }
+    __syncthreads();
+    int gcarry = 0, lcarry = 0;
     for (int e0 = 0; e0 < E; e0 += kPlanThreads) {
         const int e = e0 + threadIdx.x;
         int own = 0;
-        if (e < E)
-            for (int w = 0; w < kPlanWarps; ++w) {
-                const int c = cnt[w * E + e];
-                cnt[w * E + e] = own;
+        if (e < E) {
+#pragma unroll
+            for (int q = 0; q < kPlanWarps; ++q) {
+                const int c = cnt[q * E + e];
+                cnt[q * E + e] = own;
                 own += c;
             }
-        int tot;
-        const int base = carry + block_scan(e < E ? (totals ? totals[e] : own) : 0, part, tot);
+        }
+        int ltot, gtot;
+        const int lbase = lcarry + block_scan(own, part, ltot);
+        int gbase = lbase;
+        if (work) {
+            gbase = gcarry + block_scan(e < E ? work[(size_t)E * B + e] : 0, part, gtot);
+            gcarry += gtot;
+        }
+        lcarry += ltot;
         if (e < E) {
-            const int first = base + (before ? before[e * before_stride] : 0);
-            for (int w = 0; w < kPlanWarps; ++w) cnt[w * E + e] += first;
-            if (offsets) offsets[e] = base;
+            local[e] = lbase;
+            first[e] = gbase + (work ? work[(size_t)e * B + blockIdx.x] : 0);
+            if (blockIdx.x == 0) offsets[e] = gbase;
         }
-        carry += tot;
     }
-    if (offsets && threadIdx.x == 0) offsets[E] = carry;
+    const int total = work ? gcarry : lcarry;
+    if (blockIdx.x == 0 && threadIdx.x == 0) offsets[E] = total;
     __syncthreads();
-    return carry;
-}
-
-__device__ __forceinline__ void plan_place(const int* ids, long long lo, long long hi, int E, int* at, int* order,
-                                           int* pos, int lane) {
-    for (long long i = lo; i < hi; i += 32) {
-        const int a = plan_id(ids, i + lane, hi, E);
-        const unsigned peers = __match_any_sync(FULL, a);
-        const int r = a >= 0 ? at[a] + __popc(peers & ((1u << lane) - 1u)) : -1;
-        if (i + lane < hi) pos[i + lane] = r;
-        if (r >= 0) order[r] = (int)(i + lane);
-        __syncwarp();
-        if (a >= 0 && lane == __ffs(peers) - 1) at[a] += __popc(peers);
-        __syncwarp();
-    }
-}
-
-/* STAGE 0: the whole plan in one block.  STAGE 1: this block's counts to
- * work[e * B + b].  STAGE 2: placement, with work scanned by k_plan_scan. */
-template <int STAGE>
-__global__ void __launch_bounds__(kPlanThreads)
-k_plan(const int* __restrict__ ids, long long m, int E, long long chunk, int* __restrict__ work,
-       int* __restrict__ offsets, int* __restrict__ order, int* __restrict__ pos) {
-    extern __shared__ int cnt[];                 /* kPlanWarps x E */
-    __shared__ int part[kPlanWarps];
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const long long c0 = (long long)blockIdx.x * chunk, c1 = min(m, c0 + chunk);
-    const long long piece = ((chunk + kPlanWarps - 1) / kPlanWarps + 31) / 32 * 32;
-    const long long lo = min(c1, c0 + w * piece), hi = min(c1, lo + piece);
-    const long long B = gridDim.x;
-    for (int i = threadIdx.x; i < kPlanWarps * E; i += kPlanThreads) cnt[i] = 0;
-    __syncthreads();
-    plan_count(ids, lo, hi, E, cnt + w * E, lane);
-    __syncthreads();
-    if (STAGE == 1) {
-        for (int e = threadIdx.x; e < E; e += kPlanThreads) {
-            int s = 0;
-            for (int q = 0; q < kPlanWarps; ++q) s += cnt[q * E + e];
-            work[e * B + blockIdx.x] = s;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const long long q = lo + 32 * i + lane;
+        int p = -1;
+        if (a[i] >= 0) {
+            const int r = mine[a[i]] + rank[i];
+            p = first[a[i]] + r;
+            entry[local[a[i]] + r] = (int)q;
+            owner[local[a[i]] + r] = (unsigned short)a[i];
         }
-        return;
+        if (q < m) pos[q] = p;
     }
-    const int total = STAGE == 0 ? plan_starts(cnt, E, nullptr, 0, nullptr, offsets, part)
-                                 : plan_starts(cnt, E, work + blockIdx.x, B, work + E * B,
-                                               blockIdx.x == 0 ? offsets : nullptr, part);
-    plan_place(ids, lo, hi, E, cnt + w * E, order, pos, lane);
-    for (long long r = total + (long long)blockIdx.x * kPlanThreads + threadIdx.x; r < m; r += B * kPlanThreads)
+    __syncthreads();
+    for (int i = threadIdx.x; i < lcarry; i += kPlanThreads) {
+        const int e = owner[i];
+        order[first[e] + (i - local[e])] = entry[i];
+    }
+    for (long long r = total + (long long)blockIdx.x * kPlanThreads + threadIdx.x; r < m; r += (long long)B * kPlanThreads)
         order[r] = -1;
+}
+
+/* This block's entries of each expert, to work[e * B + b]. */
+__global__ void __launch_bounds__(kPlanThreads)
+k_plan_count(const int* __restrict__ ids, long long m, int E, int* __restrict__ work) {
+    extern __shared__ int plan_sm[];
+    for (int e = threadIdx.x; e < E; e += kPlanThreads) plan_sm[e] = 0;
+    __syncthreads();
+    int a[kPlanPer];
+#pragma unroll
+    for (int i = 0; i < kPlanPer; ++i)
+        a[i] = plan_id(ids, (long long)blockIdx.x * kPlanChunk + i * kPlanThreads + threadIdx.x, m, E);
+#pragma unroll
+    for (int i = 0; i < kPlanPer; ++i)
+        if (a[i] >= 0) atomicAdd(&plan_sm[a[i]], 1);
+    __syncthreads();
+    for (int e = threadIdx.x; e < E; e += kPlanThreads) work[(size_t)e * gridDim.x + blockIdx.x] = plan_sm[e];
 }
 
 /* One warp an expert: its counts over the blocks become their exclusive prefix,
@@ -607,6 +687,18 @@ bool type_ok(int type) { return type == MPK_TYPE_FP32 || type == MPK_TYPE_FP16 |
 
 long long plan_blocks(long long m) { return m <= kPlanOne ? 1 : (m + kPlanChunk - 1) / kPlanChunk; }
 
+template <int PER>
+cudaError_t run_plan(const int* ids, long long m, int E, int B, const int* work, int* offsets, int* order, int* pos,
+                     cudaStream_t s) {
+    const int smem = (kPlanWarps + 2) * E * (int)sizeof(int) + kPlanThreads * PER * 6;
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(k_plan<PER>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+    }
+    k_plan<PER><<<B, kPlanThreads, smem, s>>>(ids, m, E, work, offsets, order, pos);
+    return cudaGetLastError();
+}
+
 }  /* namespace */
 }  /* namespace mpk */
 
@@ -660,22 +752,21 @@ mpkStatus mpkExpertPlan(cudaStream_t stream, const int* dIds, long long n, int t
     if (m > 0 && (!dIds || !dOrder || !dPos)) return MPK_ERR_INVALID;
     const size_t need = mpkExpertPlanBytes(n, top_k, experts);
     if (need && (!dWork || work_bytes < need || reinterpret_cast<uintptr_t>(dWork) % sizeof(int))) return MPK_ERR_INVALID;
-    const int smem = kPlanWarps * experts * (int)sizeof(int);
     const int B = (int)plan_blocks(m);
     int* work = static_cast<int*>(dWork);
-    if (smem > 48 * 1024) {
-        if (cudaFuncSetAttribute(k_plan<0>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
-            cudaFuncSetAttribute(k_plan<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
-            cudaFuncSetAttribute(k_plan<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-            return MPK_ERR_CUDA;
-    }
-    if (B == 1) {
-        k_plan<0><<<1, kPlanThreads, smem, stream>>>(dIds, m, experts, m, nullptr, dOffsets, dOrder, dPos);
-    } else {
-        k_plan<1><<<B, kPlanThreads, smem, stream>>>(dIds, m, experts, kPlanChunk, work, nullptr, nullptr, nullptr);
+    cudaError_t e;
+    if (B > 1) {
+        k_plan_count<<<B, kPlanThreads, experts * (int)sizeof(int), stream>>>(dIds, m, experts, work);
         k_plan_scan<<<(experts + 7) / 8, 256, 0, stream>>>(work, experts, B);
-        k_plan<2><<<B, kPlanThreads, smem, stream>>>(dIds, m, experts, kPlanChunk, work, dOffsets, dOrder, dPos);
+        e = run_plan<kPlanPer>(dIds, m, experts, B, work, dOffsets, dOrder, dPos, stream);
+    } else if (m <= kPlanThreads) {
+        e = run_plan<1>(dIds, m, experts, 1, nullptr, dOffsets, dOrder, dPos, stream);
+    } else if (m <= 4 * kPlanThreads) {
+        e = run_plan<4>(dIds, m, experts, 1, nullptr, dOffsets, dOrder, dPos, stream);
+    } else {
+        e = run_plan<kPlanOne / kPlanThreads>(dIds, m, experts, 1, nullptr, dOffsets, dOrder, dPos, stream);
     }
+    if (e != cudaSuccess) return MPK_ERR_CUDA;
     return cudaGetLastError() == cudaSuccess ? MPK_OK : MPK_ERR_CUDA;
 }
 
