@@ -12,9 +12,13 @@
  * so weights are always the wide operand's source, a short segment of rows costs
  * only a narrow tile, and every store of a warp runs along f.  The experts' row
  * counts are on the device only: each CTA scans them into shared memory and the
- * grid walks the tiles of all experts.
+ * grid walks the tiles of all experts.  The launch has a cluster for every tile
+ * there can be; a running cluster takes over the next one that has not started
+ * (clusterlaunchcontrol), so uneven tiles spread evenly without a counter in
+ * memory.  An element's sum is formed in one order whichever cluster does it.
  *
- *   warp 0      TMA producer: one 64-deep stage of A and B at a time.
+ *   warp 0      TMA producer: one 64-deep stage of A and B at a time; asks for the
+ *               next tile as it starts one.
  *   warp 1      MMA issuer, whole contraction into one FP32 TMEM accumulator, two
  *               accumulators so that the next tile's MMAs overlap the epilogue.
  *   warps 2-9   epilogue: round to the output type, swap halves between lane
@@ -40,9 +44,15 @@
  *
  * Rows past a segment.  FWD and GRADX read whatever rows follow (the gather
  * writes zeros): a column of the accumulator depends on its own row only and those
- * columns are not stored.  GRADW contracts over the rows, so the last stage of a
- * segment fetches its rows by gather4 with an index past the tensor for the rows
- * that are not the expert's, which TMA fills with zeros.
+ * columns are not stored.  GRADW contracts over the rows, so rows of the last stage
+ * that are not the expert's must be zeros.  They come from a second tensor map of
+ * the same matrix, three-dimensional with both outer strides one row: element
+ * (c, y, z) is row y + z, y < 64.  A box of 64 rows from y = 64 - rem, z = end - 64
+ * holds the segment's last rem rows, and the rest of it lies past y's bound, which
+ * TMA fills with zeros.  (Segments that end before row 64 have no such z: gather4
+ * with an index past the tensor for the other rows, 45 ns an instruction; all
+ * tails that way made the gradient of 32 x 2048 x 4096 weights from 1200 rows
+ * take 380 us.)
  */
 #include "experts.cuh"
 #include "mpkexperts.h"
@@ -67,6 +77,7 @@ constexpr int A_STAGE = BM * BK * 2;             /* 16 KB */
 constexpr int BOX = 64 * 64 * 2;                 /* one 64 x 64 MN-major box */
 constexpr int kSmemMax = 232448;
 constexpr int kMisc = 1024 + 4 * (MPK_MAX_EXPERTS + 1);
+constexpr int kSched = 3;                        /* work indices between the producer and the epilogue */
 constexpr int kGroup = 8;                        /* row tiles that sweep the f tiles together */
 
 template <bool PAIR>
@@ -90,7 +101,8 @@ struct Cfg {
 
 template <int STAGES>
 struct EMisc {
-    uint64_t full[STAGES], empty[STAGES], t_full[2], t_empty[2], fin;
+    uint4 next[kSched];         /* the scheduler's answers */
+    uint64_t full[STAGES], empty[STAGES], t_full[2], t_empty[2], s_full[kSched], s_empty[kSched], fin;
     uint32_t tmem_slot;
     int abort_flag;
 };
@@ -146,6 +158,36 @@ __device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity) {
         if (globaltimer() - t0 > kWaitLimitNs) return;
 }
 
+/* Asks for the next cluster that has not started; the answer (16 bytes) comes to the
+ * same place in every CTA of this cluster and counts on its barrier. */
+template <bool PAIR>
+__device__ __forceinline__ void ask_next(uint4* answer, uint64_t* bar) {
+    if (PAIR)
+        asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes"
+                     ".multicast::cluster::all.b128 [%0], [%1];"
+                     :: "r"(smem_u32(answer)), "r"(smem_u32(bar)) : "memory");
+    else
+        asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+                     :: "r"(smem_u32(answer)), "r"(smem_u32(bar)) : "memory");
+}
+/* First block of the cluster taken over, or -1: none is left. */
+__device__ __forceinline__ int read_next(const uint4* answer) {
+    uint32_t yes, x;
+    uint4 a;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w) : "r"(smem_u32(answer)) : "memory");
+    asm volatile("{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t.reg .b64 lo, hi;\n\t"
+                 "mov.b64 lo, {%2, %3};\n\tmov.b64 hi, {%4, %5};\n\tmov.b128 h, {lo, hi};\n\t"
+                 "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+                 "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}"
+                 : "=r"(yes), "=r"(x) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w));
+    return yes ? (int)x : -1;
+}
+__device__ __forceinline__ void mbar_expect_tx_cluster(uint32_t cluster_addr, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" :: "r"(cluster_addr), "r"(bytes) : "memory");
+}
+
 /* One tile of one expert's output. */
 struct Tile {
     int e;
@@ -169,8 +211,9 @@ struct Tiles {
     int e;
     __device__ Tiles(const Params& p_, const int* start_) : p(p_), start(start_), ft((p_.F + FTILE - 1) / FTILE), e(0) {}
     __device__ long long total() const { return (long long)start[p.experts] * ft; }
-    /* u ascends from call to call */
+    /* u mostly ascends from call to call */
     __device__ Tile at(long long u) {
+        if ((long long)start[e] * ft > u) e = 0;
         while ((long long)start[e + 1] * ft <= u) ++e;
         Tile t;
         t.e = e;
@@ -201,7 +244,8 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, bool bf16) {
 template <int MODE, bool PAIR, int FMT>
 __global__ void __launch_bounds__(Cfg<PAIR>::THREADS, 1)
 k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-             const __grid_constant__ CUtensorMap tmAg, const __grid_constant__ CUtensorMap tmBg, const Params p) {
+             const __grid_constant__ CUtensorMap tmAg, const __grid_constant__ CUtensorMap tmBg,
+             const __grid_constant__ CUtensorMap tmAt, const __grid_constant__ CUtensorMap tmBt, const Params p) {
     static_assert(PAIR || MODE != EXP_GRADW, "the weights' gradient runs on pairs");
     using K = Cfg<PAIR>;
     constexpr int STAGES = K::STAGES, STAGE = K::STAGE, BN = K::BN, BL = K::BL;
@@ -214,7 +258,7 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
     volatile int* abort_flag = &ms.abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = PAIR ? (int)cluster_rank() : 0;
-    const long long u0 = PAIR ? blockIdx.x >> 1 : blockIdx.x, ustep = PAIR ? gridDim.x >> 1 : gridDim.x;
+    const long long u0 = PAIR ? blockIdx.x >> 1 : blockIdx.x, units = PAIR ? gridDim.x >> 1 : gridDim.x;
 
     if (smem_u32(smem) & 1023u) {
         if (threadIdx.x == 0) atomicOr(&g_experts_status, MPK_DEV_TIMEOUT);
@@ -225,6 +269,9 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
         const int arrivals = gathers ? 2 : 1;
         for (int i = 0; i < STAGES; ++i) { mbar_init(&ms.full[i], arrivals); mbar_init(&ms.empty[i], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&ms.t_full[i], 1); mbar_init(&ms.t_empty[i], (PAIR ? 2 : 1) * kEpiWarps); }
+        /* a work index is read by producer, MMA issuer (CTA 0 only), epilogue and gather warps */
+        const int readers = PAIR ? 2 * (1 + kEpiWarps) + 1 : 2 + kEpiWarps + (gathers ? kGatherWarps : 0);
+        for (int i = 0; i < kSched; ++i) { mbar_init(&ms.s_full[i], 1); mbar_init(&ms.s_empty[i], readers); }
         mbar_init(&ms.fin, 1);
         ms.abort_flag = 0;
         fence_mbar_init();
@@ -262,14 +309,51 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
     Tiles<MODE, BN, K::FT> tiles(p, start);
     const long long total = tiles.total();
 
+    /* the next tile's index, for one thread; false when there is none (or a wait ran out) */
+    int taken = 0;
+    auto next = [&](long long& u) {
+        const int sl = taken % kSched;
+        if (!mbar_wait(&ms.s_full[sl], (uint32_t)(taken / kSched) & 1u, abort_flag, &g_experts_status)) return false;
+        const int x = read_next(&ms.next[sl]);
+        fence_async_proxy();
+        if (PAIR) mbar_arrive_cluster(peer_addr(&ms.s_empty[sl], 0));
+        else mbar_arrive(&ms.s_empty[sl]);
+        ++taken;
+        u = PAIR ? x >> 1 : x;
+        return x >= 0;
+    };
+    /* the same for a whole warp */
+    auto next_warp = [&](long long& u) {
+        int go = 0;
+        if (lane == 0) go = next(u) ? 1 : 0;
+        u = __shfl_sync(0xffffffffu, u, 0);
+        return __shfl_sync(0xffffffffu, go, 0) != 0;
+    };
+
     if (warp == 0) {
         /* ------------------------------------------------- producer ---- */
         uint32_t last[STAGES];
 #pragma unroll
         for (int i = 0; i < STAGES; ++i) last[i] = 0xffffffffu;
         uint32_t it = 0;
+        int asked = -1;
         bool ok = true;
-        for (long long u = u0; u < total && ok; u += ustep) {
+        bool more = true;
+        for (long long u = u0; more && ok; more = ok && next_warp(u)) {
+            if (lane == 0 && rank == 0) {                        /* one index ahead of the loads, no more: it is taken for good */
+                const int sl = taken % kSched;
+                const uint32_t use = (uint32_t)(taken / kSched);
+                ok = mbar_wait(&ms.s_empty[sl], (use & 1u) ^ 1u, abort_flag, &g_experts_status);
+                if (ok) {
+                    mbar_expect_tx(&ms.s_full[sl], 16);
+                    if (PAIR) mbar_expect_tx_cluster(peer_addr(&ms.s_full[sl], 1), 16);
+                    ask_next<PAIR>(&ms.next[sl], &ms.s_full[sl]);
+                    asked = taken;
+                }
+            }
+            ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+            if (!ok) break;
+            if (u >= total) continue;
             const Tile t = tiles.at(u);
             const int f0 = t.f0 + rank * BM;                     /* this CTA's f's */
             const int jn = PAIR ? t.wide / 2 : BN;               /* and j's */
@@ -319,6 +403,10 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
                     if (r + BK <= end) {
                         if (lane < 2) load2(&tmA, sa + lane * BOX, f0 + 64 * lane, r);
                         if (lane < boxes) load2(&tmB, sb + lane * BOX, jl + 64 * lane, r);
+                    } else if (end >= BK) {
+                        const int y = BK - (end - r), z = end - BK;
+                        if (lane < 2) load3(&tmAt, sa + lane * BOX, f0 + 64 * lane, y, z);
+                        if (lane < boxes) load3(&tmBt, sb + lane * BOX, jl + 64 * lane, y, z);
                     } else {
                         int own[4];
 #pragma unroll
@@ -330,6 +418,7 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
             }
         }
         if (!ok && lane == 0) {
+            if (asked >= 0) drain_wait(&ms.s_full[asked % kSched], (uint32_t)(asked / kSched) & 1u);
             if (!PAIR) {
 #pragma unroll
                 for (int i = 0; i < STAGES; ++i)
@@ -355,7 +444,9 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
             };
             uint32_t it = 0, ts = 0;
             bool ok = true;
-            for (long long u = u0; u < total && ok; u += ustep) {
+            bool more = true;
+            for (long long u = u0; more && ok; more = ok && next(u)) {
+                if (u >= total) continue;
                 const Tile t = tiles.at(u);
                 if (t.nk == 0) continue;
                 const int tb = (int)(ts & 1u);
@@ -406,7 +497,9 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
             uint32_t it0 = 0, it = (uint32_t)w;                  /* first stage of the tile; this warp's next */
             bool ok = true;
             int idx[N];
-            for (long long u = u0; u < total && ok; u += ustep) {
+            bool more = true;
+            for (long long u = u0; more && ok; more = ok && next_warp(u)) {
+                if (u >= total) continue;
                 const Tile t = tiles.at(u);
                 const int end = t.r0 + t.rows;
                 const uint32_t it1 = it0 + (uint32_t)t.nk;
@@ -449,9 +542,16 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
         const bool odd = lane & 1;
         const uint32_t sel = odd ? 0x3276u : 0x5410u;
         uint16_t* out = static_cast<uint16_t*>(p.out);
-        bool ok = true;
+        bool ok = true, more = true;
         uint32_t ts = 0;
-        for (long long u = u0; u < total; u += ustep) {
+        const int valid = expert_start(p.offsets, p.experts, p.m);
+        for (long long u = u0; more && ok; more = ok && next_warp(u)) {
+            if (MODE != EXP_GRADW) {              /* rows that no expert owns: each index sets its share to zero */
+                for (long long r = valid + u; r < p.m; r += units)
+                    for (int f = rank * 32 * kEpiWarps + threadIdx.x - 64; f < p.F; f += (PAIR ? 2 : 1) * 32 * kEpiWarps)
+                        out[r * p.ldo + f] = 0;
+            }
+            if (u >= total) continue;
             const Tile t = tiles.at(u);
             const int tb = (int)(ts & 1u);
             if (t.nk > 0) {
@@ -509,12 +609,6 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
                 }
             }
         }
-        if (MODE != EXP_GRADW) {                  /* rows that no expert owns */
-            const int valid = expert_start(p.offsets, p.experts, p.m);
-            const int tid = threadIdx.x - 64;
-            for (long long r = valid + (long long)blockIdx.x; r < p.m; r += gridDim.x)
-                for (int f = tid; f < p.F; f += 32 * kEpiWarps) out[r * p.ldo + f] = 0;
-        }
     }
 
     tc_fence_before();
@@ -563,7 +657,7 @@ cudaError_t launch_t(const ExpertArgs& a, cudaStream_t s) {
     using K = Cfg<PAIR>;
     constexpr int BN = K::BN;
     auto kern = k_experts_tc<MODE, PAIR, FMT>;
-    CUtensorMap tmA{}, tmB{}, tmAg{}, tmBg{};
+    CUtensorMap tmA{}, tmB{}, tmAg{}, tmBg{}, tmAt{}, tmBt{};
     bool ok;
     if (MODE == EXP_FWD) {
         ok = row_map(&tmA, a.w, a.bf16, a.k, a.width, a.experts, a.ldw, a.stride_w, BM) &&
@@ -575,6 +669,9 @@ cudaError_t launch_t(const ExpertArgs& a, cudaStream_t s) {
         ok = row_map(&tmA, a.x, a.bf16, a.k, a.m, 0, a.ldx, 0, BK) && row_map(&tmAg, a.x, a.bf16, a.k, a.m, 0, a.ldx, 0, 1) &&
              row_map(&tmB, a.gy, a.bf16, a.width, a.m, 0, a.ldgy, 0, BK) &&
              row_map(&tmBg, a.gy, a.bf16, a.width, a.m, 0, a.ldgy, 0, 1);
+        if (a.m >= BK)                           /* rows y + z, y < 64, z <= m - 64: all inside the matrix */
+            ok = ok && row_map(&tmAt, a.x, a.bf16, a.k, BK, a.m - BK + 1, a.ldx, a.ldx, BK) &&
+                 row_map(&tmBt, a.gy, a.bf16, a.width, BK, a.m - BK + 1, a.ldgy, a.ldgy, BK);
     }
     if (!ok) return cudaErrorInvalidValue;
     Params p{a.offsets, a.order, a.top_k, (int)a.m, a.experts, a.x, a.ldx, a.k, MODE == EXP_FWD ? a.width : a.k, a.width,
@@ -582,16 +679,15 @@ cudaError_t launch_t(const ExpertArgs& a, cudaStream_t s) {
              reinterpret_cast<uintptr_t>(a.out) % 4 == 0 && a.ldo % 2 == 0 && (MODE != EXP_GRADW || a.stride_o % 2 == 0)};
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, K::SMEM_BYTES);
     if (e != cudaSuccess) return e;
-    /* the most tiles there can be: every expert with rows rounds up by one */
+    /* a cluster for every tile there can be: every expert with rows rounds up by one */
     const long long ft = (p.F + K::FT - 1) / K::FT;
     const long long some = a.m < a.experts ? a.m : a.experts;
     const long long jt = MODE == EXP_GRADW ? (long long)a.experts * ((a.width + BN - 1) / BN) : a.m / BN + some;
     const long long units = ft * jt;
-    const long long fit = PAIR ? a.sms / 2 : a.sms;
-    const int n = (int)(units < fit ? units : fit);
-    if (n == 0) return cudaSuccess;
+    if (units > (1LL << 30)) return cudaErrorInvalidConfiguration;
+    const int n = (int)units;
     if (!PAIR) {
-        kern<<<n, K::THREADS, K::SMEM_BYTES, s>>>(tmA, tmB, tmAg, tmBg, p);
+        kern<<<n, K::THREADS, K::SMEM_BYTES, s>>>(tmA, tmB, tmAg, tmBg, tmAt, tmBt, p);
         return cudaGetLastError();
     }
     cudaLaunchConfig_t cfg = {};
@@ -606,7 +702,7 @@ cudaError_t launch_t(const ExpertArgs& a, cudaStream_t s) {
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kern, tmA, tmB, tmAg, tmBg, p);
+    e = cudaLaunchKernelEx(&cfg, kern, tmA, tmB, tmAg, tmBg, tmAt, tmBt, p);
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 

@@ -2,8 +2,8 @@
  * the plan that sorts the routed rows by expert (include/mpkexperts.h).
  *
  * mpkRoute, one warp a token.  With logits l, scores s (softmax or sigmoid) and
- * choice values c = s + bias, the warp keeps the row in registers (expert 32 v +
- * lane in register v), turns every choice value into an integer key of the same
+ * choice values c = s + bias, the warp keeps the row in registers (experts VPL *
+ * lane ... in registers 0 ..), turns every choice value into an integer key of the same
  * order (NaN highest, masked lowest) and drops the groups that lose.  The top_k
  * largest of the 32 lanes' maxima give a bound that at least top_k experts reach
  * and few others do: about ten of 256 for top_k = 8.  Those are packed one a lane
@@ -24,6 +24,7 @@
 
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 namespace mpk {
 namespace {
@@ -88,15 +89,81 @@ struct RouteShape {
     int E, k, score, G, gs, top_groups, group_score, renorm;
     unsigned gmul;            /* group of expert j: (j * gmul) >> 20, exact for j, gs < 1024 */
     float scale;
+    int log_l;                /* lanes a group scan takes (log2): 2^log_l * G <= 32 */
+    int log_k;                /* lanes the slots take (log2): 2^log_k >= k */
+    int log_g;                /* lanes that hold one group, where whole lanes do and their number is a power
+                               * of two (log2); -1: groups go through shared memory */
+    int vec;                  /* a lane's experts can be loaded and stored as one word or as 16-byte words */
 };
 
-/* The groups' keys (key of the maximum, or of the sum of the two best) from the
- * experts' keys in shared memory: lanes [g * L, g * L + L) work on group g.  Every
- * lane of a group's lanes returns its key; lanes past G * L return 0.  KEY is
- * the 32-bit key of a float or the 64-bit key of a double. */
+/* Sum, maximum over the slots' lanes (the others hold the neutral value). */
+__device__ __forceinline__ float slot_sum(float v, int log_k) {
+    for (int o = (1 << log_k) >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+    return v;
+}
+__device__ __forceinline__ float slot_max(float v, int log_k) {
+    for (int o = (1 << log_k) >> 1; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(FULL, v, o));
+    return v;
+}
+
+/* A lane's VPL consecutive elements of a row, from element VPL * lane. */
+template <typename T, int VPL>
+struct LaneRow {
+    static constexpr int BYTES = VPL * (int)sizeof(T);
+    static constexpr int WORD = BYTES < 16 ? BYTES : 16;
+    using W = typename std::conditional<WORD == 2, unsigned short, typename std::conditional<WORD == 4, unsigned,
+              typename std::conditional<WORD == 8, uint2, uint4>::type>::type>::type;
+    /* -inf past the row */
+    __device__ static __forceinline__ void load(const T* row, int E, bool vec, int lane, float (&x)[VPL]) {
+        const int j = VPL * lane;
+        if (vec && j + VPL <= E) {
+            W w[BYTES / WORD];
+#pragma unroll
+            for (int i = 0; i < BYTES / WORD; ++i) w[i] = reinterpret_cast<const W*>(row + j)[i];
+            const T* t = reinterpret_cast<const T*>(w);
+#pragma unroll
+            for (int v = 0; v < VPL; ++v) x[v] = to_f(t[v]);
+        } else {
+#pragma unroll
+            for (int v = 0; v < VPL; ++v) x[v] = j + v < E ? to_f(row[j + v]) : -INFINITY;
+        }
+    }
+    __device__ static __forceinline__ void store(T* row, int E, bool vec, int lane, const float (&x)[VPL]) {
+        const int j = VPL * lane;
+        if (vec && j + VPL <= E) {
+            W w[BYTES / WORD];
+            T* t = reinterpret_cast<T*>(w);
+#pragma unroll
+            for (int v = 0; v < VPL; ++v) t[v] = from_f<T>(x[v]);
+#pragma unroll
+            for (int i = 0; i < BYTES / WORD; ++i) reinterpret_cast<W*>(row + j)[i] = w[i];
+        } else {
+#pragma unroll
+            for (int v = 0; v < VPL; ++v)
+                if (j + v < E) row[j + v] = from_f<T>(x[v]);
+        }
+    }
+};
+
+/* The two largest of two pairs (a >= b). */
 template <typename KEY>
-__device__ __forceinline__ KEY group_key(const KEY* keys, const RouteShape& sh, int L, int lane) {
-    const int g = lane / L, sub = lane - g * L;
+__device__ __forceinline__ void merge2(KEY& a, KEY& b, KEY a2, KEY b2) {
+    if (a2 > a) { b = a > b2 ? a : b2; a = a2; }
+    else b = a2 > b ? a2 : b;
+}
+/* Key of a group from those of its two best. */
+template <typename KEY>
+__device__ __forceinline__ KEY group_of_two(KEY a, KEY b, int group_score) {
+    return group_score == MPK_GROUP_TOP2 && live(b) ? key_of(of_key(a) + of_key(b)) : a;
+}
+
+/* The groups' keys (key of the maximum, or of the sum of the two best) from the
+ * experts' keys in shared memory: 2^log_l lanes work on a group and all return its
+ * key; lanes past the groups return 0.  KEY is the 32-bit key of a float or the
+ * 64-bit key of a double. */
+template <typename KEY>
+__device__ __forceinline__ KEY group_key(const KEY* keys, const RouteShape& sh, int lane) {
+    const int L = 1 << sh.log_l, g = lane >> sh.log_l, sub = lane & (L - 1);
     KEY a = 0, b = 0;
     if (g < sh.G)
         for (int i = sub; i < sh.gs; i += L) {
@@ -106,30 +173,22 @@ __device__ __forceinline__ KEY group_key(const KEY* keys, const RouteShape& sh, 
         }
     for (int o = L >> 1; o > 0; o >>= 1) {
         const KEY a2 = __shfl_xor_sync(FULL, a, o), b2 = __shfl_xor_sync(FULL, b, o);
-        if (a2 > a) { b = a > b2 ? a : b2; a = a2; }
-        else b = a2 > b ? a2 : b;
+        merge2(a, b, a2, b2);
     }
-    if (sh.group_score == MPK_GROUP_TOP2 && live(b)) a = key_of(of_key(a) + of_key(b));
-    return a;
+    return group_of_two(a, b, sh.group_score);
 }
 
-/* Bit g * L of the result: group g is among the top_groups best (ties to the
- * lowest index) and has an expert left. */
+/* Whether this lane's group, lane >> log, is among the top_groups best of G (ties to
+ * the lowest index) and has an expert left. */
 template <typename KEY>
-__device__ __forceinline__ unsigned kept_groups(KEY gk, const RouteShape& sh, int L, int lane) {
-    const int g = lane / L;
+__device__ __forceinline__ bool group_kept(KEY gk, const RouteShape& sh, int log, int lane) {
+    const int g = lane >> log;
     int rank = 0;
     for (int h = 0; h < sh.G; ++h) {
-        const KEY o = __shfl_sync(FULL, gk, h * L);
+        const KEY o = __shfl_sync(FULL, gk, h << log);
         rank += (o > gk || (o == gk && h < g)) ? 1 : 0;
     }
-    return __ballot_sync(FULL, lane == g * L && g < sh.G && live(gk) && rank < sh.top_groups);
-}
-
-__device__ __forceinline__ int lanes_per_group(int G) {
-    int L = 1;
-    while (2 * L * G <= 32) L *= 2;
-    return L;
+    return g < sh.G && live(gk) && rank < sh.top_groups;
 }
 
 /* The whole choice of one row in FP64: slot `lane`'s expert, or -1.  keys: E
@@ -155,11 +214,10 @@ __device__ __noinline__ int slow_choice(const T* __restrict__ row, const float* 
     }
     __syncwarp();
     if (sh.G > 1) {
-        const int L = lanes_per_group(sh.G);
-        const unsigned kept = kept_groups(group_key(keys, sh, L, lane), sh, L, lane);
+        const unsigned kept = __ballot_sync(FULL, group_kept(group_key(keys, sh, lane), sh, sh.log_l, lane));
         __syncwarp();
         for (int j = lane; j < sh.E; j += 32)
-            if (!((kept >> (((unsigned)j * sh.gmul >> 20) * L)) & 1u)) keys[j] = 0ull;
+            if (!((kept >> (((unsigned)j * sh.gmul >> 20) << sh.log_l)) & 1u)) keys[j] = 0ull;
         __syncwarp();
     }
     int mine = -1;
@@ -199,29 +257,34 @@ __device__ __forceinline__ void top_keys(unsigned (&key)[VPL], int takes, unsign
                                          unsigned& mykey, int& mine) {
     mykey = 0u;
     mine = -1;
-    /* bound: the takes-th largest of the lanes' maxima, or any live key */
+    /* bound: the takes-th largest value of the lanes' maxima, or any live key */
     unsigned lm = key[0], bound = kLive;
 #pragma unroll
     for (int v = 1; v < VPL; ++v) lm = max(lm, key[v]);
-    for (int seen = 0;;) {
+    for (int i = 0; i < takes; ++i) {
         const unsigned m = __reduce_max_sync(FULL, lm);
+        bound = max(m, kLive);
         if (m < kLive) break;
-        seen += __popc(__ballot_sync(FULL, lm == m));
-        if (seen >= takes) { bound = m; break; }
         if (lm == m) lm = 0u;
     }
-    int count = 0;
-    const unsigned below = (1u << lane) - 1u;
+    int own = 0;
 #pragma unroll
-    for (int v = 0; v < VPL; ++v) {
-        const bool in = key[v] >= bound;
-        const unsigned who = __ballot_sync(FULL, in);
-        const int at = count + __popc(who & below);
-        if (in && at < 32) cand[at] = (unsigned long long)key[v] << 32 | (unsigned)(32 * v + lane);
-        count += __popc(who);
+    for (int v = 0; v < VPL; ++v) own += key[v] >= bound ? 1 : 0;
+    int at = own;                                    /* candidates of this and lower lanes */
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(FULL, at, o);
+        if (lane >= o) at += u;
     }
-    __syncwarp();
+    const int count = __shfl_sync(FULL, at, 31);
     if (count <= 32) {
+        at -= own;
+        if (own) {
+#pragma unroll
+            for (int v = 0; v < VPL; ++v)
+                if (key[v] >= bound) cand[at++] = (unsigned long long)key[v] << 32 | (unsigned)(VPL * lane + v);
+        }
+        __syncwarp();
         /* candidate `lane`, in ascending order of index; its rank among them */
         const unsigned long long c = lane < count ? cand[lane] : 0ull;
         const unsigned k = (unsigned)(c >> 32);
@@ -237,6 +300,7 @@ __device__ __forceinline__ void top_keys(unsigned (&key)[VPL], int takes, unsign
             mykey = (unsigned)(cand[lane] >> 32);
             mine = (int)(unsigned)cand[lane];
         }
+        __syncwarp();
     } else {
         /* many equal maxima: the maximum, takes times */
         for (int i = 0; i < takes; ++i) {
@@ -244,17 +308,16 @@ __device__ __forceinline__ void top_keys(unsigned (&key)[VPL], int takes, unsign
             int bj = INT_MAX;
 #pragma unroll
             for (int v = 0; v < VPL; ++v)
-                if (key[v] > bk) { bk = key[v]; bj = 32 * v + lane; }
+                if (key[v] > bk) { bk = key[v]; bj = VPL * lane + v; }
             const unsigned top = __reduce_max_sync(FULL, bk);
             if (top < kLive) break;
             const int j = __reduce_min_sync(FULL, bk == top ? bj : INT_MAX);
             if (lane == i) { mykey = top; mine = j; }
 #pragma unroll
             for (int v = 0; v < VPL; ++v)
-                if (32 * v + lane == j) key[v] = 0u;
+                if (VPL * lane + v == j) key[v] = 0u;
         }
     }
-    __syncwarp();
 }
 
 template <typename T, int VPL>
@@ -271,27 +334,21 @@ k_route(const T* __restrict__ logits, long long n, long long ld, const float* __
     const bool top2 = grouped && sh.group_score == MPK_GROUP_TOP2;
     const bool by_score = bias || top2;                       /* keys are choice values c, else logits */
     const bool scores = by_score || (softmax && !sh.renorm);  /* some use of all experts' scores */
-    const int L = lanes_per_group(sh.G);
-    /* the bias and the groups of this lane's experts, kept over the rows where registers allow */
+    const bool by_logit_after = top2 && !bias;                /* once groups are chosen, the logits' order again */
+    /* the bias of this lane's experts, kept over the rows where registers allow */
     constexpr bool KEEP = VPL <= 8;
     float bv[KEEP ? VPL : 1];
-    unsigned char gv[KEEP ? VPL : 1];
-    auto bias_of = [&](int v) { return 32 * v + lane < sh.E ? bias[32 * v + lane] : 0.f; };
-    auto group_of = [&](int v) { return (unsigned char)min(31u, ((unsigned)(32 * v + lane) * sh.gmul >> 20) * L); };
+    auto bias_of = [&](int v) { return VPL * lane + v < sh.E ? bias[VPL * lane + v] : 0.f; };
     if constexpr (KEEP) {
 #pragma unroll
-        for (int v = 0; v < VPL; ++v) {
-            bv[v] = bias ? bias_of(v) : 0.f;
-            gv[v] = group_of(v);
-        }
+        for (int v = 0; v < VPL; ++v) bv[v] = bias ? bias_of(v) : 0.f;
     }
     const long long step = (long long)gridDim.x * kRouteWarps;
     for (long long t = (long long)blockIdx.x * kRouteWarps + warp; t < n; t += step) {
         const T* row = logits + t * ld;
         float x[VPL];
         unsigned key[VPL];
-#pragma unroll
-        for (int v = 0; v < VPL; ++v) x[v] = 32 * v + lane < sh.E ? to_f(row[32 * v + lane]) : -INFINITY;
+        LaneRow<T, VPL>::load(row, sh.E, sh.vec, lane, x);
         float mx = 0.f, sum = 1.f, smax = 1.f;
         if (scores) {
             float c[VPL];
@@ -332,26 +389,47 @@ k_route(const T* __restrict__ logits, long long n, long long ld, const float* __
         };
         bool slow = false;
         if (grouped) {
+            unsigned gk;
+            bool in;
+            const int log = sh.log_g >= 0 ? sh.log_g : sh.log_l;
+            if (sh.log_g >= 0) {
+                unsigned a = 0u, b = 0u;
 #pragma unroll
-            for (int v = 0; v < VPL; ++v)
-                if (32 * v + lane < sh.E) keys32[32 * v + lane] = key[v];
-            __syncwarp();
-            const unsigned gk = group_key(keys32, sh, L, lane);
-            const unsigned kept = kept_groups(gk, sh, L, lane);
-            if (by_score) {
-                const int g = lane / L;
-                const bool there = lane == g * L && g < sh.G, in = (kept >> lane) & 1u;
-                const unsigned lo = __reduce_min_sync(FULL, there && in ? gk : 0xffffffffu);
+                for (int v = 0; v < VPL; ++v) {
+                    b = max(b, min(a, key[v]));
+                    a = max(a, key[v]);
+                }
+                for (int o = (1 << log) >> 1; o > 0; o >>= 1) {
+                    const unsigned a2 = __shfl_xor_sync(FULL, a, o), b2 = __shfl_xor_sync(FULL, b, o);
+                    merge2(a, b, a2, b2);
+                }
+                gk = group_of_two(a, b, sh.group_score);
+                in = group_kept(gk, sh, log, lane);
+#pragma unroll
+                for (int v = 0; v < VPL; ++v)
+                    key[v] = !in ? 0u : by_logit_after ? key_of(x[v]) : key[v];
+            } else {
+#pragma unroll
+                for (int v = 0; v < VPL; ++v)
+                    if (VPL * lane + v < sh.E) keys32[VPL * lane + v] = key[v];
+                __syncwarp();
+                gk = group_key(keys32, sh, lane);
+                in = group_kept(gk, sh, log, lane);
+                const unsigned kept = __ballot_sync(FULL, in);
+#pragma unroll
+                for (int v = 0; v < VPL; ++v) {
+                    const unsigned g = min(31u, ((unsigned)(VPL * lane + v) * sh.gmul >> 20) << log);
+                    if (!((kept >> g) & 1u) || VPL * lane + v >= sh.E) key[v] = 0u;
+                    else if (by_logit_after) key[v] = key_of(x[v]);
+                }
+                __syncwarp();
+            }
+            if (by_score) {                                        /* the groups on both sides of the cut */
+                const bool there = (lane >> log) < sh.G;
+                const unsigned lo = __reduce_min_sync(FULL, in ? gk : 0xffffffffu);
                 const unsigned hi = __reduce_max_sync(FULL, there && !in ? gk : 0u);
-                if (kept && live(hi)) slow = near(of_key(lo), of_key(hi));
+                if (live(hi)) slow = near(of_key(lo), of_key(hi));
             }
-#pragma unroll
-            for (int v = 0; v < VPL; ++v) {
-                const unsigned g = KEEP ? gv[KEEP ? v : 0] : group_of(v);
-                if (!((kept >> g) & 1u) || 32 * v + lane >= sh.E) key[v] = 0u;
-                else if (top2 && !bias) key[v] = key_of(x[v]);      /* groups chosen: the logits' order again */
-            }
-            __syncwarp();
         }
         int mine;
         unsigned mykey;
@@ -370,9 +448,9 @@ k_route(const T* __restrict__ logits, long long n, long long ld, const float* __
         const float xi = !valid ? -INFINITY : (bias || again) ? to_f(row[mine]) : of_key(mykey);
         float w;
         if (sh.renorm) {
-            const float m = warp_max(xi);
+            const float m = slot_max(xi, sh.log_k);
             const float e = valid ? chosen_score(xi, m, softmax) : 0.f;
-            const float total = warp_sum(e);
+            const float total = slot_sum(e, sh.log_k);
             w = total == 0.f ? 0.f : e / total;
             if (valid && sum != sum) w = NAN;
         } else {
@@ -413,12 +491,11 @@ k_route_grad(const T* __restrict__ logits, long long n, long long ld, RouteShape
 #pragma unroll
         for (int v = 0; v < VPL; ++v) acc[v] = 0.f;
         if (whole) {
-            float mx = -INFINITY, sum = 0.f;
+            float sum = 0.f;
+            LaneRow<T, VPL>::load(row, sh.E, sh.vec, lane, s);
+            float mx = s[0];
 #pragma unroll
-            for (int v = 0; v < VPL; ++v) {
-                s[v] = 32 * v + lane < sh.E ? to_f(row[32 * v + lane]) : -INFINITY;
-                mx = fmaxf(mx, s[v]);
-            }
+            for (int v = 1; v < VPL; ++v) mx = fmaxf(mx, s[v]);
             mx = warp_max(mx);
             if (mx == -INFINITY) mx = 0.f;
 #pragma unroll
@@ -427,42 +504,42 @@ k_route_grad(const T* __restrict__ logits, long long n, long long ld, RouteShape
             const float inv = sum == 0.f ? 0.f : 1.f / sum;        /* every expert masked: no gradient */
 #pragma unroll
             for (int v = 0; v < VPL; ++v) s[v] *= inv;
-            dot = warp_sum(valid ? g * (expf(xi - mx) * inv) : 0.f);
+            dot = slot_sum(valid ? g * (expf(xi - mx) * inv) : 0.f, sh.log_k);
+            dot = __shfl_sync(FULL, dot, 0);
             term = g;
         } else {
             const float si = valid ? 1.f / (1.f + expf(-xi)) : 0.f;
             const float left = softmax ? 1.f : 1.f / (1.f + expf(xi));      /* 1 - s */
             if (sh.renorm) {
-                const float m = warp_max(xi);
+                const float m = slot_max(xi, sh.log_k);
                 const float e = (!valid || m == -INFINITY) ? 0.f : chosen_score(xi, m, softmax);
-                const float total = warp_sum(e);
+                const float total = slot_sum(e, sh.log_k);
                 const float w = total == 0.f ? 0.f : e / total;
-                const float G = warp_sum(valid ? g * w : 0.f);
+                const float G = slot_sum(valid ? g * w : 0.f, sh.log_k);
                 term = w * left * (g - G);
             } else {
                 term = g * si * left;
             }
         }
         for (int i = 0; i < sh.k; ++i) {
-            const int j = __shfl_sync(FULL, id, i);
+            const int j = __shfl_sync(FULL, id, i) - VPL * lane;
             const float d = __shfl_sync(FULL, term, i);
-            if (j >= 0 && (j & 31) == lane) {
 #pragma unroll
-                for (int v = 0; v < VPL; ++v)
-                    if (v == (j >> 5)) acc[v] += d;
-            }
+            for (int v = 0; v < VPL; ++v) acc[v] += j == v ? d : 0.f;
         }
-        T* dst = out + t * ldg;
+        if (whole) {
 #pragma unroll
-        for (int v = 0; v < VPL; ++v)
-            if (32 * v + lane < sh.E) dst[32 * v + lane] = from_f<T>(whole ? s[v] * (acc[v] - dot) : acc[v]);
+            for (int v = 0; v < VPL; ++v) acc[v] = s[v] * (acc[v] - dot);
+        }
+        LaneRow<T, VPL>::store(out + t * ldg, sh.E, sh.vec, lane, acc);
     }
 }
 
 /* -------------------------------------------------------------- the plan ---- */
 /* A stable counting sort.  A block takes a chunk of the entries, each of its
- * warps a contiguous piece, 32 at a time: match_any gives the lanes that share an
- * expert, so an entry's rank among its expert's is (entries of earlier blocks) +
+ * warps a contiguous piece, 32 at a time: a ballot for each bit of the expert's
+ * number gives the lanes that share it (match_any takes longer the more experts a
+ * warp meets), so an entry's rank among its expert's is (entries of earlier blocks) +
  * (of earlier warps) + (of this warp so far) + (lower lanes of its match): no
  * atomics decide an order.  The block sorts its entries in shared memory first and
  * writes each expert's run in one piece.
@@ -477,6 +554,18 @@ constexpr int kPlanOne = 2 * kPlanChunk;
 __device__ __forceinline__ int plan_id(const int* ids, long long i, long long end, int E) {
     const int a = i < end ? ids[i] : -1;
     return (unsigned)a < (unsigned)E ? a : -1;
+}
+
+/* The lanes that have a's expert, `bits` bits of which tell experts apart; any for
+ * a < 0. */
+__device__ __forceinline__ unsigned same_expert(int a, int bits) {
+    unsigned m = __ballot_sync(FULL, a >= 0);
+    for (int b = 0; b < bits; ++b) {
+        const bool one = (a >> b) & 1;
+        const unsigned v = __ballot_sync(FULL, one);
+        m &= one ? v : ~v;
+    }
+    return m;
 }
 
 /* Exclusive scan of one int per thread over the block; tot receives the total. */
@@ -517,7 +606,7 @@ k_plan(const int* __restrict__ ids, long long m, int E, const int* __restrict__ 
     int* entry = local + E;                      /* CHUNK: the chunk's entries, sorted */
     unsigned short* owner = reinterpret_cast<unsigned short*>(entry + CHUNK);
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int B = gridDim.x;
+    const int B = gridDim.x, bits = 32 - __clz(E - 1);
     const long long lo = (long long)blockIdx.x * CHUNK + w * (32 * PER);
     int a[PER], rank[PER];
 #pragma unroll
@@ -527,7 +616,7 @@ k_plan(const int* __restrict__ ids, long long m, int E, const int* __restrict__ 
     int* mine = cnt + w * E;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        const unsigned peers = __match_any_sync(FULL, a[i]);
+        const unsigned peers = same_expert(a[i], bits);
         const int old = a[i] >= 0 ? mine[a[i]] : 0;
         rank[i] = old + __popc(peers & ((1u << lane) - 1u));
         __syncwarp();
@@ -630,7 +719,7 @@ bool route_shape(const mpkRouteParams* p, RouteShape& sh, bool choice) {
         p->top_k > p->experts || (p->score != MPK_SCORE_SOFTMAX && p->score != MPK_SCORE_SIGMOID) ||
         !std::isfinite(p->scale))
         return false;
-    sh = RouteShape{p->experts, p->top_k, p->score, 1, p->experts, 1, MPK_GROUP_MAX, p->renormalize ? 1 : 0, 0, p->scale};
+    sh = RouteShape{p->experts, p->top_k, p->score, 1, p->experts, 1, MPK_GROUP_MAX, p->renormalize ? 1 : 0, 0, p->scale, 0, 0, -1, 0};
     if (choice) {
         if (p->groups < 1 || p->groups > MPK_MAX_GROUPS || p->experts % p->groups || p->top_groups < 1 ||
             p->top_groups > p->groups || (p->group_score != MPK_GROUP_MAX && p->group_score != MPK_GROUP_TOP2))
@@ -640,6 +729,8 @@ bool route_shape(const mpkRouteParams* p, RouteShape& sh, bool choice) {
         sh.top_groups = p->top_groups;
         sh.group_score = p->group_score;
     }
+    while ((2 << sh.log_l) * sh.G <= 32) ++sh.log_l;
+    while ((1 << sh.log_k) < sh.k) ++sh.log_k;
     /* j * gmul / 2^20 exceeds j / gs by less than j / 2^20 < 1 / gs */
     sh.gmul = ((1u << 20) + sh.gs - 1) / sh.gs;
     return true;
@@ -658,9 +749,22 @@ int route_grid(long long n, int sms) {
     return (int)(b < (long long)sms * 16 ? b : (long long)sms * 16);
 }
 
+/* Addresses and row stride let a lane move its VPL elements as whole words. */
 template <typename T, int VPL>
-cudaError_t run_route(const RouteShape& sh, const void* logits, long long n, long long ld, const float* bias, int* ids,
+bool lane_words(const void* p, long long n, long long ld) {
+    constexpr int W = LaneRow<T, VPL>::WORD;
+    return reinterpret_cast<uintptr_t>(p) % W == 0 && (n <= 1 || ld * (long long)sizeof(T) % W == 0);
+}
+
+template <typename T, int VPL>
+cudaError_t run_route(RouteShape sh, const void* logits, long long n, long long ld, const float* bias, int* ids,
                       float* w, int sms, cudaStream_t s) {
+    sh.vec = lane_words<T, VPL>(logits, n, ld);
+    const int lanes = sh.gs / VPL;
+    if (sh.gs % VPL == 0 && (lanes & (lanes - 1)) == 0) {
+        sh.log_g = 0;
+        while ((1 << sh.log_g) < lanes) ++sh.log_g;
+    }
     const size_t smem = (bias || sh.G > 1) ? (size_t)kRouteWarps * sh.E * 8 : 0;
     k_route<T, VPL><<<route_grid(n, sms), 32 * kRouteWarps, smem, s>>>(static_cast<const T*>(logits), n, ld, bias, sh,
                                                                       ids, w);
@@ -668,8 +772,9 @@ cudaError_t run_route(const RouteShape& sh, const void* logits, long long n, lon
 }
 
 template <typename T, int VPL>
-cudaError_t run_route_grad(const RouteShape& sh, const void* logits, long long n, long long ld, const int* ids,
+cudaError_t run_route_grad(RouteShape sh, const void* logits, long long n, long long ld, const int* ids,
                            const float* gw, void* out, long long ldg, int sms, cudaStream_t s) {
+    sh.vec = lane_words<T, VPL>(logits, n, ld) && lane_words<T, VPL>(out, n, ldg);
     k_route_grad<T, VPL><<<route_grid(n, sms), 32 * kRouteWarps, 0, s>>>(static_cast<const T*>(logits), n, ld, sh, ids,
                                                                         gw, static_cast<T*>(out), ldg);
     return cudaGetLastError();
