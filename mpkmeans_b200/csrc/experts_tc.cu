@@ -565,9 +565,11 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
                                                : out + (long long)(t.r0 + t.j0) * p.ldo;
             const int nj = t.nj - half * K::HALF;                /* columns of this warp that exist */
             base += (long long)(half * K::HALF) * p.ldo;
+            /* the whole warp's 32 f's exist */
+            const bool inside = p.pairs && t.f0 + rank * BM + q * 32 + 32 <= p.F;
+            const long long two = 2 * p.ldo;
 #pragma unroll 1
-            for (int c = 0; c < K::HALF; c += CH) {
-                if (c >= nj) break;
+            for (int c = 0; c < K::HALF && c < nj; c += CH) {
                 uint32_t r[CH];
                 if (t.nk > 0) {
                     if constexpr (CH == 32) tmem_ld32(t_lane + (uint32_t)(tb * BN + c), r);
@@ -578,18 +580,26 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
                     for (int e = 0; e < CH; ++e) r[e] = 0u;
                 }
                 if (p.pairs) {
-                    const int fe = f - (odd ? 1 : 0);
-                    uint16_t* dst = base + (long long)(c + (odd ? 1 : 0)) * p.ldo + fe;
+                    /* columns e, e + 1 of this lane's f and of its neighbour's: the even lane takes column e
+                     * of both, the odd lane column e + 1 */
+                    uint32_t v[CH / 2];
 #pragma unroll
                     for (int e = 0; e < CH; e += 2) {
                         const uint32_t own = pack2(__uint_as_float(r[e]), __uint_as_float(r[e + 1]), FMT == 1);
-                        const uint32_t other = __shfl_xor_sync(0xffffffffu, own, 1);
-                        const uint32_t v = __byte_perm(own, other, sel);
-                        if (c + e + (odd ? 1 : 0) < nj) {
-                            if (fe + 1 < p.F) *reinterpret_cast<uint32_t*>(dst) = v;
-                            else if (fe < p.F) *dst = (uint16_t)v;
-                        }
-                        dst += 2 * p.ldo;
+                        v[e / 2] = __byte_perm(own, __shfl_xor_sync(0xffffffffu, own, 1), sel);
+                    }
+                    const int fe = f - (odd ? 1 : 0);
+                    uint16_t* dst = base + (long long)(c + (odd ? 1 : 0)) * p.ldo + fe;
+                    if (inside && c + CH <= nj) {
+#pragma unroll
+                        for (int e = 0; e < CH / 2; ++e, dst += two) *reinterpret_cast<uint32_t*>(dst) = v[e];
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < CH / 2; ++e, dst += two)
+                            if (c + 2 * e + (odd ? 1 : 0) < nj) {
+                                if (fe + 1 < p.F) *reinterpret_cast<uint32_t*>(dst) = v[e];
+                                else if (fe < p.F) *dst = (uint16_t)v[e];
+                            }
                     }
                 } else {
                     uint16_t* dst = base + (long long)c * p.ldo + f;
