@@ -71,18 +71,16 @@ __device__ int g_experts_status;
 constexpr int BM = 128, BK = 64;
 constexpr int kEpiWarps = 8;
 constexpr int kGatherWarps = 6;
-constexpr int kFewRows = 32;                     /* j's of a tile where experts have few rows */
 constexpr int BROWS = 32;                        /* rows of one K-major box of B */
 constexpr int A_STAGE = BM * BK * 2;             /* 16 KB */
 constexpr int BOX = 64 * 64 * 2;                 /* one 64 x 64 MN-major box */
 constexpr int kSmemMax = 232448;
-constexpr int kMisc = 1024 + 4 * (MPK_MAX_EXPERTS + 1);
-constexpr int kSched = 3;                        /* work indices between the producer and the epilogue */
+constexpr int kMisc = 1024 + 8 * (MPK_MAX_EXPERTS + 1);
+constexpr int kInfo = 4;                         /* tiles between the producer and the epilogue */
 constexpr int kGroup = 8;                        /* row tiles that sweep the f tiles together */
 
-template <bool PAIR>
+template <bool PAIR, int BN>
 struct Cfg {
-    static constexpr int BN = PAIR ? 256 : kFewRows;           /* j's of a tile, at most */
     static constexpr int BL = PAIR ? BN / 2 : BN;              /* j's this CTA stages */
     static constexpr int FT = PAIR ? 2 * BM : BM;              /* f's of one tile */
     static constexpr int B_STAGE = BL * BK * 2;
@@ -99,10 +97,24 @@ struct Cfg {
     static_assert(STAGE % 1024 == 0, "swizzle atoms");
 };
 
+/* One tile of one expert's output. */
+struct Tile {
+    int u;                      /* its index; -1: there are no more */
+    int e;
+    int r0, rows;               /* the expert's sorted rows */
+    int j0, nj;                 /* first output row inside the expert, rows of this tile (0: an index past the tiles) */
+    int wide;                   /* columns of the MMA */
+    int f0;
+    int nk;                     /* 64-deep contraction steps */
+    int pad[3];
+};
+static_assert(sizeof(Tile) % 16 == 0, "moved in 16-byte words");
+
 template <int STAGES>
 struct EMisc {
-    uint4 next[kSched];         /* the scheduler's answers */
-    uint64_t full[STAGES], empty[STAGES], t_full[2], t_empty[2], s_full[kSched], s_empty[kSched], fin;
+    uint4 next[2];              /* answers to ask_next */
+    Tile info[kInfo];           /* the tiles the producer has started */
+    uint64_t full[STAGES], empty[STAGES], t_full[2], t_empty[2], s_full[2], s_empty[2], i_full[kInfo], i_empty[kInfo], fin;
     uint32_t tmem_slot;
     int abort_flag;
 };
@@ -188,51 +200,66 @@ __device__ __forceinline__ void mbar_expect_tx_cluster(uint32_t cluster_addr, ui
     asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" :: "r"(cluster_addr), "r"(bytes) : "memory");
 }
 
-/* One tile of one expert's output. */
-struct Tile {
-    int e;
-    int r0, rows;               /* the expert's sorted rows */
-    int j0, nj;                 /* first output row inside the expert, rows of this tile */
-    int wide;                   /* columns of the MMA */
-    int f0;
-    int nk;                     /* 64-deep contraction steps */
-};
-
 /* The tiles of all experts in the order they are worked on: expert by expert,
  * inside one kGroup row tiles at a time, their f tiles in turn, the row tiles
- * innermost -- CTAs that run together then share a few tiles of W and of X, and
- * a weight matrix larger than L2 is read once per kGroup row tiles.
- * start[e] is the first row tile of expert e. */
+ * innermost -- clusters that run together then share a few tiles of W and of X, and
+ * a weight matrix larger than L2 is read once per kGroup row tiles.  start[e] is
+ * the first row tile of expert e, row[e] its first sorted row. */
 template <int MODE, int BN, int FTILE>
 struct Tiles {
-    const Params& p;
     const int* start;
+    const int* row;
+    int experts, J, nk;
     int ft;                     /* f tiles */
     int e;
-    __device__ Tiles(const Params& p_, const int* start_) : p(p_), start(start_), ft((p_.F + FTILE - 1) / FTILE), e(0) {}
-    __device__ long long total() const { return (long long)start[p.experts] * ft; }
+    __device__ Tiles(const Params& p, const int* start_, const int* row_)
+        : start(start_), row(row_), experts(p.experts), J(p.J), nk((p.C + BK - 1) / BK), ft((p.F + FTILE - 1) / FTILE), e(0) {}
     /* u mostly ascends from call to call */
-    __device__ Tile at(long long u) {
+    __device__ Tile at(int u) {
+        Tile t;
+        t.u = u;
+        t.e = 0;
+        t.r0 = t.rows = t.j0 = t.nj = t.wide = t.f0 = t.nk = 0;
+        if (u >= (long long)start[experts] * ft) return t;
         if ((long long)start[e] * ft > u) e = 0;
         while ((long long)start[e + 1] * ft <= u) ++e;
-        Tile t;
         t.e = e;
         const int l0 = start[e], count = start[e + 1] - l0;
-        const long long l = u - (long long)l0 * ft;
-        const int g = (int)(l / ((long long)kGroup * ft));
-        const int rem = (int)(l - (long long)g * kGroup * ft);
+        const int l = (int)(u - (long long)l0 * ft);
+        const int g = l / (kGroup * ft);
+        const int rem = l - g * kGroup * ft;
         const int in = min(kGroup, count - g * kGroup);
-        const int jt = g * kGroup + rem % in;
-        t.f0 = rem / in * FTILE;
-        t.j0 = jt * BN;
-        t.r0 = expert_start(p.offsets, e, p.m);
-        t.rows = max(expert_start(p.offsets, e + 1, p.m) - t.r0, 0);
-        t.nj = min(BN, (MODE == EXP_GRADW ? p.J : t.rows) - t.j0);
+        const int f = rem / in;
+        t.f0 = f * FTILE;
+        t.j0 = (g * kGroup + rem - f * in) * BN;
+        t.r0 = row[e];
+        t.rows = max(row[e + 1] - t.r0, 0);
+        t.nj = min(BN, (MODE == EXP_GRADW ? J : t.rows) - t.j0);
         t.wide = min(BN, (t.nj + 31) & ~31);
-        t.nk = ((MODE == EXP_GRADW ? t.rows : p.C) + BK - 1) / BK;
+        t.nk = MODE == EXP_GRADW ? (t.rows + BK - 1) / BK : nk;
         return t;
     }
 };
+
+/* Waits for a warp's TMEM loads; the registers pass through, so that no use of them
+ * can be placed before the wait. */
+template <int N>
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[N]) {
+    static_assert(N == 16 || N == 32, "one load");
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :: "memory");
+    if constexpr (N == 32)
+        asm volatile("" : "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                          "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                          "+r"(r[30]), "+r"(r[31]) :: "memory");
+}
+template <int N>
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[N]) {
+    if constexpr (N == 32) tmem_ld32(taddr, r);
+    else tmem_ld16(taddr, r);
+}
 
 __device__ __forceinline__ uint32_t pack2(float a, float b, bool bf16) {
     uint32_t r;
@@ -241,24 +268,24 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, bool bf16) {
     return r;
 }
 
-template <int MODE, bool PAIR, int FMT>
-__global__ void __launch_bounds__(Cfg<PAIR>::THREADS, 1)
+template <int MODE, bool PAIR, int BN, int FMT>
+__global__ void __launch_bounds__(Cfg<PAIR, BN>::THREADS, 1)
 k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
              const __grid_constant__ CUtensorMap tmAg, const __grid_constant__ CUtensorMap tmBg,
              const __grid_constant__ CUtensorMap tmAt, const __grid_constant__ CUtensorMap tmBt, const Params p) {
     static_assert(PAIR || MODE != EXP_GRADW, "the weights' gradient runs on pairs");
-    using K = Cfg<PAIR>;
-    constexpr int STAGES = K::STAGES, STAGE = K::STAGE, BN = K::BN, BL = K::BL;
+    using K = Cfg<PAIR, BN>;
+    constexpr int STAGES = K::STAGES, STAGE = K::STAGE, BL = K::BL;
     constexpr bool A_MN = MODE != EXP_FWD, B_MN = MODE == EXP_GRADW;
     const bool gathers = !PAIR && p.order != nullptr;
     static_assert(sizeof(EMisc<STAGES>) <= 1024, "misc");
     extern __shared__ __align__(1024) uint8_t smem[];
     EMisc<STAGES>& ms = *reinterpret_cast<EMisc<STAGES>*>(smem + STAGES * STAGE);
     int* start = reinterpret_cast<int*>(smem + STAGES * STAGE + 1024);
+    int* first = start + MPK_MAX_EXPERTS + 1;
     volatile int* abort_flag = &ms.abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = PAIR ? (int)cluster_rank() : 0;
-    const long long u0 = PAIR ? blockIdx.x >> 1 : blockIdx.x, units = PAIR ? gridDim.x >> 1 : gridDim.x;
 
     if (smem_u32(smem) & 1023u) {
         if (threadIdx.x == 0) atomicOr(&g_experts_status, MPK_DEV_TIMEOUT);
@@ -269,9 +296,10 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
         const int arrivals = gathers ? 2 : 1;
         for (int i = 0; i < STAGES; ++i) { mbar_init(&ms.full[i], arrivals); mbar_init(&ms.empty[i], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&ms.t_full[i], 1); mbar_init(&ms.t_empty[i], (PAIR ? 2 : 1) * kEpiWarps); }
-        /* a work index is read by producer, MMA issuer (CTA 0 only), epilogue and gather warps */
-        const int readers = PAIR ? 2 * (1 + kEpiWarps) + 1 : 2 + kEpiWarps + (gathers ? kGatherWarps : 0);
-        for (int i = 0; i < kSched; ++i) { mbar_init(&ms.s_full[i], 1); mbar_init(&ms.s_empty[i], readers); }
+        /* answers are read by the producers, tiles by this CTA's MMA issuer, epilogue and gather warps */
+        for (int i = 0; i < 2; ++i) { mbar_init(&ms.s_full[i], 1); mbar_init(&ms.s_empty[i], PAIR ? 2 : 1); }
+        const int readers = (rank == 0 ? 1 : 0) + kEpiWarps + (gathers ? kGatherWarps : 0);
+        for (int i = 0; i < kInfo; ++i) { mbar_init(&ms.i_full[i], 1); mbar_init(&ms.i_empty[i], readers); }
         mbar_init(&ms.fin, 1);
         ms.abort_flag = 0;
         fence_mbar_init();
@@ -281,15 +309,16 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
         if (PAIR) tmem_alloc_pair(&ms.tmem_slot, K::TMEM_COLS);
         else tmem_alloc(&ms.tmem_slot, K::TMEM_COLS);
     }
-    if (warp == 2) {                             /* first row tile of every expert */
+    if (warp == 2) {                             /* first row tile and first row of every expert */
         int run = 0;
         for (int e0 = 0; e0 < p.experts; e0 += 32) {
             const int e = e0 + lane;
             int t = 0;
             if (e < p.experts) {
-                const int rows = MODE == EXP_GRADW ? p.J
-                    : max(expert_start(p.offsets, e + 1, p.m) - expert_start(p.offsets, e, p.m), 0);
+                const int r = expert_start(p.offsets, e, p.m);
+                const int rows = MODE == EXP_GRADW ? p.J : max(expert_start(p.offsets, e + 1, p.m) - r, 0);
                 t = (rows + BN - 1) / BN;
+                first[e] = r;
             }
             int incl = t;
             for (int o = 1; o < 32; o <<= 1) {
@@ -299,68 +328,73 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
             if (e < p.experts) start[e] = run + incl - t;
             run += __shfl_sync(0xffffffffu, incl, 31);
         }
-        if (lane == 0) start[p.experts] = run;
+        if (lane == 0) {
+            start[p.experts] = run;
+            first[p.experts] = expert_start(p.offsets, p.experts, p.m);
+        }
     }
     tc_fence_before();
     if (PAIR) cluster_sync();
     else __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = ms.tmem_slot;
-    Tiles<MODE, BN, K::FT> tiles(p, start);
-    const long long total = tiles.total();
 
-    /* the next tile's index, for one thread; false when there is none (or a wait ran out) */
+    /* The next tile, for a whole warp or (LONE) for its lane 0 alone; false when there is none or a wait
+     * ran out. */
     int taken = 0;
-    auto next = [&](long long& u) {
-        const int sl = taken % kSched;
-        if (!mbar_wait(&ms.s_full[sl], (uint32_t)(taken / kSched) & 1u, abort_flag, &g_experts_status)) return false;
-        const int x = read_next(&ms.next[sl]);
-        fence_async_proxy();
-        if (PAIR) mbar_arrive_cluster(peer_addr(&ms.s_empty[sl], 0));
-        else mbar_arrive(&ms.s_empty[sl]);
+    auto take = [&](Tile& t, bool lone) {
+        const int sl = taken % kInfo;
+        const uint32_t parity = (uint32_t)(taken / kInfo) & 1u;
         ++taken;
-        u = PAIR ? x >> 1 : x;
-        return x >= 0;
-    };
-    /* the same for a whole warp */
-    auto next_warp = [&](long long& u) {
-        int go = 0;
-        if (lane == 0) go = next(u) ? 1 : 0;
-        u = __shfl_sync(0xffffffffu, u, 0);
-        return __shfl_sync(0xffffffffu, go, 0) != 0;
+        if (lone ? !mbar_wait(&ms.i_full[sl], parity, abort_flag, &g_experts_status)
+                 : !wait_warp(&ms.i_full[sl], parity, abort_flag)) return false;
+        t = ms.info[sl];
+        if (!lone) __syncwarp();
+        if (lane == 0) mbar_arrive(&ms.i_empty[sl]);
+        return t.u >= 0;
     };
 
     if (warp == 0) {
         /* ------------------------------------------------- producer ---- */
+        Tiles<MODE, BN, K::FT> tiles(p, start, first);
         uint32_t last[STAGES];
 #pragma unroll
         for (int i = 0; i < STAGES; ++i) last[i] = 0xffffffffu;
         uint32_t it = 0;
-        int asked = -1;
+        int u = PAIR ? blockIdx.x >> 1 : blockIdx.x;
+        int told = 0, asked = 0;                 /* tiles passed on, indices asked for */
         bool ok = true;
-        bool more = true;
-        for (long long u = u0; more && ok; more = ok && next_warp(u)) {
-            if (lane == 0 && rank == 0) {                        /* one index ahead of the loads, no more: it is taken for good */
-                const int sl = taken % kSched;
-                const uint32_t use = (uint32_t)(taken / kSched);
-                ok = mbar_wait(&ms.s_empty[sl], (use & 1u) ^ 1u, abort_flag, &g_experts_status);
+        while (ok) {
+            /* The next index is asked for as this tile starts, no earlier: once given it is this cluster's. */
+            if (lane == 0 && rank == 0 && u >= 0) {
+                const int sl = asked & 1;
+                ok = mbar_wait(&ms.s_empty[sl], ((uint32_t)(asked >> 1) & 1u) ^ 1u, abort_flag, &g_experts_status);
                 if (ok) {
                     mbar_expect_tx(&ms.s_full[sl], 16);
                     if (PAIR) mbar_expect_tx_cluster(peer_addr(&ms.s_full[sl], 1), 16);
                     ask_next<PAIR>(&ms.next[sl], &ms.s_full[sl]);
-                    asked = taken;
                 }
             }
-            ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-            if (!ok) break;
-            if (u >= total) continue;
-            const Tile t = tiles.at(u);
+            if (!__shfl_sync(0xffffffffu, ok ? 1 : 0, 0)) { ok = false; break; }
+            if (u >= 0) ++asked;
+            Tile t = tiles.at(u < 0 ? 0x7fffffff : u);
+            t.u = u;
+            {
+                const int sl = told % kInfo;
+                if (!wait_warp(&ms.i_empty[sl], ((uint32_t)(told / kInfo) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+                if (lane == 0) {
+                    ms.info[sl] = t;
+                    mbar_arrive(&ms.i_full[sl]);
+                }
+                ++told;
+            }
+            if (u < 0) break;
             const int f0 = t.f0 + rank * BM;                     /* this CTA's f's */
             const int jn = PAIR ? t.wide / 2 : BN;               /* and j's */
             const int jl = t.j0 + rank * jn;
             const int end = t.r0 + t.rows;
             const int boxes = MODE == EXP_GRADW ? (jn + 63) / 64 : (jn + BROWS - 1) / BROWS;
-            uint32_t bytes = A_STAGE + (gathers ? 0 : boxes * (MODE == EXP_GRADW ? BOX : BROWS * BK * 2));
+            const uint32_t bytes = A_STAGE + (gathers ? 0 : boxes * (MODE == EXP_GRADW ? BOX : BROWS * BK * 2));
             /* GRADW's last stage: lane l fetches rows 4 (l mod 16) .. of the 64-element chunk l / 16 */
             const int q4 = 4 * (lane & 15), ch = lane >> 4;
             for (int kc = 0; kc < t.nk; ++kc, ++it) {
@@ -416,9 +450,26 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
                     }
                 }
             }
+            if (!ok) break;
+            /* the answer to this tile's question */
+            const int sl = (asked - 1) & 1;
+            int x = -1, got = 0;
+            if (lane == 0) {
+                got = mbar_wait(&ms.s_full[sl], (uint32_t)((asked - 1) >> 1) & 1u, abort_flag, &g_experts_status) ? 1 : 0;
+                if (got) {
+                    x = read_next(&ms.next[sl]);
+                    fence_async_proxy();
+                    if (PAIR) mbar_arrive_cluster(peer_addr(&ms.s_empty[sl], 0));
+                    else mbar_arrive(&ms.s_empty[sl]);
+                }
+            }
+            ok = __shfl_sync(0xffffffffu, got, 0) != 0;
+            x = __shfl_sync(0xffffffffu, x, 0);
+            u = x < 0 ? -1 : PAIR ? x >> 1 : x;
         }
         if (!ok && lane == 0) {
-            if (asked >= 0) drain_wait(&ms.s_full[asked % kSched], (uint32_t)(asked / kSched) & 1u);
+            /* let what is in flight land before the CTA exits */
+            if (asked > 0) drain_wait(&ms.s_full[(asked - 1) & 1], (uint32_t)((asked - 1) >> 1) & 1u);
             if (!PAIR) {
 #pragma unroll
                 for (int i = 0; i < STAGES; ++i)
@@ -444,11 +495,9 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
             };
             uint32_t it = 0, ts = 0;
             bool ok = true;
-            bool more = true;
-            for (long long u = u0; more && ok; more = ok && next(u)) {
-                if (u >= total) continue;
-                const Tile t = tiles.at(u);
-                if (t.nk == 0) continue;
+            Tile t;
+            while (ok && take(t, true)) {
+                if (t.nk == 0 || t.nj == 0) continue;
                 const int tb = (int)(ts & 1u);
                 if (!mbar_wait(&ms.t_empty[tb], ((ts >> 1) & 1u) ^ 1u, abort_flag, &g_experts_status)) { ok = false; break; }
                 tc_fence_after();
@@ -497,10 +546,8 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
             uint32_t it0 = 0, it = (uint32_t)w;                  /* first stage of the tile; this warp's next */
             bool ok = true;
             int idx[N];
-            bool more = true;
-            for (long long u = u0; more && ok; more = ok && next_warp(u)) {
-                if (u >= total) continue;
-                const Tile t = tiles.at(u);
+            Tile t;
+            while (ok && take(t, false)) {
                 const int end = t.r0 + t.rows;
                 const uint32_t it1 = it0 + (uint32_t)t.nk;
                 if (it < it1) {                                  /* token rows, -1 past the segment */
@@ -535,50 +582,34 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
         }
     } else {
         /* --------------------------------------------------- epilogue --- */
-        constexpr int CH = K::CH;
+        constexpr int CH = K::CH, HALF = K::HALF;
         const int half = (warp - 2) >> 2;         /* which columns of the tile */
         const int q = warp & 3;                   /* TMEM lane quarter */
-        const uint32_t t_lane = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * K::HALF);
-        const bool odd = lane & 1;
+        const uint32_t t_lane = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * HALF);
+        const int odd = lane & 1;
         const uint32_t sel = odd ? 0x3276u : 0x5410u;
+        const int units = PAIR ? gridDim.x >> 1 : gridDim.x;
+        const int valid = first[p.experts];
+        const long long two = 2 * p.ldo;
         uint16_t* out = static_cast<uint16_t*>(p.out);
-        bool ok = true, more = true;
+        bool ok = true;
         uint32_t ts = 0;
-        const int valid = expert_start(p.offsets, p.experts, p.m);
-        for (long long u = u0; more && ok; more = ok && next_warp(u)) {
+        Tile t;
+        while (ok && take(t, false)) {
             if (MODE != EXP_GRADW) {              /* rows that no expert owns: each index sets its share to zero */
-                for (long long r = valid + u; r < p.m; r += units)
-                    for (int f = rank * 32 * kEpiWarps + threadIdx.x - 64; f < p.F; f += (PAIR ? 2 : 1) * 32 * kEpiWarps)
+                for (long long r = (long long)valid + t.u; r < p.m; r += units)
+                    for (int f = rank * 32 * kEpiWarps + (int)threadIdx.x - 64; f < p.F; f += (PAIR ? 2 : 1) * 32 * kEpiWarps)
                         out[r * p.ldo + f] = 0;
             }
-            if (u >= total) continue;
-            const Tile t = tiles.at(u);
-            const int tb = (int)(ts & 1u);
-            if (t.nk > 0) {
-                if (ok) ok = wait_warp(&ms.t_full[tb], (ts >> 1) & 1u, abort_flag);
-                ++ts;
-                if (!ok) continue;
-                tc_fence_after();
-            }
+            if (t.nj == 0) continue;
             const int f = t.f0 + rank * BM + q * 32 + lane;
             uint16_t* base = MODE == EXP_GRADW ? out + (long long)t.e * p.stride_o + (long long)t.j0 * p.ldo
                                                : out + (long long)(t.r0 + t.j0) * p.ldo;
-            const int nj = t.nj - half * K::HALF;                /* columns of this warp that exist */
-            base += (long long)(half * K::HALF) * p.ldo;
+            const int nj = t.nj - half * HALF;                   /* columns of this warp that exist */
+            base += (long long)(half * HALF) * p.ldo;
             /* the whole warp's 32 f's exist */
             const bool inside = p.pairs && t.f0 + rank * BM + q * 32 + 32 <= p.F;
-            const long long two = 2 * p.ldo;
-#pragma unroll 1
-            for (int c = 0; c < K::HALF && c < nj; c += CH) {
-                uint32_t r[CH];
-                if (t.nk > 0) {
-                    if constexpr (CH == 32) tmem_ld32(t_lane + (uint32_t)(tb * BN + c), r);
-                    else tmem_ld16(t_lane + (uint32_t)(tb * BN + c), r);
-                    tmem_ld_wait();
-                } else {
-#pragma unroll
-                    for (int e = 0; e < CH; ++e) r[e] = 0u;
-                }
+            auto put = [&](const uint32_t (&r)[CH], int c) {
                 if (p.pairs) {
                     /* columns e, e + 1 of this lane's f and of its neighbour's: the even lane takes column e
                      * of both, the odd lane column e + 1 */
@@ -588,15 +619,15 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
                         const uint32_t own = pack2(__uint_as_float(r[e]), __uint_as_float(r[e + 1]), FMT == 1);
                         v[e / 2] = __byte_perm(own, __shfl_xor_sync(0xffffffffu, own, 1), sel);
                     }
-                    const int fe = f - (odd ? 1 : 0);
-                    uint16_t* dst = base + (long long)(c + (odd ? 1 : 0)) * p.ldo + fe;
+                    const int fe = f - odd;
+                    uint16_t* dst = base + (long long)(c + odd) * p.ldo + fe;
                     if (inside && c + CH <= nj) {
 #pragma unroll
                         for (int e = 0; e < CH / 2; ++e, dst += two) *reinterpret_cast<uint32_t*>(dst) = v[e];
                     } else {
 #pragma unroll
                         for (int e = 0; e < CH / 2; ++e, dst += two)
-                            if (c + 2 * e + (odd ? 1 : 0) < nj) {
+                            if (c + 2 * e + odd < nj) {
                                 if (fe + 1 < p.F) *reinterpret_cast<uint32_t*>(dst) = v[e];
                                 else if (fe < p.F) *dst = (uint16_t)v[e];
                             }
@@ -609,13 +640,43 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
                         dst += p.ldo;
                     }
                 }
+            };
+            if (t.nk == 0) {                                     /* an expert without rows */
+                uint32_t r[CH];
+#pragma unroll
+                for (int e = 0; e < CH; ++e) r[e] = 0u;
+#pragma unroll 1
+                for (int c = 0; c < HALF && c < nj; c += CH) put(r, c);
+                continue;
             }
-            if (t.nk > 0) {
+            const int tb = (int)(ts & 1u);
+            if (!wait_warp(&ms.t_full[tb], (ts >> 1) & 1u, abort_flag)) { ok = false; break; }
+            ++ts;
+            tc_fence_after();
+            /* the accumulator is free again once its last columns are in registers */
+            auto release = [&]() {
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) {
                     if (PAIR) mbar_arrive_cluster(peer_addr(&ms.t_empty[tb], 0));
                     else mbar_arrive(&ms.t_empty[tb]);
+                }
+            };
+            const uint32_t col = t_lane + (uint32_t)(tb * BN);
+            if (nj <= 0) {
+                release();
+                continue;
+            }
+            const int chunks = min(HALF / CH, (nj + CH - 1) / CH);
+            uint32_t r[2][CH];
+            tmem_load(col, r[0]);
+#pragma unroll
+            for (int c = 0; c < HALF / CH; ++c) {
+                if (c < chunks) {
+                    tmem_wait(r[c & 1]);
+                    if (c + 1 < chunks) tmem_load(col + (uint32_t)((c + 1) * CH), r[(c + 1) & 1]);
+                    else release();
+                    put(r[c & 1], c * CH);
                 }
             }
         }
@@ -662,11 +723,10 @@ bool row_map(CUtensorMap* map, const void* base, bool bf16, long long cols, long
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int MODE, bool PAIR, int FMT>
+template <int MODE, bool PAIR, int BN, int FMT>
 cudaError_t launch_t(const ExpertArgs& a, cudaStream_t s) {
-    using K = Cfg<PAIR>;
-    constexpr int BN = K::BN;
-    auto kern = k_experts_tc<MODE, PAIR, FMT>;
+    using K = Cfg<PAIR, BN>;
+    auto kern = k_experts_tc<MODE, PAIR, BN, FMT>;
     CUtensorMap tmA{}, tmB{}, tmAg{}, tmBg{}, tmAt{}, tmBt{};
     bool ok;
     if (MODE == EXP_FWD) {
@@ -716,19 +776,25 @@ cudaError_t launch_t(const ExpertArgs& a, cudaStream_t s) {
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 
+/* Tile widths by the average expert's rows; see experts_few_rows for FWD's few.  A
+ * pair's 64-wide tile has ten stages of W in flight, the 256-wide one six. */
 template <int FMT>
 cudaError_t launch_fmt(const ExpertArgs& a, cudaStream_t s) {
-    if (a.mode == EXP_GRADW) return launch_t<EXP_GRADW, true, FMT>(a, s);
-    if (experts_few_rows(a.m, a.experts))
-        return a.mode == EXP_FWD ? launch_t<EXP_FWD, false, FMT>(a, s) : launch_t<EXP_GRADX, false, FMT>(a, s);
-    return a.mode == EXP_FWD ? launch_t<EXP_FWD, true, FMT>(a, s) : launch_t<EXP_GRADX, true, FMT>(a, s);
+    const long long rows = a.m / a.experts;
+    if (a.mode == EXP_GRADW) return launch_t<EXP_GRADW, true, 256, FMT>(a, s);
+    if (a.mode == EXP_GRADX) {
+        if (rows <= 2) return launch_t<EXP_GRADX, false, 32, FMT>(a, s);
+        return rows <= 48 ? launch_t<EXP_GRADX, true, 64, FMT>(a, s) : launch_t<EXP_GRADX, true, 256, FMT>(a, s);
+    }
+    if (experts_few_rows(a.m, a.experts)) return launch_t<EXP_FWD, false, 32, FMT>(a, s);
+    return rows <= 48 ? launch_t<EXP_FWD, true, 64, FMT>(a, s) : launch_t<EXP_FWD, true, 256, FMT>(a, s);
 }
 
 bool rows16(const void* q, long long ld) { return reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld % 8 == 0; }
 
 }  /* namespace */
 
-bool experts_few_rows(long long m, int experts) { return m / experts <= 24; }
+bool experts_few_rows(long long m, int experts) { return m / experts <= 12; }
 
 bool experts_tc_ok(const ExpertArgs& a) {
     /* TMA addresses and strides: 16-byte steps, strides below 2^40 bytes; one row has no stride */
