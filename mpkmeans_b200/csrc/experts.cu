@@ -177,6 +177,148 @@ cudaError_t launch_any(const ExpertArgs& a, cudaStream_t s) {
     return cudaGetLastError();
 }
 
+/* ------------------------------------------------- products of few rows ---- */
+
+constexpr int kFewThreads = 256;
+constexpr int kFewF = 4;                     /* outputs a warp forms at a time */
+constexpr int kFewBlockF = kFewF * kFewThreads / 32;
+
+template <typename T>
+__device__ __forceinline__ float2 two_floats(uint32_t u);
+template <>
+__device__ __forceinline__ float2 two_floats<__half>(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
+template <>
+__device__ __forceinline__ float2 two_floats<__nv_bfloat16>(uint32_t u) {
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+
+/* Eight elements from column c of a row; zeros past k, which nothing is read of. */
+template <typename T>
+__device__ __forceinline__ uint4 eight(const T* row, int c, int k) {
+    if (c + 8 <= k) return *reinterpret_cast<const uint4*>(row + c);
+    uint4 u = make_uint4(0u, 0u, 0u, 0u);
+    T* t = reinterpret_cast<T*>(&u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (c + i < k) t[i] = row[c + i];
+    return u;
+}
+
+/* R rows of one expert (from sorted row r, there of them real) times kFewF of its
+ * outputs from f: lane l takes elements 8 l ... of every 256.  Rows and outputs
+ * that do not exist repeat one that does, so that no load waits on a branch. */
+template <typename T, int R>
+__device__ __forceinline__ void few_rows(const ExpertArgs& a, const T* we, int f, int r, int there, int lane) {
+    const T* x[R];
+    const T* w[kFewF];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const long long q = x_row(a, r + min(i, there - 1));
+        x[i] = static_cast<const T*>(a.x) + max(q, 0LL) * a.ldx;
+    }
+#pragma unroll
+    for (int j = 0; j < kFewF; ++j) w[j] = we + (long long)min(f + j, a.width - 1) * a.ldw;
+    float acc[kFewF][R] = {};
+    auto step = [&](const uint4 (&uw)[kFewF], const uint4 (&ux)[R]) {
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            float2 fx[R];
+#pragma unroll
+            for (int i = 0; i < R; ++i) fx[i] = two_floats<T>((&ux[i].x)[h]);
+#pragma unroll
+            for (int j = 0; j < kFewF; ++j) {
+                const float2 fw = two_floats<T>((&uw[j].x)[h]);
+#pragma unroll
+                for (int i = 0; i < R; ++i) acc[j][i] = fmaf(fw.y, fx[i].y, fmaf(fw.x, fx[i].x, acc[j][i]));
+            }
+        }
+    };
+    constexpr int U = R <= 2 ? 4 : 2;        /* steps whose loads are in flight together */
+    int c = 8 * lane;
+    const int whole = a.k / (256 * U) * (256 * U);
+    for (; c < whole; c += 256 * U) {
+        uint4 uw[U][kFewF], ux[U][R];
+#pragma unroll
+        for (int t = 0; t < U; ++t) {
+#pragma unroll
+            for (int j = 0; j < kFewF; ++j) uw[t][j] = __ldcs(reinterpret_cast<const uint4*>(w[j] + c + 256 * t));
+#pragma unroll
+            for (int i = 0; i < R; ++i) ux[t][i] = *reinterpret_cast<const uint4*>(x[i] + c + 256 * t);
+        }
+#pragma unroll
+        for (int t = 0; t < U; ++t) step(uw[t], ux[t]);
+    }
+    for (; c < a.k; c += 256) {
+        uint4 uw[kFewF], ux[R];
+#pragma unroll
+        for (int j = 0; j < kFewF; ++j) uw[j] = eight(w[j], c, a.k);
+#pragma unroll
+        for (int i = 0; i < R; ++i) ux[i] = eight(x[i], c, a.k);
+        step(uw, ux);
+    }
+    float mine = 0.f;                        /* lane j * R + i ends with output j of row i */
+#pragma unroll
+    for (int j = 0; j < kFewF; ++j)
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            float v = acc[j][i];
+            for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+            if (lane == j * R + i) mine = v;
+        }
+    const int j = lane / R, i = lane % R;
+    if (j < kFewF && i < there && f + j < a.width)
+        static_cast<T*>(a.out)[(long long)(r + i) * a.ldo + f + j] = from_f<T>(mine);
+}
+
+/* FWD for a handful of rows: bound by reading the chosen experts' matrices once,
+ * which many small pieces spread over the SMs better than 128-row tiles do (eight
+ * experts of 1536 x 2048 make 96 tiles, 384 blocks here).  blockIdx.y counts the
+ * experts that have rows, blockIdx.x their outputs, kFewBlockF a block; four rows
+ * at a time share a pass over W. */
+template <typename T>
+__global__ void __launch_bounds__(kFewThreads, 2) k_experts_few(const ExpertArgs a) {
+    __shared__ int found;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, m = (int)a.m;
+    if (warp == 0) {                         /* the blockIdx.y-th expert with rows */
+        int seen = 0, e = -1;
+        for (int e0 = 0; e0 < a.experts && e < 0; e0 += 32) {
+            const int q = e0 + lane;
+            const bool some = q < a.experts && expert_start(a.offsets, q + 1, m) > expert_start(a.offsets, q, m);
+            unsigned who = __ballot_sync(FULL, some);
+            const int more = __popc(who);
+            if (seen + more > (int)blockIdx.y) {
+                for (int skip = (int)blockIdx.y - seen; skip > 0; --skip) who &= who - 1;
+                e = e0 + __ffs(who) - 1;
+            }
+            seen += more;
+        }
+        if (lane == 0) found = e;
+    }
+    __syncthreads();
+    const int e = found, f0 = blockIdx.x * kFewBlockF;
+    /* rows that no expert owns: this block's outputs of its share */
+    for (int r = expert_start(a.offsets, a.experts, m) + (int)blockIdx.y; r < m; r += gridDim.y)
+        if ((int)threadIdx.x < kFewBlockF && f0 + (int)threadIdx.x < a.width)
+            static_cast<T*>(a.out)[(long long)r * a.ldo + f0 + threadIdx.x] = from_f<T>(0.f);
+    if (e < 0) return;
+    const int r1 = expert_start(a.offsets, e + 1, m);
+    const T* w = static_cast<const T*>(a.w) + (long long)e * a.stride_w;
+    const int f = f0 + warp * kFewF;
+    if (f >= a.width) return;
+    for (int r = expert_start(a.offsets, e, m); r < r1; r += 4) {
+        if (r1 - r == 1) few_rows<T, 1>(a, w, f, r, 1, lane);
+        else if (r1 - r == 2) few_rows<T, 2>(a, w, f, r, 2, lane);
+        else few_rows<T, 4>(a, w, f, r, min(4, r1 - r), lane);
+    }
+}
+
+template <typename T>
+cudaError_t launch_few(const ExpertArgs& a, cudaStream_t s) {
+    const dim3 g((unsigned)((a.width + kFewBlockF - 1) / kFewBlockF), (unsigned)(a.m < a.experts ? a.m : a.experts));
+    k_experts_few<T><<<g, kFewThreads, 0, s>>>(a);
+    return cudaGetLastError();
+}
+
 /* ------------------------------------------------------ sorted copy of X ---- */
 
 constexpr int kCopyThreads = 256;
@@ -372,6 +514,9 @@ size_t copy_bytes(int mode, long long m, int experts, int k) {
     return mode == EXP_FWD && experts_few_rows(m, experts) ? 0 : (size_t)m * copy_ld(k) * 2;
 }
 
+/* Up to so many rows the product is a pass over the chosen matrices by plain loads. */
+long long few_limit(int experts) { return experts < 16 ? 16 : experts; }
+
 /* With a sorted copy the product sees plain sorted rows; the tiled kernel gathers
  * for itself and takes none. */
 mpkStatus run_product(ExpertArgs& a, void* work, cudaStream_t s) {
@@ -385,6 +530,8 @@ mpkStatus run_product(ExpertArgs& a, void* work, cudaStream_t s) {
     }
     if (!experts_tc_ok(sorted))
         return (a.bf16 ? launch_any<__nv_bfloat16>(a, s) : launch_any<__half>(a, s)) == cudaSuccess ? MPK_OK : MPK_ERR_CUDA;
+    if (a.mode == EXP_FWD && a.m <= few_limit(a.experts))
+        return (a.bf16 ? launch_few<__nv_bfloat16>(a, s) : launch_few<__half>(a, s)) == cudaSuccess ? MPK_OK : MPK_ERR_CUDA;
     if (a.order && !sorted.order) {
         const long long rows8 = (a.m + kCopyThreads / 32 - 1) / (kCopyThreads / 32), most = (long long)a.sms * 8;
         const int grid = (int)(rows8 < most ? rows8 : most);
