@@ -624,8 +624,8 @@ def route(logits, top_k: int, *, score: str = "softmax", bias=None, groups: int 
     params = _route_params(experts, top_k, score, groups, top_groups, group_score, renormalize, scale)
     used = (logits,) if bias is None else (logits, bias)
     pbias = None if bias is None else _array("bias", bias, torch.float32, experts)
-    ids = torch.empty((n, max(top_k, 0)), dtype=torch.int32, device=logits.device)
-    weights = torch.empty((n, max(top_k, 0)), dtype=torch.float32, device=logits.device)
+    ids = logits.new_empty((n, max(top_k, 0)), dtype=torch.int32)
+    weights = logits.new_empty((n, max(top_k, 0)), dtype=torch.float32)
     _run("mpkRoute", used, ctypes.byref(params), address, code, n, ld, pbias, ids.data_ptr(),
          weights.data_ptr())
     return ids, weights
@@ -680,12 +680,16 @@ def expert_plan(ids, experts: int) -> ExpertPlan:
     n, top_k = ids.shape
     address = _array("ids", ids, _types() and torch.int32, n, top_k)
     need = int(lib().mpkExpertPlanBytes(n, top_k, experts))
-    buf = torch.empty(max(experts, 0) + 1 + 2 * n * top_k, dtype=torch.int32, device=ids.device)
-    offsets, order, pos = buf.split([max(experts, 0) + 1, n * top_k, n * top_k])
+    rows = n * top_k
+    offsets = ids.new_empty(max(experts, 0) + 1)
+    order = ids.new_empty(rows)
+    pos = ids.new_empty((n, top_k))
     work = torch.empty(need, dtype=torch.uint8, device=ids.device) if need else None
     _run("mpkExpertPlan", (ids,), address, n, top_k, experts, offsets.data_ptr(), order.data_ptr(),
          pos.data_ptr(), None if work is None else work.data_ptr(), need)
-    return ExpertPlan(offsets, order, pos.view(n, top_k))
+    plan = object.__new__(ExpertPlan)
+    plan.offsets, plan.order, plan.pos, plan.n, plan.top_k, plan.rows, plan.experts = offsets, order, pos, n, top_k, rows, experts
+    return plan
 
 
 def _sorted_copy(grad_w: int, x, plan: "ExpertPlan", gather: bool) -> tuple:

@@ -418,6 +418,7 @@ k_combine_grad(const T* __restrict__ go, long long ldgo, const T* __restrict__ y
                const int* __restrict__ pos, const int* __restrict__ rows, const float* __restrict__ weights,
                long long n, int top_k, int width, int log_tpr, T* __restrict__ gy, long long ldgy,
                float* __restrict__ gw) {
+    constexpr int U = S <= 4 ? 2 : 1;            /* pieces of the row in flight */
     __shared__ float part[kCombineThreads / 32][S];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const long long m = n * top_k;
@@ -435,31 +436,40 @@ k_combine_grad(const T* __restrict__ go, long long ldgo, const T* __restrict__ y
             dot[s] = 0.f;
         }
         if (t < n)
-            for (int c = own * V; c < width; c += tpr * V) {
-                float g[V];
-                Pack<T, V>::open(Pack<T, V>::raw(go + t * ldgo + c), g);
-                if (gw) {
-                    typename Pack<T, V>::Raw f[S];
+            for (int c0 = own * V; c0 < width; c0 += U * tpr * V) {
+                typename Pack<T, V>::Raw rg[U], f[U][S];
 #pragma unroll
-                    for (int s = 0; s < S; ++s)
-                        f[s] = p[s] >= 0 ? Pack<T, V>::raw(y + (long long)p[s] * ldy + c) : typename Pack<T, V>::Raw{};
+                for (int i = 0; i < U; ++i) {
+                    const int c = c0 + i * tpr * V;
+                    if (c < width) {
+                        rg[i] = Pack<T, V>::raw(go + t * ldgo + c);
+                        if (gw) {
 #pragma unroll
-                    for (int s = 0; s < S; ++s) {
-                        float v[V];
-                        Pack<T, V>::open(f[s], v);
-                        /* a dropped slot stays 0 whatever the gradient holds */
-#pragma unroll
-                        for (int u = 0; u < V; ++u) dot[s] = p[s] >= 0 ? fmaf(g[u], v[u], dot[s]) : 0.f;
+                            for (int s = 0; s < S; ++s)
+                                if (p[s] >= 0) f[i][s] = Pack<T, V>::raw(y + (long long)p[s] * ldy + c);
+                        }
                     }
                 }
 #pragma unroll
-                for (int s = 0; s < S; ++s)
-                    if (p[s] >= 0) {
-                        float v[V];
+                for (int i = 0; i < U; ++i) {
+                    const int c = c0 + i * tpr * V;
+                    if (c >= width) continue;
+                    float g[V];
+                    Pack<T, V>::open(rg[i], g);
 #pragma unroll
-                        for (int u = 0; u < V; ++u) v[u] = wt[s] * g[u];
-                        Pack<T, V>::store(gy + (long long)p[s] * ldgy + c, v);
-                    }
+                    for (int s = 0; s < S; ++s)
+                        if (p[s] >= 0) {
+                            float v[V];
+                            if (gw) {
+                                Pack<T, V>::open(f[i][s], v);
+#pragma unroll
+                                for (int u = 0; u < V; ++u) dot[s] = fmaf(g[u], v[u], dot[s]);
+                            }
+#pragma unroll
+                            for (int u = 0; u < V; ++u) v[u] = wt[s] * g[u];
+                            Pack<T, V>::store(gy + (long long)p[s] * ldgy + c, v);
+                        }
+                }
             }
         if (gw) {
 #pragma unroll

@@ -32,6 +32,7 @@ namespace {
 constexpr unsigned FULL = 0xffffffffu;
 constexpr int kRouteWarps = 4;
 
+
 template <typename T>
 __device__ __forceinline__ float to_f(T v);
 template <>
@@ -179,13 +180,28 @@ __device__ __forceinline__ KEY group_key(const KEY* keys, const RouteShape& sh, 
 }
 
 /* Whether this lane's group, lane >> log, is among the top_groups best of G (ties to
- * the lowest index) and has an expert left. */
-template <typename KEY>
-__device__ __forceinline__ bool group_kept(KEY gk, const RouteShape& sh, int log, int lane) {
+ * the lowest index) and has an expert left: the best is taken top_groups times. */
+__device__ __forceinline__ bool group_kept(unsigned gk, const RouteShape& sh, int log, int lane) {
+    unsigned left = (lane >> log) < sh.G ? gk : 0u;
+    bool in = false;
+    auto best = [&]() {
+        const unsigned m = __reduce_max_sync(FULL, left);
+        const int l = __ffs(__ballot_sync(FULL, left == m)) - 1;
+        if (live(m) && (lane ^ l) >> log == 0) { in = true; left = 0u; }
+    };
+    /* the first ones without a loop: branches that the compiler cannot see to be uniform cost a warp
+     * synchronisation at every warp-wide operation behind them */
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (i < sh.top_groups) best();
+    for (int i = 4; i < sh.top_groups; ++i) best();
+    return in;
+}
+__device__ __forceinline__ bool group_kept(unsigned long long gk, const RouteShape& sh, int log, int lane) {
     const int g = lane >> log;
     int rank = 0;
     for (int h = 0; h < sh.G; ++h) {
-        const KEY o = __shfl_sync(FULL, gk, h << log);
+        const unsigned long long o = __shfl_sync(FULL, gk, h << log);
         rank += (o > gk || (o == gk && h < g)) ? 1 : 0;
     }
     return g < sh.G && live(gk) && rank < sh.top_groups;
@@ -240,33 +256,49 @@ __device__ __noinline__ int slow_choice(const T* __restrict__ row, const float* 
     return mine;
 }
 
+/* 2^x and 1 / x in one instruction each, within 2^-22 and 2^-23 of the value. */
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+constexpr float kLog2e = 1.44269504f;
+
 /* A chosen score up to a factor that the row's slots share, m being the largest
  * chosen logit: e^(x - m) for softmax, and for sigmoids that are all below e^-60,
  * where sigmoid(x) = e^x to the last bit.  As in FP64, a sigmoid below -745 is 0. */
 __device__ __forceinline__ float chosen_score(float x, float m, bool softmax) {
     if (softmax) return expf(x - m);
     if (m < -60.f) return x < -745.f ? 0.f : expf(x - m);
-    return 1.f / (1.f + expf(-x));
+    return __fdividef(1.f, 1.f + expf(-x));
 }
 
 /* The `takes` largest of a warp's keys in descending order, the lowest index first
  * among equals: lane i returns the i-th in (key, index), index -1 where there are
  * fewer.  cand: 32 words of this warp's shared memory. */
 template <int VPL>
-__device__ __forceinline__ void top_keys(unsigned (&key)[VPL], int takes, unsigned long long* cand, int lane,
-                                         unsigned& mykey, int& mine) {
+__device__ __forceinline__ void top_keys(unsigned (&key)[VPL], int takes, uint2* cand, int lane, unsigned& mykey,
+                                         int& mine) {
     mykey = 0u;
     mine = -1;
     /* bound: the takes-th largest value of the lanes' maxima, or any live key */
     unsigned lm = key[0], bound = kLive;
 #pragma unroll
     for (int v = 1; v < VPL; ++v) lm = max(lm, key[v]);
-    for (int i = 0; i < takes; ++i) {
-        const unsigned m = __reduce_max_sync(FULL, lm);
-        bound = max(m, kLive);
-        if (m < kLive) break;
-        if (lm == m) lm = 0u;
-    }
+    auto lower = [&]() {
+        bound = __reduce_max_sync(FULL, lm);
+        if (lm == bound) lm = 0u;
+    };
+#pragma unroll
+    for (int i = 0; i < 9; ++i)
+        if (i < takes) lower();
+    for (int i = 9; i < takes; ++i) lower();
+    bound = max(bound, kLive);
     int own = 0;
 #pragma unroll
     for (int v = 0; v < VPL; ++v) own += key[v] >= bound ? 1 : 0;
@@ -277,32 +309,40 @@ __device__ __forceinline__ void top_keys(unsigned (&key)[VPL], int takes, unsign
         if (lane >= o) at += u;
     }
     const int count = __shfl_sync(FULL, at, 31);
-    if (count <= 32) {
-        at -= own;
-        if (own) {
+    at -= own;
 #pragma unroll
-            for (int v = 0; v < VPL; ++v)
-                if (key[v] >= bound) cand[at++] = (unsigned long long)key[v] << 32 | (unsigned)(VPL * lane + v);
-        }
-        __syncwarp();
+    for (int v = 0; v < VPL; ++v) {
+        const bool in = key[v] >= bound;
+        if (in && at < 32) cand[at] = make_uint2(key[v], (unsigned)(VPL * lane + v));
+        at += in ? 1 : 0;
+    }
+    __syncwarp();
+    {
         /* candidate `lane`, in ascending order of index; its rank among them */
-        const unsigned long long c = lane < count ? cand[lane] : 0ull;
-        const unsigned k = (unsigned)(c >> 32);
+        const uint2 c = lane < count ? cand[lane] : make_uint2(0u, 0u);
         int rank = 0;
-        for (int q = 0; q < count; ++q) {
-            const unsigned o = __shfl_sync(FULL, k, q);
-            rank += (o > k || (o == k && q < lane)) ? 1 : 0;
-        }
+        auto against = [&](int q) {
+            const unsigned o = __shfl_sync(FULL, c.x, q);
+            rank += o > c.x || (o == c.x && q < lane) ? 1 : 0;
+        };
+#pragma unroll
+        for (int q = 0; q < 12; ++q) against(q);
+        if (count > 12)
+            for (int q = 12; q < 32; ++q) against(q);
         __syncwarp();
         if (lane < count && rank < takes) cand[rank] = c;
         __syncwarp();
         if (lane < min(count, takes)) {
-            mykey = (unsigned)(cand[lane] >> 32);
-            mine = (int)(unsigned)cand[lane];
+            const uint2 m = cand[lane];
+            mykey = m.x;
+            mine = (int)m.y;
         }
         __syncwarp();
-    } else {
+    }
+    if (count > 32) {
         /* many equal maxima: the maximum, takes times */
+        mykey = 0u;
+        mine = -1;
         for (int i = 0; i < takes; ++i) {
             unsigned bk = 0u;
             int bj = INT_MAX;
@@ -320,28 +360,30 @@ __device__ __forceinline__ void top_keys(unsigned (&key)[VPL], int takes, unsign
     }
 }
 
-template <typename T, int VPL>
-__global__ void __launch_bounds__(32 * kRouteWarps)
+/* Blocks an SM that the fast path's registers are cut to; slow_choice spills. */
+constexpr int route_blocks(int vpl) { return vpl <= 4 ? 12 : vpl == 8 ? 10 : 1; }
+
+/* BY_SCORE: keys are choice values c (a bias, or groups by their two best), else
+ * logits.  GROUPED: some groups are cut. */
+template <typename T, int VPL, bool BY_SCORE, bool GROUPED>
+__global__ void __launch_bounds__(32 * kRouteWarps, route_blocks(VPL))
 k_route(const T* __restrict__ logits, long long n, long long ld, const float* __restrict__ bias, RouteShape sh,
         int* __restrict__ ids, float* __restrict__ weights) {
     extern __shared__ unsigned long long route_sm[];
-    __shared__ unsigned long long route_cand[kRouteWarps][32];
+    __shared__ uint2 route_cand[kRouteWarps][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     unsigned long long* keys64 = route_sm + (size_t)warp * sh.E;
     unsigned* keys32 = reinterpret_cast<unsigned*>(keys64);
     const bool softmax = sh.score == MPK_SCORE_SOFTMAX;
-    const bool grouped = sh.G > 1 && sh.top_groups < sh.G;
-    const bool top2 = grouped && sh.group_score == MPK_GROUP_TOP2;
-    const bool by_score = bias || top2;                       /* keys are choice values c, else logits */
-    const bool scores = by_score || (softmax && !sh.renorm);  /* some use of all experts' scores */
-    const bool by_logit_after = top2 && !bias;                /* once groups are chosen, the logits' order again */
+    const bool scores = BY_SCORE || (softmax && !sh.renorm);   /* some use of all experts' scores */
+    const bool by_logit_after = BY_SCORE && !bias;             /* once groups are chosen, the logits' order again */
     /* the bias of this lane's experts, kept over the rows where registers allow */
-    constexpr bool KEEP = VPL <= 8;
+    constexpr bool KEEP = BY_SCORE && VPL <= 8;
     float bv[KEEP ? VPL : 1];
-    auto bias_of = [&](int v) { return VPL * lane + v < sh.E ? bias[VPL * lane + v] : 0.f; };
+    auto bias_of = [&](int v) { return bias && VPL * lane + v < sh.E ? bias[VPL * lane + v] : 0.f; };
     if constexpr (KEEP) {
 #pragma unroll
-        for (int v = 0; v < VPL; ++v) bv[v] = bias ? bias_of(v) : 0.f;
+        for (int v = 0; v < VPL; ++v) bv[v] = bias_of(v);
     }
     const long long step = (long long)gridDim.x * kRouteWarps;
     for (long long t = (long long)blockIdx.x * kRouteWarps + warp; t < n; t += step) {
@@ -360,35 +402,40 @@ k_route(const T* __restrict__ logits, long long n, long long ld, const float* __
                 if (mx == -INFINITY) mx = 0.f;
                 sum = 0.f;
 #pragma unroll
-                for (int v = 0; v < VPL; ++v) { c[v] = expf(x[v] - mx); sum += c[v]; }
+                for (int v = 0; v < VPL; ++v) { c[v] = exp2_fast((x[v] - mx) * kLog2e); sum += c[v]; }
                 sum = warp_sum(sum);
-                smax = 1.f / sum;
+                smax = rcp_fast(sum);
 #pragma unroll
                 for (int v = 0; v < VPL; ++v) c[v] *= smax;
             } else {
 #pragma unroll
-                for (int v = 0; v < VPL; ++v) c[v] = __fdividef(1.f, 1.f + expf(-x[v]));
+                for (int v = 0; v < VPL; ++v) c[v] = rcp_fast(1.f + exp2_fast(x[v] * -kLog2e));
             }
+            if constexpr (BY_SCORE) {
 #pragma unroll
-            for (int v = 0; v < VPL; ++v) {
-                if (bias) c[v] += KEEP ? bv[KEEP ? v : 0] : bias_of(v);
-                key[v] = x[v] == -INFINITY ? 0u : key_of(by_score ? c[v] : x[v]);
+                for (int v = 0; v < VPL; ++v) {
+                    c[v] += KEEP ? bv[KEEP ? v : 0] : bias_of(v);
+                    key[v] = x[v] == -INFINITY ? 0u : key_of(c[v]);
+                }
             }
-        } else {
+        }
+        if constexpr (!BY_SCORE) {
 #pragma unroll
             for (int v = 0; v < VPL; ++v) key[v] = key_of(x[v]);
         }
-        /* Error bounds of c.  expf (2 ulp) and the sigmoid's division (2 ulp) leave 1.5 2^-22
-         * of 1; softmax adds |x - mx| 2^-24 s from the rounded argument, which is
-         * under 2^-17 s wherever s does not underflow and under 2^-19 of the
-         * row's largest score everywhere; adding the bias rounds by 2^-24 |c|. */
+        /* Error bounds of c.  e^d from exp2_fast is off by (2^-22 + 1.5 |d| 2^-24) of itself: the instruction,
+         * and the rounding of d log2 e.  A sigmoid turns that into s (1 - s) of it, under 2^-23, and adds 2^-23 s
+         * for the reciprocal and 2^-24 for the sum; a softmax value adds its argument's rounding, |d| 2^-24, and the
+         * sum's and reciprocal's error, which all scores share: under 2^-20 of the row's largest score in all, and
+         * (1 + 0.7 |d|) 2^-22 of the score itself, under 2^-16 of it wherever it does not underflow.  Adding the
+         * bias rounds by 2^-24 |c|. */
         auto near = [&](float a, float b) {
             const float tol = bias ? (softmax ? 0x1.0p-18f : 0x1.0p-20f) * smax + 0x1.0p-22f * (fabsf(a) + fabsf(b))
-                                   : 0x1.0p-16f * (fabsf(a) + fabsf(b)) + 1e-44f;
+                                   : 0x1.0p-15f * (fabsf(a) + fabsf(b)) + 1e-37f;
             return !(a - b > tol);
         };
         bool slow = false;
-        if (grouped) {
+        if constexpr (GROUPED) {
             unsigned gk;
             bool in;
             const int log = sh.log_g >= 0 ? sh.log_g : sh.log_l;
@@ -401,7 +448,8 @@ k_route(const T* __restrict__ logits, long long n, long long ld, const float* __
                 }
                 for (int o = (1 << log) >> 1; o > 0; o >>= 1) {
                     const unsigned a2 = __shfl_xor_sync(FULL, a, o), b2 = __shfl_xor_sync(FULL, b, o);
-                    merge2(a, b, a2, b2);
+                    b = max(min(a, a2), max(b, b2));
+                    a = max(a, a2);
                 }
                 gk = group_of_two(a, b, sh.group_score);
                 in = group_kept(gk, sh, log, lane);
@@ -424,7 +472,7 @@ k_route(const T* __restrict__ logits, long long n, long long ld, const float* __
                 }
                 __syncwarp();
             }
-            if (by_score) {                                        /* the groups on both sides of the cut */
+            if constexpr (BY_SCORE) {                              /* the groups on both sides of the cut */
                 const bool there = (lane >> log) < sh.G;
                 const unsigned lo = __reduce_min_sync(FULL, in ? gk : 0xffffffffu);
                 const unsigned hi = __reduce_max_sync(FULL, there && !in ? gk : 0u);
@@ -433,28 +481,32 @@ k_route(const T* __restrict__ logits, long long n, long long ld, const float* __
         }
         int mine;
         unsigned mykey;
-        top_keys(key, sh.k + (bias && sh.k < 32 ? 1 : 0), route_cand[warp], lane, mykey, mine);
-        if (bias) {
-            const unsigned nk = __shfl_down_sync(FULL, mykey, 1);
-            const int nj = __shfl_down_sync(FULL, mine, 1);
-            if (lane < sh.k && lane < 31 && mine >= 0 && nj >= 0 && near(of_key(mykey), of_key(nk)))
-                slow = slow || !(to_f(row[mine]) == to_f(row[nj]) && bias[mine] == bias[nj]);
-            if (sh.k == 32) slow = true;                            /* no lane holds the first loser */
+        top_keys(key, sh.k + (BY_SCORE && bias && sh.k < 32 ? 1 : 0), route_cand[warp], lane, mykey, mine);
+        float xi;
+        if constexpr (BY_SCORE) {
+            if (bias) {
+                const unsigned nk = __shfl_down_sync(FULL, mykey, 1);
+                const int nj = __shfl_down_sync(FULL, mine, 1);
+                if (lane < sh.k && lane < 31 && mine >= 0 && nj >= 0 && near(of_key(mykey), of_key(nk)))
+                    slow = slow || !(to_f(row[mine]) == to_f(row[nj]) && bias[mine] == bias[nj]);
+                if (sh.k == 32) slow = true;                       /* no lane holds the first loser */
+            }
+            if (__any_sync(FULL, slow)) mine = slow_choice(row, bias, sh, keys64, lane);
+            if (lane >= sh.k) mine = -1;
+            xi = mine >= 0 ? to_f(row[mine]) : -INFINITY;
+        } else {
+            xi = mine >= 0 ? of_key(mykey) : -INFINITY;
         }
-        const bool again = __any_sync(FULL, slow);
-        if (again) mine = slow_choice(row, bias, sh, keys64, lane);
-        if (lane >= sh.k) mine = -1;
         const bool valid = mine >= 0;
-        const float xi = !valid ? -INFINITY : (bias || again) ? to_f(row[mine]) : of_key(mykey);
         float w;
         if (sh.renorm) {
             const float m = slot_max(xi, sh.log_k);
             const float e = valid ? chosen_score(xi, m, softmax) : 0.f;
             const float total = slot_sum(e, sh.log_k);
-            w = total == 0.f ? 0.f : e / total;
+            w = total == 0.f ? 0.f : __fdividef(e, total);
             if (valid && sum != sum) w = NAN;
         } else {
-            w = !valid ? 0.f : softmax ? expf(xi - mx) / sum : 1.f / (1.f + expf(-xi));
+            w = !valid ? 0.f : softmax ? __fdividef(expf(xi - mx), sum) : __fdividef(1.f, 1.f + expf(-xi));
         }
         if (lane < sh.k) {
             ids[t * sh.k + lane] = mine;
@@ -463,21 +515,79 @@ k_route(const T* __restrict__ logits, long long n, long long ld, const float* __
     }
 }
 
-/* Gradient of the weights, one warp a token.  With w the weights at scale 1, g
- * the incoming gradient times the scale and G = sum of g w over the slots:
+/* Gradient of the weights.  With w the weights at scale 1, g the incoming gradient
+ * times the scale and G = sum of g w over the slots:
  *   renormalized:  softmax  dl_i = w_i (g_i - G)
  *                  sigmoid  dl_i = w_i (1 - s_i) (g_i - G)      0 off the slots
  *   otherwise:     sigmoid  dl_i = g_i s_i (1 - s_i)            0 off the slots
  *                  softmax  dl_j = s_j ([j chosen] g_j - sum over slots of g s)
- * so only the last form reads the whole row.  Slot i's term is formed by lane i;
- * every lane then collects the terms of its own experts, so a row is written once. */
-template <typename T, int VPL>
+ * The first three need the chosen logits only: k_route_grad_slots gives a token
+ * 2^log_k lanes, one a slot, and a warp 32 / 2^log_k tokens, whose rows it fills with
+ * zeros before the slots' terms go in (ordered by __syncwarp; slots of one expert
+ * all write their sum).  (A warp a token took 263 instructions a row and 14 us for
+ * 30001 x 60.)  The last form reads and writes whole rows: k_route_grad_whole, one
+ * warp a token. */
+template <typename T, typename W>
 __global__ void __launch_bounds__(32 * kRouteWarps)
-k_route_grad(const T* __restrict__ logits, long long n, long long ld, RouteShape sh, const int* __restrict__ ids,
-             const float* __restrict__ gw, T* __restrict__ out, long long ldg) {
+k_route_grad_slots(const T* __restrict__ logits, long long n, long long ld, RouteShape sh, const int* __restrict__ ids,
+                   const float* __restrict__ gw, T* __restrict__ out, long long ldg) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const bool softmax = sh.score == MPK_SCORE_SOFTMAX;
-    const bool whole = softmax && !sh.renorm;
+    const int slots = 1 << sh.log_k, tokens = 32 >> sh.log_k;
+    const int slot = lane & (slots - 1);
+    const int words = sh.E * (int)sizeof(T) / (int)sizeof(W);       /* of a row */
+    const long long step = (long long)gridDim.x * kRouteWarps * tokens;
+    for (long long t0 = ((long long)blockIdx.x * kRouteWarps + warp) * tokens; t0 < n; t0 += step) {
+        const long long t = t0 + (lane >> sh.log_k);
+        const bool here = t < n && slot < sh.k;
+        int id = here ? ids[t * sh.k + slot] : -1;
+        if ((unsigned)id >= (unsigned)sh.E) id = -1;
+        const bool valid = id >= 0;
+        const float g = valid ? gw[t * sh.k + slot] * sh.scale : 0.f;
+        const float xi = valid ? to_f(logits[t * ld + id]) : -INFINITY;
+        {
+            const int rows = (int)min((long long)tokens, n - t0);
+            T* first = out + t0 * ldg;
+            const W zero = {};
+            if (ldg == sh.E) {
+                for (int i = lane; i < rows * words; i += 32) reinterpret_cast<W*>(first)[i] = zero;
+            } else {
+                for (int r = 0; r < rows; ++r)
+                    for (int i = lane; i < words; i += 32) reinterpret_cast<W*>(first + r * ldg)[i] = zero;
+            }
+        }
+        float si = 0.f, left = 1.f, term;                           /* s, 1 - s */
+        if (!softmax) {
+            si = valid ? __fdividef(1.f, 1.f + expf(-xi)) : 0.f;
+            left = valid ? __fdividef(1.f, 1.f + expf(xi)) : 0.f;
+        }
+        if (sh.renorm) {
+            const float m = slot_max(xi, sh.log_k);
+            const float e = (!valid || m == -INFINITY) ? 0.f : chosen_score(xi, m, softmax);
+            const float total = slot_sum(e, sh.log_k);
+            const float w = total == 0.f ? 0.f : __fdividef(e, total);
+            const float G = slot_sum(valid ? g * w : 0.f, sh.log_k);
+            term = w * left * (g - G);
+        } else {
+            term = g * si * left;
+        }
+        float sum = 0.f;                                            /* over the slots of the same expert */
+        for (int i = 0; i < sh.k; ++i) {
+            const int from = (lane & ~(slots - 1)) + i;
+            const int j = __shfl_sync(FULL, id, from);
+            const float d = __shfl_sync(FULL, term, from);
+            sum += j == id ? d : 0.f;
+        }
+        __syncwarp();
+        if (valid) out[t * ldg + id] = from_f<T>(sum);
+    }
+}
+
+template <typename T, int VPL>
+__global__ void __launch_bounds__(32 * kRouteWarps)
+k_route_grad_whole(const T* __restrict__ logits, long long n, long long ld, RouteShape sh, const int* __restrict__ ids,
+                   const float* __restrict__ gw, T* __restrict__ out, long long ldg) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const long long step = (long long)gridDim.x * kRouteWarps;
     for (long long t = (long long)blockIdx.x * kRouteWarps + warp; t < n; t += step) {
         const T* row = logits + t * ld;
@@ -487,50 +597,29 @@ k_route_grad(const T* __restrict__ logits, long long n, long long ld, RouteShape
         const float g = valid ? gw[t * sh.k + lane] * sh.scale : 0.f;
         const float xi = valid ? to_f(row[id]) : -INFINITY;
         float s[VPL], acc[VPL];
-        float term, dot = 0.f;
+        float sum = 0.f;
+        LaneRow<T, VPL>::load(row, sh.E, sh.vec, lane, s);
+        float mx = s[0];
 #pragma unroll
-        for (int v = 0; v < VPL; ++v) acc[v] = 0.f;
-        if (whole) {
-            float sum = 0.f;
-            LaneRow<T, VPL>::load(row, sh.E, sh.vec, lane, s);
-            float mx = s[0];
+        for (int v = 1; v < VPL; ++v) mx = fmaxf(mx, s[v]);
+        mx = warp_max(mx);
+        if (mx == -INFINITY) mx = 0.f;
 #pragma unroll
-            for (int v = 1; v < VPL; ++v) mx = fmaxf(mx, s[v]);
-            mx = warp_max(mx);
-            if (mx == -INFINITY) mx = 0.f;
+        for (int v = 0; v < VPL; ++v) { s[v] = expf(s[v] - mx); sum += s[v]; }
+        sum = warp_sum(sum);
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;            /* every expert masked: no gradient */
 #pragma unroll
-            for (int v = 0; v < VPL; ++v) { s[v] = expf(s[v] - mx); sum += s[v]; }
-            sum = warp_sum(sum);
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;        /* every expert masked: no gradient */
-#pragma unroll
-            for (int v = 0; v < VPL; ++v) s[v] *= inv;
-            dot = slot_sum(valid ? g * (expf(xi - mx) * inv) : 0.f, sh.log_k);
-            dot = __shfl_sync(FULL, dot, 0);
-            term = g;
-        } else {
-            const float si = valid ? 1.f / (1.f + expf(-xi)) : 0.f;
-            const float left = softmax ? 1.f : 1.f / (1.f + expf(xi));      /* 1 - s */
-            if (sh.renorm) {
-                const float m = slot_max(xi, sh.log_k);
-                const float e = (!valid || m == -INFINITY) ? 0.f : chosen_score(xi, m, softmax);
-                const float total = slot_sum(e, sh.log_k);
-                const float w = total == 0.f ? 0.f : e / total;
-                const float G = slot_sum(valid ? g * w : 0.f, sh.log_k);
-                term = w * left * (g - G);
-            } else {
-                term = g * si * left;
-            }
-        }
+        for (int v = 0; v < VPL; ++v) { s[v] *= inv; acc[v] = 0.f; }
+        float dot = slot_sum(valid ? g * (expf(xi - mx) * inv) : 0.f, sh.log_k);
+        dot = __shfl_sync(FULL, dot, 0);
         for (int i = 0; i < sh.k; ++i) {
             const int j = __shfl_sync(FULL, id, i) - VPL * lane;
-            const float d = __shfl_sync(FULL, term, i);
+            const float d = __shfl_sync(FULL, g, i);
 #pragma unroll
             for (int v = 0; v < VPL; ++v) acc[v] += j == v ? d : 0.f;
         }
-        if (whole) {
 #pragma unroll
-            for (int v = 0; v < VPL; ++v) acc[v] = s[v] * (acc[v] - dot);
-        }
+        for (int v = 0; v < VPL; ++v) acc[v] = s[v] * (acc[v] - dot);
         LaneRow<T, VPL>::store(out + t * ldg, sh.E, sh.vec, lane, acc);
     }
 }
@@ -765,18 +854,32 @@ cudaError_t run_route(RouteShape sh, const void* logits, long long n, long long 
         sh.log_g = 0;
         while ((1 << sh.log_g) < lanes) ++sh.log_g;
     }
-    const size_t smem = (bias || sh.G > 1) ? (size_t)kRouteWarps * sh.E * 8 : 0;
-    k_route<T, VPL><<<route_grid(n, sms), 32 * kRouteWarps, smem, s>>>(static_cast<const T*>(logits), n, ld, bias, sh,
-                                                                      ids, w);
+    const bool grouped = sh.G > 1 && sh.top_groups < sh.G;
+    const bool by_score = bias || (grouped && sh.group_score == MPK_GROUP_TOP2);
+    const size_t smem = (by_score || grouped) ? (size_t)kRouteWarps * sh.E * 8 : 0;
+    const auto kern = by_score ? (grouped ? k_route<T, VPL, true, true> : k_route<T, VPL, true, false>)
+                               : (grouped ? k_route<T, VPL, false, true> : k_route<T, VPL, false, false>);
+    kern<<<route_grid(n, sms), 32 * kRouteWarps, smem, s>>>(static_cast<const T*>(logits), n, ld, bias, sh, ids, w);
     return cudaGetLastError();
 }
 
 template <typename T, int VPL>
 cudaError_t run_route_grad(RouteShape sh, const void* logits, long long n, long long ld, const int* ids,
                            const float* gw, void* out, long long ldg, int sms, cudaStream_t s) {
-    sh.vec = lane_words<T, VPL>(logits, n, ld) && lane_words<T, VPL>(out, n, ldg);
-    k_route_grad<T, VPL><<<route_grid(n, sms), 32 * kRouteWarps, 0, s>>>(static_cast<const T*>(logits), n, ld, sh, ids,
-                                                                        gw, static_cast<T*>(out), ldg);
+    const T* x = static_cast<const T*>(logits);
+    T* o = static_cast<T*>(out);
+    if (sh.score == MPK_SCORE_SOFTMAX && !sh.renorm) {
+        sh.vec = lane_words<T, VPL>(logits, n, ld) && lane_words<T, VPL>(out, n, ldg);
+        k_route_grad_whole<T, VPL><<<route_grid(n, sms), 32 * kRouteWarps, 0, s>>>(x, n, ld, sh, ids, gw, o, ldg);
+        return cudaGetLastError();
+    }
+    const int tokens = 32 >> sh.log_k, grid = route_grid((n + tokens - 1) / tokens, sms);
+    /* the widest word that rows are made of */
+    const uintptr_t grain = reinterpret_cast<uintptr_t>(out) | (uintptr_t)(sh.E * sizeof(T)) |
+                            (n > 1 ? (uintptr_t)ldg * sizeof(T) : 0);
+    if (grain % 16 == 0) k_route_grad_slots<T, uint4><<<grid, 32 * kRouteWarps, 0, s>>>(x, n, ld, sh, ids, gw, o, ldg);
+    else if (grain % 4 == 0) k_route_grad_slots<T, unsigned><<<grid, 32 * kRouteWarps, 0, s>>>(x, n, ld, sh, ids, gw, o, ldg);
+    else k_route_grad_slots<T, unsigned short><<<grid, 32 * kRouteWarps, 0, s>>>(x, n, ld, sh, ids, gw, o, ldg);
     return cudaGetLastError();
 }
 
