@@ -207,11 +207,20 @@ __device__ __forceinline__ bool group_kept(unsigned long long gk, const RouteSha
     return g < sh.G && live(gk) && rank < sh.top_groups;
 }
 
-/* The whole choice of one row in FP64: slot `lane`'s expert, or -1.  keys: E
- * 64-bit words of this warp's shared memory. */
+/* The choice of one row in FP64: slot `lane`'s expert, or -1.  keys: E 64-bit words
+ * of this warp's shared memory.  Slot `lane` has `mine` so far, slot k being the
+ * first loser, and `close` says that the next slot's value is close; where that is
+ * no exact tie (the same logit and bias) the order is decided again, and so is the
+ * whole choice where the first loser is involved or `whole` is set.  (With 32 slots
+ * no lane holds the first loser and every row is decided here.) */
 template <typename T>
 __device__ __noinline__ int slow_choice(const T* __restrict__ row, const float* __restrict__ bias, RouteShape sh,
-                                        unsigned long long* keys, int lane) {
+                                        unsigned long long* keys, int lane, int mine, bool close, bool whole) {
+    const int nj = __shfl_down_sync(FULL, mine, 1);
+    if (close && mine >= 0 && nj >= 0) close = !(to_f(row[mine]) == to_f(row[nj]) && bias[mine] == bias[nj]);
+    const bool order_only = !__any_sync(FULL, whole || (close && lane == sh.k - 1));
+    if (!__any_sync(FULL, whole || close)) return mine;
+    if (lane >= sh.k) mine = -1;
     double mx = 0.0, sum = 1.0;
     if (sh.score == MPK_SCORE_SOFTMAX) {
         float m = -INFINITY;
@@ -222,12 +231,27 @@ __device__ __noinline__ int slow_choice(const T* __restrict__ row, const float* 
         for (int j = lane; j < sh.E; j += 32) sum += exp((double)to_f(row[j]) - mx);
         sum = warp_sum(sum);
     }
-    for (int j = lane; j < sh.E; j += 32) {
+    auto key = [&](int j) {
         const double x = (double)to_f(row[j]);
         const double s = sh.score == MPK_SCORE_SOFTMAX ? exp(x - mx) / sum : 1.0 / (1.0 + exp(-x));
         const double c = bias ? s + (double)bias[j] : s;
-        keys[j] = x == -(double)INFINITY ? 0ull : key_of(c);
+        return x == -(double)INFINITY ? 0ull : key_of(c);
+    };
+    if (order_only) {
+        const unsigned long long k = mine >= 0 ? key(mine) : 0ull;
+        int rank = 0;
+        for (int i = 0; i < sh.k; ++i) {
+            const unsigned long long k2 = __shfl_sync(FULL, k, i);
+            const int j2 = __shfl_sync(FULL, mine, i);
+            rank += k2 > k || (k2 == k && j2 < mine) ? 1 : 0;
+        }
+        if (lane < sh.k && mine >= 0) keys[rank] = (unsigned long long)mine;
+        __syncwarp();
+        if (mine >= 0 && lane < sh.k) mine = (int)keys[lane];
+        __syncwarp();
+        return mine;
     }
+    for (int j = lane; j < sh.E; j += 32) keys[j] = key(j);
     __syncwarp();
     if (sh.G > 1) {
         const unsigned kept = __ballot_sync(FULL, group_kept(group_key(keys, sh, lane), sh, sh.log_l, lane));
@@ -236,7 +260,7 @@ __device__ __noinline__ int slow_choice(const T* __restrict__ row, const float* 
             if (!((kept >> (((unsigned)j * sh.gmul >> 20) << sh.log_l)) & 1u)) keys[j] = 0ull;
         __syncwarp();
     }
-    int mine = -1;
+    mine = -1;
     for (int i = 0; i < sh.k; ++i) {
         unsigned long long b = 0ull;
         int bj = INT_MAX;
@@ -364,8 +388,9 @@ __device__ __forceinline__ void top_keys(unsigned (&key)[VPL], int takes, uint2*
 constexpr int route_blocks(int vpl) { return vpl <= 4 ? 12 : vpl == 8 ? 10 : 1; }
 
 /* BY_SCORE: keys are choice values c (a bias, or groups by their two best), else
- * logits.  GROUPED: some groups are cut. */
-template <typename T, int VPL, bool BY_SCORE, bool GROUPED>
+ * logits.  GROUPS: 0 none are cut; 1 whole lanes hold a group (log_g >= 0); 2 any
+ * others, through shared memory. */
+template <typename T, int VPL, bool BY_SCORE, int GROUPS>
 __global__ void __launch_bounds__(32 * kRouteWarps, route_blocks(VPL))
 k_route(const T* __restrict__ logits, long long n, long long ld, const float* __restrict__ bias, RouteShape sh,
         int* __restrict__ ids, float* __restrict__ weights) {
@@ -425,21 +450,21 @@ k_route(const T* __restrict__ logits, long long n, long long ld, const float* __
         }
         /* Error bounds of c.  e^d from exp2_fast is off by (2^-22 + 1.5 |d| 2^-24) of itself: the instruction,
          * and the rounding of d log2 e.  A sigmoid turns that into s (1 - s) of it, under 2^-23, and adds 2^-23 s
-         * for the reciprocal and 2^-24 for the sum; a softmax value adds its argument's rounding, |d| 2^-24, and the
+         * for the reciprocal and 2^-24 for the sum, 2.1 2^-23 in all; a softmax value adds its argument's rounding, |d| 2^-24, and the
          * sum's and reciprocal's error, which all scores share: under 2^-20 of the row's largest score in all, and
          * (1 + 0.7 |d|) 2^-22 of the score itself, under 2^-16 of it wherever it does not underflow.  Adding the
          * bias rounds by 2^-24 |c|. */
         auto near = [&](float a, float b) {
-            const float tol = bias ? (softmax ? 0x1.0p-18f : 0x1.0p-20f) * smax + 0x1.0p-22f * (fabsf(a) + fabsf(b))
+            const float tol = bias ? (softmax ? 0x1.0p-18f : 0x1.4p-21f) * smax + 0x1.1p-24f * (fabsf(a) + fabsf(b))
                                    : 0x1.0p-15f * (fabsf(a) + fabsf(b)) + 1e-37f;
             return !(a - b > tol);
         };
-        bool slow = false;
-        if constexpr (GROUPED) {
+        bool slow = false;                                         /* the groups are not certain */
+        if constexpr (GROUPS != 0) {
             unsigned gk;
             bool in;
-            const int log = sh.log_g >= 0 ? sh.log_g : sh.log_l;
-            if (sh.log_g >= 0) {
+            const int log = GROUPS == 1 ? sh.log_g : sh.log_l;
+            if constexpr (GROUPS == 1) {
                 unsigned a = 0u, b = 0u;
 #pragma unroll
                 for (int v = 0; v < VPL; ++v) {
@@ -476,7 +501,7 @@ k_route(const T* __restrict__ logits, long long n, long long ld, const float* __
                 const bool there = (lane >> log) < sh.G;
                 const unsigned lo = __reduce_min_sync(FULL, in ? gk : 0xffffffffu);
                 const unsigned hi = __reduce_max_sync(FULL, there && !in ? gk : 0u);
-                if (live(hi)) slow = near(of_key(lo), of_key(hi));
+                slow = live(hi) && near(of_key(lo), of_key(hi));
             }
         }
         int mine;
@@ -484,14 +509,13 @@ k_route(const T* __restrict__ logits, long long n, long long ld, const float* __
         top_keys(key, sh.k + (BY_SCORE && bias && sh.k < 32 ? 1 : 0), route_cand[warp], lane, mykey, mine);
         float xi;
         if constexpr (BY_SCORE) {
+            bool close = false;                                    /* this slot and the next */
             if (bias) {
                 const unsigned nk = __shfl_down_sync(FULL, mykey, 1);
-                const int nj = __shfl_down_sync(FULL, mine, 1);
-                if (lane < sh.k && lane < 31 && mine >= 0 && nj >= 0 && near(of_key(mykey), of_key(nk)))
-                    slow = slow || !(to_f(row[mine]) == to_f(row[nj]) && bias[mine] == bias[nj]);
-                if (sh.k == 32) slow = true;                       /* no lane holds the first loser */
+                close = lane < sh.k && lane < 31 && live(nk) && near(of_key(mykey), of_key(nk));
             }
-            if (__any_sync(FULL, slow)) mine = slow_choice(row, bias, sh, keys64, lane);
+            if (__any_sync(FULL, slow || close || sh.k == 32))
+                mine = slow_choice(row, bias, sh, keys64, lane, mine, close, slow || sh.k == 32);
             if (lane >= sh.k) mine = -1;
             xi = mine >= 0 ? to_f(row[mine]) : -INFINITY;
         } else {
@@ -857,8 +881,9 @@ cudaError_t run_route(RouteShape sh, const void* logits, long long n, long long 
     const bool grouped = sh.G > 1 && sh.top_groups < sh.G;
     const bool by_score = bias || (grouped && sh.group_score == MPK_GROUP_TOP2);
     const size_t smem = (by_score || grouped) ? (size_t)kRouteWarps * sh.E * 8 : 0;
-    const auto kern = by_score ? (grouped ? k_route<T, VPL, true, true> : k_route<T, VPL, true, false>)
-                               : (grouped ? k_route<T, VPL, false, true> : k_route<T, VPL, false, false>);
+    const auto kern = !grouped ? (by_score ? k_route<T, VPL, true, 0> : k_route<T, VPL, false, 0>)
+                    : sh.log_g >= 0 ? (by_score ? k_route<T, VPL, true, 1> : k_route<T, VPL, false, 1>)
+                                    : (by_score ? k_route<T, VPL, true, 2> : k_route<T, VPL, false, 2>);
     kern<<<route_grid(n, sms), 32 * kRouteWarps, smem, s>>>(static_cast<const T*>(logits), n, ld, bias, sh, ids, w);
     return cudaGetLastError();
 }
