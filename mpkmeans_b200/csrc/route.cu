@@ -384,14 +384,16 @@ __device__ __forceinline__ void top_keys(unsigned (&key)[VPL], int takes, uint2*
     }
 }
 
-/* Blocks an SM that the fast path's registers are cut to; slow_choice spills. */
-constexpr int route_blocks(int vpl) { return vpl <= 4 ? 12 : vpl == 8 ? 10 : 1; }
+/* Blocks an SM that the registers are cut to, so that slow_choice, which is called
+ * from the main path but rarely runs, does not set their number.  (256 experts with
+ * a bias: 6, 8, 10 and 12 blocks took 40, 44, 41 and 46 us; without: no difference.) */
+constexpr int route_blocks(int vpl, bool by_score) { return vpl <= 4 ? 12 : vpl > 8 ? 1 : by_score ? 6 : 10; }
 
 /* BY_SCORE: keys are choice values c (a bias, or groups by their two best), else
  * logits.  GROUPS: 0 none are cut; 1 whole lanes hold a group (log_g >= 0); 2 any
  * others, through shared memory. */
 template <typename T, int VPL, bool BY_SCORE, int GROUPS>
-__global__ void __launch_bounds__(32 * kRouteWarps, route_blocks(VPL))
+__global__ void __launch_bounds__(32 * kRouteWarps, route_blocks(VPL, BY_SCORE))
 k_route(const T* __restrict__ logits, long long n, long long ld, const float* __restrict__ bias, RouteShape sh,
         int* __restrict__ ids, float* __restrict__ weights) {
     extern __shared__ unsigned long long route_sm[];
