@@ -12,7 +12,8 @@
  * t * top_k + s is slot s of token t.  All pointers named dX are device pointers
  * of the current device, owned by the caller; work runs on `stream`, is only
  * enqueued (no synchronisation, no allocation, no state kept between calls) and
- * can be captured into a CUDA graph.  Leading dimensions (ld...) count elements.
+ * can be captured into a CUDA graph (after one call outside a capture, which
+ * loads the kernels).  Outputs and scratch overlap nothing else.  Leading dimensions (ld...) count elements.
  * A call with n = 0 (or m = 0) writes only what its comment says.  Bad arguments
  * return MPK_ERR_INVALID before anything is enqueued. */
 #ifndef MPKEXPERTS_B200_H

@@ -776,8 +776,13 @@ cudaError_t launch_t(const ExpertArgs& a, cudaStream_t s) {
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 
-/* Tile widths by the average expert's rows; see experts_few_rows for FWD's few.  A
- * pair's 64-wide tile has ten stages of W in flight, the 256-wide one six. */
+/* Tile widths by the average expert's rows.  A pair's 64-wide tile has ten stages of
+ * W in flight, the 256-wide one six.  Measured, 64 experts of 1024 x 2048, GRADX:
+ * 1 row an expert 39 us on 32-wide tiles and 38 on 256-wide pairs, 6 rows 63, 57 and
+ * 52 on 64-wide pairs, 20 rows 76, 58 and 58, 64 rows 70 on 64-wide and 61 on
+ * 256-wide pairs.  FWD gathers rows itself on 32-wide tiles, which the copy of a
+ * sorted X must be weighed against: 12 rows 60 us there, 67 on pairs with the copy,
+ * 16 rows 72 and 64. */
 template <int FMT>
 cudaError_t launch_fmt(const ExpertArgs& a, cudaStream_t s) {
     const long long rows = a.m / a.experts;

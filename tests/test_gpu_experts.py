@@ -128,7 +128,8 @@ def test_route_masks(score, dtype):
 def test_route_nan_rows_stay_inside(score):
     x = normal(1, 6, 48)
     x[1, 7] = float("nan")
-    x[2] = float("nan")
+    x[2].view(torch.int32).fill_(0xffc00000 - 2 ** 32)             # NaN with the sign bit set
+    assert torch.signbit(x[2]).all()
     for kw in (dict(), dict(renormalize=False), dict(bias=normal(2, 48, scale=0.1)),
                dict(groups=6, top_groups=2, group_score="top2")):
         ids, w = M.route(x, 4, score=score, **kw)
@@ -158,6 +159,7 @@ def test_route_tiny_scores_keep_their_ratios():
 
 @pytest.mark.parametrize("dtype", list(TYPES))
 def test_route_strided_rows(dtype):
+    assert M.route(normal(3, 0, 8, dtype=TYPES[dtype]), 2)[0].shape == (0, 2)
     big = normal(3, 20, 80, dtype=TYPES[dtype])
     check_route(big[:, 3:63], 5)
     check_route(big[::2, :60], 5, score="sigmoid", bias=normal(5, 60, scale=0.1))
@@ -233,7 +235,7 @@ def random_ids(seed, n, top_k, experts, dropped=0.0, skew=0.0):
 
 @pytest.mark.parametrize("n,top_k,experts,dropped", [(0, 2, 5, 0), (1, 1, 1, 0), (1, 8, 64, 0), (1, 1, 1024, 0), (7, 3, 33, 0.3),
                                                      (500, 4, 16, 1.0), (2731, 6, 160, 0.1), (16384, 1, 8, 0), (16385, 1, 3, 0.1),
-                                                     (9000, 8, 256, 0.05), (4097, 17, 1000, 0.2), (131072, 2, 64, 0)])
+                                                     (9000, 8, 256, 0.05), (4097, 17, 1000, 0.2), (131072, 2, 64, 0), (8000, 1, 1024, 0.1), (8192, 1, 1, 0)])
 def test_plan(n, top_k, experts, dropped):
     ids = random_ids(n + experts, n, top_k, experts, dropped, 1.0)
     p = M.expert_plan(ids, experts)
@@ -309,6 +311,9 @@ SHAPES = [  # n, top_k, experts, k, width, dropped, skew
     (700, 1, 1, 384, 384, 0, 0),
     (64, 4, 8, 8, 1000, 1.0, 0),
     (999, 2, 40, 320, 48, 0.05, 1),
+    (2000, 2, 1000, 64, 64, 0.05, 1),
+    (2100, 4, 2, 64, 96, 0, 0.5),
+    (16, 1, 1, 264, 136, 0, 0),
 ]
 
 
@@ -332,10 +337,10 @@ def test_products_odd_widths(n, top_k, experts, k, width, gather, dtype):
 
 @pytest.mark.parametrize("gather", [True, False])
 @pytest.mark.parametrize("pad", [8, 3])
-def test_products_strides(gather, pad):
+@pytest.mark.parametrize("n,top_k,experts,k,width", [(150, 2, 5, 136, 264), (16, 1, 1, 64, 72), (7, 2, 4, 88, 40), (60, 2, 12, 64, 64)])
+def test_products_strides(n, top_k, experts, k, width, gather, pad):
     """Operands and outputs inside larger buffers; nothing beside the results is written."""
     dtype = torch.bfloat16
-    n, top_k, experts, k, width = 150, 2, 5, 136, 264
     plan, off, x, xs, w, g = setup_products(4, n, top_k, experts, k, width, dtype, gather, 0.1, 1)
 
     def inside(t):
@@ -532,9 +537,10 @@ def test_layer_forward_and_gradients(n, top_k):
         assert off(got, leaf.grad) < 0.01
 
 
-def test_layer_captured_and_replayed():
+@pytest.mark.parametrize("n", [4, 40, 900])
+def test_layer_captured_and_replayed(n):
     """The run captured once and replayed on other inputs equals the eager run, bit for bit, beside a second graph."""
-    experts, d, hidden, n, top_k = 16, 128, 192, 40, 3
+    experts, d, hidden, top_k = 16, 128, 192, 3
     gate = normal(2, experts, d, scale=d ** -0.5)
     w1 = normal(3, experts, hidden, d, dtype=torch.bfloat16, scale=d ** -0.5)
     w2 = normal(4, experts, d, hidden, dtype=torch.bfloat16, scale=hidden ** -0.5)
@@ -565,6 +571,42 @@ def test_layer_captured_and_replayed():
         for graph, x, go, outs in graphs:
             for a, b in zip(outs, whole(x, go)):
                 assert torch.equal(a, b)
+
+
+def test_offsets_past_32_bits():
+    """Rows and matrices that start more than 2^31 elements into their buffers: the last ones are checked."""
+    dtype, n, top_k, width = torch.bfloat16, 300000, 4, 2048
+    ids = torch.arange(n * top_k, dtype=torch.int32, device="cuda").view(n, top_k) % 3
+    plan = M.expert_plan(ids, 3)
+    y = torch.empty(n * top_k, width, dtype=dtype, device="cuda")
+    assert y.numel() > 2 ** 31
+    y.copy_((torch.arange(n * top_k, device="cuda") % 251)[:, None].to(dtype).expand(-1, width))
+    out = M.expert_combine(y, plan)
+    want = y[plan.pos.long().flatten(), 0].view(n, top_k).float().sum(1)       # sums of four integers under 251
+    assert torch.equal(out[:, 0].float(), want.to(dtype).float()) and torch.equal(out[:, -1], out[:, 0])
+    dy, dw = M.expert_combine_grad(out, y, plan)
+    token = plan.order.long() // top_k
+    assert torch.equal(dy[:, 5], out[token, 5]) and torch.equal(dy[-1], out[token[-1]])
+    del y, dy, dw, out
+    experts, k = 70, 4096                                                      # matrices of 8192 x 4096
+    w = torch.zeros(experts, 8192, k, dtype=dtype, device="cuda")
+    assert w.numel() > 2 ** 31
+    w[-1] = normal(1, 8192, k, dtype=dtype, scale=k ** -0.5)
+    for rows in (5, 400, 20000):
+        x = normal(2, rows, k, dtype=dtype)
+        plan = M.expert_plan(torch.full((rows, 1), experts - 1, dtype=torch.int32, device="cuda"), experts)
+        got = M.expert_gemm(x, w, plan)
+        at = [0, rows // 2, rows - 1]
+        want, mag = f64(x[at]) @ f64(w[-1]).T, np.abs(f64(x[at])) @ np.abs(f64(w[-1])).T
+        assert np.all(np.abs(f64(got[at]) - want) <= product_tolerance(want, mag, k, dtype))
+        g = normal(3, rows, 8192, dtype=dtype)
+        got = M.expert_gemm_grad_x(g, w, plan)
+        want, mag = f64(g[at]) @ f64(w[-1]), np.abs(f64(g[at])) @ np.abs(f64(w[-1]))
+        assert np.all(np.abs(f64(got[at]) - want) <= product_tolerance(want, mag, 8192, dtype))
+    dw = M.expert_gemm_grad_w(g[:400], x[:400], M.expert_plan(torch.full((400, 1), experts - 1, dtype=torch.int32, device="cuda"), experts), out=w)
+    want, mag = f64(g[:400]).T @ f64(x[:400, :64]), np.abs(f64(g[:400])).T @ np.abs(f64(x[:400, :64]))
+    assert np.all(np.abs(f64(dw[-1, :, :64]) - want) <= product_tolerance(want, mag, 400, dtype))
+    assert not dw[:-1].any()
 
 
 def test_two_streams_at_once():
