@@ -660,11 +660,17 @@ k_route_grad_whole(const T* __restrict__ logits, long long n, long long ld, Rout
  * writes each expert's run in one piece.
  *
  * Up to kPlanOne entries one block does everything; above, the blocks' counts
- * (k_plan_count), their prefixes (k_plan_scan) and the placement are three launches. */
+ * (k_plan_count), their prefixes (k_plan_scan) and the placement are three launches,
+ * each started as the one before it starts (programmatic dependent launch) and
+ * waiting for its end only where it reads its results: the placement ranks its
+ * entries meanwhile. */
 constexpr int kPlanThreads = 512, kPlanWarps = kPlanThreads / 32;
 constexpr int kPlanPer = 8;                                 /* entries a lane */
 constexpr int kPlanChunk = kPlanThreads * kPlanPer;         /* and a block of the multi-block plan */
 constexpr int kPlanOne = 2 * kPlanChunk;
+
+__device__ __forceinline__ void next_launch_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_last_launch() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 __device__ __forceinline__ int plan_id(const int* ids, long long i, long long end, int E) {
     const int a = i < end ? ids[i] : -1;
@@ -738,6 +744,7 @@ k_plan(const int* __restrict__ ids, long long m, int E, const int* __restrict__ 
         if (a[i] >= 0 && lane == __ffs(peers) - 1) mine[a[i]] = old + __popc(peers);
         __syncwarp();
     }
+    if (work) wait_for_last_launch();
     __syncthreads();
     int gcarry = 0, lcarry = 0;
     for (int e0 = 0; e0 < E; e0 += kPlanThreads) {
@@ -793,6 +800,7 @@ k_plan(const int* __restrict__ ids, long long m, int E, const int* __restrict__ 
 __global__ void __launch_bounds__(kPlanThreads)
 k_plan_count(const int* __restrict__ ids, long long m, int E, int* __restrict__ work) {
     extern __shared__ int plan_sm[];
+    next_launch_may_start();
     for (int e = threadIdx.x; e < E; e += kPlanThreads) plan_sm[e] = 0;
     __syncthreads();
     int a[kPlanPer];
@@ -810,6 +818,8 @@ k_plan_count(const int* __restrict__ ids, long long m, int E, int* __restrict__ 
  * its total goes behind them. */
 __global__ void k_plan_scan(int* __restrict__ work, int E, int B) {
     const int lane = threadIdx.x & 31, e = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    next_launch_may_start();
+    wait_for_last_launch();
     if (e >= E) return;
     int* row = work + (size_t)e * B;
     int run = 0;
@@ -922,6 +932,22 @@ bool type_ok(int type) { return type == MPK_TYPE_FP32 || type == MPK_TYPE_FP16 |
 
 long long plan_blocks(long long m) { return m <= kPlanOne ? 1 : (m + kPlanChunk - 1) / kPlanChunk; }
 
+/* A launch that may start as the one before it in the stream starts. */
+template <typename... P, typename... A>
+cudaError_t launch_behind(void (*kern)(P...), int grid, int block, int smem, cudaStream_t s, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3((unsigned)grid, 1, 1);
+    cfg.blockDim = dim3((unsigned)block, 1, 1);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, P(args)...);
+}
+
 template <int PER>
 cudaError_t run_plan(const int* ids, long long m, int E, int B, const int* work, int* offsets, int* order, int* pos,
                      cudaStream_t s) {
@@ -930,8 +956,11 @@ cudaError_t run_plan(const int* ids, long long m, int E, int B, const int* work,
         const cudaError_t e = cudaFuncSetAttribute(k_plan<PER>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return e;
     }
-    k_plan<PER><<<B, kPlanThreads, smem, s>>>(ids, m, E, work, offsets, order, pos);
-    return cudaGetLastError();
+    if (!work) {
+        k_plan<PER><<<B, kPlanThreads, smem, s>>>(ids, m, E, work, offsets, order, pos);
+        return cudaGetLastError();
+    }
+    return launch_behind(k_plan<PER>, B, kPlanThreads, smem, s, ids, m, E, work, offsets, order, pos);
 }
 
 }  /* namespace */
@@ -992,8 +1021,9 @@ mpkStatus mpkExpertPlan(cudaStream_t stream, const int* dIds, long long n, int t
     cudaError_t e;
     if (B > 1) {
         k_plan_count<<<B, kPlanThreads, experts * (int)sizeof(int), stream>>>(dIds, m, experts, work);
-        k_plan_scan<<<(experts + 7) / 8, 256, 0, stream>>>(work, experts, B);
-        e = run_plan<kPlanPer>(dIds, m, experts, B, work, dOffsets, dOrder, dPos, stream);
+        e = cudaGetLastError();
+        if (e == cudaSuccess) e = launch_behind(k_plan_scan, (experts + 7) / 8, 256, 0, stream, work, experts, B);
+        if (e == cudaSuccess) e = run_plan<kPlanPer>(dIds, m, experts, B, work, dOffsets, dOrder, dPos, stream);
     } else if (m <= kPlanThreads) {
         e = run_plan<1>(dIds, m, experts, 1, nullptr, dOffsets, dOrder, dPos, stream);
     } else if (m <= 4 * kPlanThreads) {
