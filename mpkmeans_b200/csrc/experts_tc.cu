@@ -112,7 +112,9 @@ static_assert(sizeof(Tile) % 16 == 0, "moved in 16-byte words");
 
 template <int STAGES>
 struct EMisc {
-    uint4 next[2];              /* answers to ask_next */
+    uint4 next[2];              /* answers to ask_next (CTA 0) */
+    int passed[2];              /* the same as CTA 0 passes them to CTA 1 */
+    int pad[2];
     Tile info[kInfo];           /* the tiles the producer has started */
     uint64_t full[STAGES], empty[STAGES], t_full[2], t_empty[2], s_full[2], s_empty[2], i_full[kInfo], i_empty[kInfo], fin;
     uint32_t tmem_slot;
@@ -170,17 +172,16 @@ __device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity) {
         if (globaltimer() - t0 > kWaitLimitNs) return;
 }
 
-/* Asks for the next cluster that has not started; the answer (16 bytes) comes to the
- * same place in every CTA of this cluster and counts on its barrier. */
-template <bool PAIR>
+/* Asks for the next cluster that has not started; the answer (16 bytes) comes to this
+ * CTA's shared memory and counts on its barrier. */
 __device__ __forceinline__ void ask_next(uint4* answer, uint64_t* bar) {
-    if (PAIR)
-        asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes"
-                     ".multicast::cluster::all.b128 [%0], [%1];"
-                     :: "r"(smem_u32(answer)), "r"(smem_u32(bar)) : "memory");
-    else
-        asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
-                     :: "r"(smem_u32(answer)), "r"(smem_u32(bar)) : "memory");
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+                 :: "r"(smem_u32(answer)), "r"(smem_u32(bar)) : "memory");
+}
+/* A word to another CTA of the cluster, counted on its barrier. */
+__device__ __forceinline__ void send_word(uint32_t cluster_addr, int v, uint32_t cluster_bar) {
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.u32 [%0], %1, [%2];"
+                 :: "r"(cluster_addr), "r"(v), "r"(cluster_bar) : "memory");
 }
 /* First block of the cluster taken over, or -1: none is left. */
 __device__ __forceinline__ int read_next(const uint4* answer) {
@@ -196,10 +197,6 @@ __device__ __forceinline__ int read_next(const uint4* answer) {
                  : "=r"(yes), "=r"(x) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w));
     return yes ? (int)x : -1;
 }
-__device__ __forceinline__ void mbar_expect_tx_cluster(uint32_t cluster_addr, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" :: "r"(cluster_addr), "r"(bytes) : "memory");
-}
-
 /* The tiles of all experts in the order they are worked on: expert by expert,
  * inside one kGroup row tiles at a time, their f tiles in turn, the row tiles
  * innermost -- clusters that run together then share a few tiles of W and of X, and
@@ -371,8 +368,7 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
                 ok = mbar_wait(&ms.s_empty[sl], ((uint32_t)(asked >> 1) & 1u) ^ 1u, abort_flag, &g_experts_status);
                 if (ok) {
                     mbar_expect_tx(&ms.s_full[sl], 16);
-                    if (PAIR) mbar_expect_tx_cluster(peer_addr(&ms.s_full[sl], 1), 16);
-                    ask_next<PAIR>(&ms.next[sl], &ms.s_full[sl]);
+                    ask_next(&ms.next[sl], &ms.s_full[sl]);
                 }
             }
             if (!__shfl_sync(0xffffffffu, ok ? 1 : 0, 0)) { ok = false; break; }
@@ -455,12 +451,16 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
             const int sl = (asked - 1) & 1;
             int x = -1, got = 0;
             if (lane == 0) {
+                if (rank == 1) mbar_expect_tx(&ms.s_full[sl], 4);
                 got = mbar_wait(&ms.s_full[sl], (uint32_t)((asked - 1) >> 1) & 1u, abort_flag, &g_experts_status) ? 1 : 0;
-                if (got) {
+                if (got && rank == 1) {
+                    x = *const_cast<volatile int*>(&ms.passed[sl]);
+                    mbar_arrive_cluster(peer_addr(&ms.s_empty[sl], 0));
+                } else if (got) {
                     x = read_next(&ms.next[sl]);
                     fence_async_proxy();
-                    if (PAIR) mbar_arrive_cluster(peer_addr(&ms.s_empty[sl], 0));
-                    else mbar_arrive(&ms.s_empty[sl]);
+                    if (PAIR) send_word(peer_addr(&ms.passed[sl], 1), x, peer_addr(&ms.s_full[sl], 1));
+                    mbar_arrive(&ms.s_empty[sl]);
                 }
             }
             ok = __shfl_sync(0xffffffffu, got, 0) != 0;
@@ -469,7 +469,7 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
         }
         if (!ok && lane == 0) {
             /* let what is in flight land before the CTA exits */
-            if (asked > 0) drain_wait(&ms.s_full[(asked - 1) & 1], (uint32_t)((asked - 1) >> 1) & 1u);
+            if (asked > 0 && rank == 0) drain_wait(&ms.s_full[(asked - 1) & 1], (uint32_t)((asked - 1) >> 1) & 1u);
             if (!PAIR) {
 #pragma unroll
                 for (int i = 0; i < STAGES; ++i)
