@@ -265,6 +265,9 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, bool bf16) {
     return r;
 }
 
+/* tmB: FWD, GRADX: boxes of 32 rows, tmBg one of 128 for the tiles that need four of
+ * those (GRADX of 32768 x 2048 by 4096, 32 experts: 478 us with four, 456 with one).
+ * GRADW: tmB 64 x 64 boxes, tmAg and tmBg single rows, tmAt and tmBt the tails. */
 template <int MODE, bool PAIR, int BN, int FMT>
 __global__ void __launch_bounds__(Cfg<PAIR, BN>::THREADS, 1)
 k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
@@ -426,8 +429,11 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
                             load3(&tmA, sa + BOX, f0 + 64, kc * BK, t.e);
                         }
                     }
-                    if (!gathers && lane < boxes)
+                    if (BL == 128 && boxes == 128 / BROWS) {
+                        if (lane == 0) load2(&tmBg, sb, kc * BK, t.r0 + jl);
+                    } else if (!gathers && lane < boxes) {
                         load2(&tmB, sb + lane * (BROWS * BK * 2), kc * BK, t.r0 + jl + BROWS * lane);
+                    }
                 } else {
                     const int r = t.r0 + kc * BK;
                     if (r + BK <= end) {
@@ -731,10 +737,12 @@ cudaError_t launch_t(const ExpertArgs& a, cudaStream_t s) {
     bool ok;
     if (MODE == EXP_FWD) {
         ok = row_map(&tmA, a.w, a.bf16, a.k, a.width, a.experts, a.ldw, a.stride_w, BM) &&
-             (a.order || row_map(&tmB, a.x, a.bf16, a.k, a.m, 0, a.ldx, 0, BROWS));
+             (a.order || (row_map(&tmB, a.x, a.bf16, a.k, a.m, 0, a.ldx, 0, BROWS) &&
+                          row_map(&tmBg, a.x, a.bf16, a.k, a.m, 0, a.ldx, 0, 128)));
     } else if (MODE == EXP_GRADX) {
         ok = row_map(&tmA, a.w, a.bf16, a.k, a.width, a.experts, a.ldw, a.stride_w, BK) &&
-             row_map(&tmB, a.gy, a.bf16, a.width, a.m, 0, a.ldgy, 0, BROWS);
+             row_map(&tmB, a.gy, a.bf16, a.width, a.m, 0, a.ldgy, 0, BROWS) &&
+             row_map(&tmBg, a.gy, a.bf16, a.width, a.m, 0, a.ldgy, 0, 128);
     } else {
         ok = row_map(&tmA, a.x, a.bf16, a.k, a.m, 0, a.ldx, 0, BK) && row_map(&tmAg, a.x, a.bf16, a.k, a.m, 0, a.ldx, 0, 1) &&
              row_map(&tmB, a.gy, a.bf16, a.width, a.m, 0, a.ldgy, 0, BK) &&
