@@ -32,7 +32,6 @@ namespace {
 constexpr unsigned FULL = 0xffffffffu;
 constexpr int kRouteWarps = 4;
 
-
 template <typename T>
 __device__ __forceinline__ float to_f(T v);
 template <>
@@ -212,7 +211,7 @@ __device__ __forceinline__ bool group_kept(unsigned long long gk, const RouteSha
  * first loser, and `close` says that the next slot's value is close; where that is
  * no exact tie (the same logit and bias) the order is decided again, and so is the
  * whole choice where the first loser is involved or `whole` is set.  (With 32 slots
- * no lane holds the first loser and every row is decided here.) */
+ * no lane holds the first loser and every row with a bias is decided here.) */
 template <typename T>
 __device__ __noinline__ int slow_choice(const T* __restrict__ row, const float* __restrict__ bias, RouteShape sh,
                                         unsigned long long* keys, int lane, int mine, bool close, bool whole) {
@@ -256,8 +255,10 @@ __device__ __noinline__ int slow_choice(const T* __restrict__ row, const float* 
     if (sh.G > 1) {
         const unsigned kept = __ballot_sync(FULL, group_kept(group_key(keys, sh, lane), sh, sh.log_l, lane));
         __syncwarp();
-        for (int j = lane; j < sh.E; j += 32)
+        for (int j = lane; j < sh.E; j += 32) {
             if (!((kept >> (((unsigned)j * sh.gmul >> 20) << sh.log_l)) & 1u)) keys[j] = 0ull;
+            else if (!bias) keys[j] = key_of((double)to_f(row[j]));      /* groups chosen: the logits' order again */
+        }
         __syncwarp();
     }
     mine = -1;
@@ -516,8 +517,8 @@ k_route(const T* __restrict__ logits, long long n, long long ld, const float* __
                 const unsigned nk = __shfl_down_sync(FULL, mykey, 1);
                 close = lane < sh.k && lane < 31 && live(nk) && near(of_key(mykey), of_key(nk));
             }
-            if (__any_sync(FULL, slow || close || sh.k == 32))
-                mine = slow_choice(row, bias, sh, keys64, lane, mine, close, slow || sh.k == 32);
+            const bool whole = slow || (bias && sh.k == 32);
+            if (__any_sync(FULL, whole || close)) mine = slow_choice(row, bias, sh, keys64, lane, mine, close, whole);
             if (lane >= sh.k) mine = -1;
             xi = mine >= 0 ? to_f(row[mine]) : -INFINITY;
         } else {
