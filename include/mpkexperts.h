@@ -15,7 +15,10 @@
  * can be captured into a CUDA graph (after one call outside a capture, which
  * loads the kernels).  Outputs and scratch overlap nothing else.  Leading dimensions (ld...) count elements.
  * A call with n = 0 (or m = 0) writes only what its comment says.  Bad arguments
- * return MPK_ERR_INVALID before anything is enqueued. */
+ * return MPK_ERR_INVALID before anything is enqueued.  The tensor-core products'
+ * waits are bounded (4 s): one that runs out ends the kernel with its output
+ * incomplete and sets the status word of mpkDebugExpertStatus
+ * (mpkmeans_debug.h). */
 #ifndef MPKEXPERTS_B200_H
 #define MPKEXPERTS_B200_H
 

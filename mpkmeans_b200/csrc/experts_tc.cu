@@ -34,7 +34,7 @@
  * TMA's gather4, 45 ns an instruction; sorted rows take 0.47 ms and the copy
  * 0.06 ms.)
  *
- * Few rows an expert: one CTA, 128 f x 32 j, bound by reading W once, eleven
+ * Few rows an expert: one CTA, 128 f x 32 j, bound by reading W once, ten
  * stages of 20 KB in flight.  Gathered rows come by cp.async in warps 10-15, 16
  * bytes a copy, into the same swizzled layout.  Warp w fills ring slots w, w + 6,
  * ...: handing a stage to the tensor cores (proxy fence, arrive) waits for all

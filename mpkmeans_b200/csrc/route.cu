@@ -9,6 +9,8 @@
  * and few others do: about ten of 256 for top_k = 8.  Those are packed one a lane
  * and ranked against each other.  (Taking the maximum top_k times, rescanning the
  * registers of the lane that held it, was a third of 1800 instructions a row.)
+ * Bound by instruction issue: 32768 x 256 FP32 takes 24 us with softmax, 43 with
+ * sigmoid, bias and groups.
  *
  * The choice is exact, as the assignment's is: without a bias, and with groups
  * scored by their maximum, the order of c is the order of l and the keys are the
@@ -664,7 +666,9 @@ k_route_grad_whole(const T* __restrict__ logits, long long n, long long ld, Rout
  * (k_plan_count), their prefixes (k_plan_scan) and the placement are three launches,
  * each started as the one before it starts (programmatic dependent launch) and
  * waiting for its end only where it reads its results: the placement ranks its
- * entries meanwhile. */
+ * entries meanwhile.  Bound by the latency of those phases, not by memory: 15 us on
+ * the device for 1048576 entries of 256 experts.  Chunks of 2048 entries took 18 us
+ * there and 7 instead of 9 for 131072; one of 8192 14 and 13. */
 constexpr int kPlanThreads = 512, kPlanWarps = kPlanThreads / 32;
 constexpr int kPlanPer = 8;                                 /* entries a lane */
 constexpr int kPlanChunk = kPlanThreads * kPlanPer;         /* and a block of the multi-block plan */
