@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(kAnyThreads) k_experts_any(const ExpertArgs a)
                     fe = e0 + l;
                     ft = (int)blockIdx.x - run - __shfl_sync(FULL, incl - t, l);
                 }
-                run += __shfl_sync(FULL, incl, 31);
+                run = min(run + __shfl_sync(FULL, incl, 31), 1 << 29);   /* more than any plan's tiles */
             }
             if (lane == 0) { where[0] = fe; where[1] = fe < 0 ? (int)blockIdx.x - run : ft; }
         }

@@ -31,7 +31,7 @@
  * up to 32), so the last tile of a segment costs its share.  X comes sorted: the
  * caller copies gathered rows first.  (Gathering 128-byte pieces of rows inside
  * this kernel held 32768 x 4096 by 2048 at 0.80 ms with cp.async and 1.45 ms with
- * TMA's gather4, 45 ns an instruction; sorted rows take 0.47 ms and the copy
+ * TMA's gather4, 45 ns an instruction; sorted rows take 0.45 ms and the copy
  * 0.06 ms.)
  *
  * Few rows an expert: one CTA, 128 f x 32 j, bound by reading W once, ten
@@ -77,6 +77,7 @@ constexpr int BOX = 64 * 64 * 2;                 /* one 64 x 64 MN-major box */
 constexpr int kSmemMax = 232448;
 constexpr int kMisc = 1024 + 8 * (MPK_MAX_EXPERTS + 1);
 constexpr int kInfo = 4;                         /* tiles between the producer and the epilogue */
+constexpr int kMostTiles = 1 << 29;              /* more than any plan's; offsets that are none stay below it */
 constexpr int kGroup = 8;                        /* row tiles that sweep the f tiles together */
 
 template <bool PAIR, int BN>
@@ -325,8 +326,8 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
                 const int v = __shfl_up_sync(0xffffffffu, incl, o);
                 if (lane >= o) incl += v;
             }
-            if (e < p.experts) start[e] = run + incl - t;
-            run += __shfl_sync(0xffffffffu, incl, 31);
+            if (e < p.experts) start[e] = min(run + incl - t, kMostTiles);
+            run = min(run + __shfl_sync(0xffffffffu, incl, 31), kMostTiles);
         }
         if (lane == 0) {
             start[p.experts] = run;
