@@ -546,6 +546,14 @@ def _matrix(name: str, t, rows: int | None = None, cols: int | None = None, dtyp
     return t.data_ptr(), ld
 
 
+def _output(out, rows: int, cols: int, like) -> tuple:
+    """(out, address, row stride): a new rows x cols matrix like `like` when out is None."""
+    if out is None:
+        out = like.new_empty((rows, cols))
+        return out, out.data_ptr(), cols
+    return (out, *_matrix("out", out, rows, cols, like.dtype))
+
+
 def _type_of(name: str, t, least: int = 0) -> int:
     """mpkType of a tensor; least 1 leaves FP32 out."""
     code = _types().get(t.dtype, -1)
@@ -594,7 +602,7 @@ def _run(fn_name: str, tensors: tuple, *args) -> None:
             raise ValueError(f"{fn_name}: tensors on {tensors[0].device} and {t.device}")
     stream = torch._C._cuda_getCurrentRawStream(device)
     fn = getattr(_lib or lib(), fn_name)
-    if device == torch.cuda.current_device():
+    if device == torch._C._cuda_getDevice():
         status = fn(stream, *args)
     else:
         with torch.cuda.device(device):
@@ -642,9 +650,7 @@ def route_grad(grad_weights, logits, ids, *, score: str = "softmax", renormalize
         raise ValueError(f"ids: expected n x top_k, got {tuple(ids.shape)}")
     top_k = ids.shape[1]
     params = _route_params(experts, top_k, score, 1, 1, "max", renormalize, scale)
-    if out is None:
-        out = torch.empty((n, experts), dtype=logits.dtype, device=logits.device)
-    address_out, ldg = _matrix("out", out, n, experts, logits.dtype)
+    out, address_out, ldg = _output(out, n, experts, logits)
     _run("mpkRouteGrad", (logits, ids, grad_weights, out), ctypes.byref(params), address,
          code, n, ld, _array("ids", ids, torch.int32, n, top_k),
          _array("grad_weights", grad_weights, torch.float32, n, top_k), address_out, ldg)
@@ -666,9 +672,12 @@ class ExpertPlan:
         self.rows = self.n * self.top_k
         self.experts = offsets.shape[0] - 1
         int32 = _types() and torch.int32
-        _array("offsets", offsets, int32, self.experts + 1)
-        _array("order", order, int32, self.rows)
-        _array("pos", pos, int32, self.n, self.top_k)
+        if not (offsets.dtype == order.dtype == pos.dtype == int32 and order.shape == (self.rows,) and
+                offsets.is_cuda and order.is_cuda and pos.is_cuda and
+                offsets.is_contiguous() and order.is_contiguous() and pos.is_contiguous()):
+            _array("offsets", offsets, int32, self.experts + 1)      # says what is wrong
+            _array("order", order, int32, self.rows)
+            _array("pos", pos, int32, self.n, self.top_k)
         self.offsets, self.order, self.pos = offsets, order, pos
 
 
@@ -684,7 +693,7 @@ def expert_plan(ids, experts: int) -> ExpertPlan:
     offsets = ids.new_empty(max(experts, 0) + 1)
     order = ids.new_empty(rows)
     pos = ids.new_empty((n, top_k))
-    work = torch.empty(need, dtype=torch.uint8, device=ids.device) if need else None
+    work = ids.new_empty(need // 4) if need else None
     _run("mpkExpertPlan", (ids,), address, n, top_k, experts, offsets.data_ptr(), order.data_ptr(),
          pos.data_ptr(), None if work is None else work.data_ptr(), need)
     plan = object.__new__(ExpertPlan)
@@ -709,9 +718,7 @@ def expert_gemm(x, w, plan: ExpertPlan, *, gather: bool = True, out=None):
     address, ldx = _matrix("x", x, plan.n if gather else plan.rows)
     pw, ldw, sw = _matrices("w", w, x.dtype, (plan.experts, None, x.shape[1]))
     width, k = w.shape[1], w.shape[2]
-    if out is None:
-        out = torch.empty((plan.rows, width), dtype=x.dtype, device=x.device)
-    po, ldo = _matrix("out", out, plan.rows, width, x.dtype)
+    out, po, ldo = _output(out, plan.rows, width, x)
     work, pwork, need = _sorted_copy(0, x, plan, gather)
     _run("mpkExpertGemm", (x, w, plan.offsets, plan.order, out), code, address, ldx, pw, ldw, sw,
          plan.offsets.data_ptr(), plan.order.data_ptr() if gather else None, plan.top_k, plan.rows, plan.experts,
@@ -727,9 +734,7 @@ def expert_gemm_grad_x(grad, w, plan: ExpertPlan, *, out=None):
     address, ldg = _matrix("grad", grad, plan.rows)
     pw, ldw, sw = _matrices("w", w, grad.dtype, (plan.experts, grad.shape[1], None))
     width, k = w.shape[1], w.shape[2]
-    if out is None:
-        out = torch.empty((plan.rows, k), dtype=grad.dtype, device=grad.device)
-    po, ldo = _matrix("out", out, plan.rows, k, grad.dtype)
+    out, po, ldo = _output(out, plan.rows, k, grad)
     _run("mpkExpertGemmGradX", (grad, w, plan.offsets, out), code, address, ldg, pw, ldw, sw,
          plan.offsets.data_ptr(), plan.rows, plan.experts, width, k, po, ldo)
     return out
@@ -743,7 +748,7 @@ def expert_gemm_grad_w(grad, x, plan: ExpertPlan, *, gather: bool = True, out=No
     pg, ldg = _matrix("grad", grad, plan.rows, None, x.dtype)
     width, k = grad.shape[1], x.shape[1]
     if out is None:
-        out = torch.empty((plan.experts, width, k), dtype=x.dtype, device=x.device)
+        out = x.new_empty((plan.experts, width, k))
     po, ldo, so = _matrices("out", out, x.dtype, (plan.experts, width, k))
     work, pwork, need = _sorted_copy(1, x, plan, gather)
     _run("mpkExpertGemmGradW", (grad, x, plan.offsets, plan.order, out), code, pg, ldg, address,
@@ -758,9 +763,7 @@ def expert_combine(y, plan: ExpertPlan, weights=None, *, out=None):
     code = _type_of("y", y)
     address, ldy = _matrix("y", y, plan.rows)
     width = y.shape[1]
-    if out is None:
-        out = torch.empty((plan.n, width), dtype=y.dtype, device=y.device)
-    po, ldo = _matrix("out", out, plan.n, width, y.dtype)
+    out, po, ldo = _output(out, plan.n, width, y)
     used = (y, plan.pos, out) if weights is None else (y, plan.pos, out, weights)
     pweights = None if weights is None else _array("weights", weights, torch.float32, plan.n, plan.top_k)
     _run("mpkExpertCombine", used, code, address, ldy, plan.pos.data_ptr(), pweights, plan.n,
@@ -775,14 +778,12 @@ def expert_combine_grad(grad, y, plan: ExpertPlan, weights=None, *, out=None):
     code = _type_of("grad", grad)
     address, ldgo = _matrix("grad", grad, plan.n)
     width = grad.shape[1]
-    if out is None:
-        out = torch.empty((plan.rows, width), dtype=grad.dtype, device=grad.device)
-    po, ldo = _matrix("out", out, plan.rows, width, grad.dtype)
+    out, po, ldo = _output(out, plan.rows, width, grad)
     used = [grad, plan.pos, plan.offsets, out]
     py, ldy, grad_weights, pgw, pweights = None, 0, None, None, None
     if y is not None:
         py, ldy = _matrix("y", y, plan.rows, width, grad.dtype)
-        grad_weights = torch.empty((plan.n, plan.top_k), dtype=torch.float32, device=grad.device)
+        grad_weights = grad.new_empty((plan.n, plan.top_k), dtype=torch.float32)
         pgw = grad_weights.data_ptr()
         used.append(y)
     if weights is not None:

@@ -5,6 +5,7 @@
 #include "experts.cuh"
 #include "mpkexperts.h"
 
+#include <atomic>
 #include <type_traits>
 
 namespace mpk {
@@ -502,13 +503,6 @@ k_combine_grad(const T* __restrict__ go, long long ldgo, const T* __restrict__ y
 
 /* ------------------------------------------------------------- host side ---- */
 
-int sm_count() {
-    int dev = 0, sms = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-    return sms;
-}
-
 bool half_type(int type) { return type == MPK_TYPE_FP16 || type == MPK_TYPE_BF16; }
 
 bool aligned16(const void* p, long long ld, size_t size) {
@@ -632,6 +626,17 @@ bool combine_ok(int type, long long n, int top_k, int width) {
 }
 
 }  /* namespace */
+
+int sm_count() {
+    static std::atomic<int> known[64];
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    if (dev >= 0 && dev < 64 && (sms = known[dev].load(std::memory_order_relaxed)) > 0) return sms;
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    if (dev >= 0 && dev < 64) known[dev].store(sms, std::memory_order_relaxed);
+    return sms;
+}
+
 }  /* namespace mpk */
 
 using namespace mpk;

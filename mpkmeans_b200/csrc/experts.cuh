@@ -38,6 +38,9 @@ bool experts_few_rows(long long m, int experts);
 bool experts_tc_ok(const ExpertArgs& a);
 cudaError_t launch_experts_tc(const ExpertArgs& a, cudaStream_t s);
 
+/* Multiprocessors of the current device, 0 on an error; looked up once a device. */
+int sm_count();
+
 /* Sorted row range of expert e, clamped to the rows there are. */
 __device__ __forceinline__ int expert_start(const int* offsets, int e, int m) {
     const int o = offsets[e];

@@ -21,7 +21,7 @@
  * and the same bias, which is an exact tie.  The scores of a 256-expert row lie
  * some 1e-3 apart and the bound is about 1e-6, so few rows go there.
  */
-#include "common.cuh"
+#include "experts.cuh"
 #include "mpkexperts.h"
 
 #include <climits>
@@ -864,13 +864,6 @@ bool route_shape(const mpkRouteParams* p, RouteShape& sh, bool choice) {
     /* j * gmul / 2^20 exceeds j / gs by less than j / 2^20 < 1 / gs */
     sh.gmul = ((1u << 20) + sh.gs - 1) / sh.gs;
     return true;
-}
-
-int sm_count() {
-    int dev = 0, sms = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-    return sms;
 }
 
 /* one warp a token until every SM holds its 16 blocks of four warps */
