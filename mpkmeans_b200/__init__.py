@@ -633,7 +633,7 @@ def route(logits, top_k: int, *, score: str = "softmax", bias=None, groups: int 
     used = (logits,) if bias is None else (logits, bias)
     pbias = None if bias is None else _array("bias", bias, torch.float32, experts)
     ids = logits.new_empty((n, max(top_k, 0)), dtype=torch.int32)
-    weights = logits.new_empty((n, max(top_k, 0)), dtype=torch.float32)
+    weights = torch.empty_like(ids, dtype=torch.float32)
     _run("mpkRoute", used, ctypes.byref(params), address, code, n, ld, pbias, ids.data_ptr(),
          weights.data_ptr())
     return ids, weights
@@ -692,7 +692,7 @@ def expert_plan(ids, experts: int) -> ExpertPlan:
     rows = n * top_k
     offsets = ids.new_empty(max(experts, 0) + 1)
     order = ids.new_empty(rows)
-    pos = ids.new_empty((n, top_k))
+    pos = torch.empty_like(ids)                        # ids is contiguous
     work = ids.new_empty(need // 4) if need else None
     _run("mpkExpertPlan", (ids,), address, n, top_k, experts, offsets.data_ptr(), order.data_ptr(),
          pos.data_ptr(), None if work is None else work.data_ptr(), need)
