@@ -415,6 +415,16 @@ k_route(const T* __restrict__ logits, long long n, long long ld, const float* __
 #pragma unroll
         for (int v = 0; v < VPL; ++v) bv[v] = bias_of(v);
     }
+    float most = 1.f;                                          /* no finite |c| exceeds it */
+    if constexpr (BY_SCORE && GROUPS != 0) {
+        float b = 0.f;
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) {
+            const float a = fabsf(KEEP ? bv[KEEP ? v : 0] : bias_of(v));
+            b = a < INFINITY ? fmaxf(b, a) : b;
+        }
+        most += warp_max(b);
+    }
     const long long step = (long long)gridDim.x * kRouteWarps;
     for (long long t = (long long)blockIdx.x * kRouteWarps + warp; t < n; t += step) {
         const T* row = logits + t * ld;
@@ -464,6 +474,11 @@ k_route(const T* __restrict__ logits, long long n, long long ld, const float* __
                                    : 0x1.0p-15f * (fabsf(a) + fabsf(b)) + 1e-37f;
             return !(a - b > tol);
         };
+        /* A group's value may be the sum of two c of opposite signs: twice the bound, and roundings (of both and of
+         * the sum) that are relative to the largest |c|, not to the sum. */
+        auto near_groups = [&](float a, float b) {
+            return bias ? !(a - b > (softmax ? 0x1.0p-17f * smax : 0x1.4p-20f) + 0x1.0p-21f * most) : near(a, b);
+        };
         bool slow = false;                                         /* the groups are not certain */
         if constexpr (GROUPS != 0) {
             unsigned gk;
@@ -506,7 +521,7 @@ k_route(const T* __restrict__ logits, long long n, long long ld, const float* __
                 const bool there = (lane >> log) < sh.G;
                 const unsigned lo = __reduce_min_sync(FULL, in ? gk : 0xffffffffu);
                 const unsigned hi = __reduce_max_sync(FULL, there && !in ? gk : 0u);
-                slow = live(hi) && near(of_key(lo), of_key(hi));
+                slow = live(hi) && near_groups(of_key(lo), of_key(hi));
             }
         }
         int mine;

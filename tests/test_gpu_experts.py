@@ -91,6 +91,19 @@ def test_route_near_ties_are_decided_exactly(score):
     check_route(x, 16, score=score, groups=8, top_groups=3, group_score="top2")
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_route_near_groups_are_decided_exactly(score):
+    """Groups whose sums differ by less than FP32 scores are off, with biases that cancel inside a group."""
+    gen = np.random.default_rng(2)
+    base = gen.normal(size=(400, 8))
+    x = np.concatenate([base + gen.integers(-3, 4, size=base.shape) * 2.0 ** -23 * np.abs(base) for _ in range(4)], 1)
+    x = torch.from_numpy(x.astype(np.float32)).cuda()
+    for size in (0.0, 1.0, 20.0):
+        bias = torch.from_numpy(np.tile(size * gen.normal(size=8), 4).astype(np.float32)).cuda()
+        for group_score in ("max", "top2"):
+            check_route(x, 6, score=score, bias=bias, groups=4, top_groups=2, group_score=group_score)
+
+
 def test_route_saturated_scores_follow_the_logits():
     """Sigmoids that FP64 rounds to one another: the order stays the logits', in rows decided in FP64 too."""
     x = torch.full((4, 64), -1.0, device="cuda")
