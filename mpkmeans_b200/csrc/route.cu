@@ -9,7 +9,7 @@
  * and few others do: about ten of 256 for top_k = 8.  Those are packed one a lane
  * and ranked against each other.  (Taking the maximum top_k times, rescanning the
  * registers of the lane that held it, was a third of 1800 instructions a row.)
- * Bound by instruction issue: 32768 x 256 FP32 takes 24 us with softmax, 43 with
+ * Bound by instruction issue: 32768 x 256 FP32 takes 24 us with softmax, 41 to 47 with
  * sigmoid, bias and groups.
  *
  * The choice is exact, as the assignment's is: without a bias, and with groups
