@@ -18,8 +18,11 @@
  * row in which two neighbours of the chosen sequence (the first loser included)
  * or the groups on both sides of the cut come within twice that bound is
  * decided again in FP64 (slow_choice), except where the two have the same logit
- * and the same bias, which is an exact tie.  The scores of a 256-expert row lie
- * some 1e-3 apart and the bound is about 1e-6, so few rows go there.
+ * and the same bias, which is an exact tie.  A tie of the last slot with the
+ * first loser says nothing of the losers behind: those within the bound of the
+ * tie that the logits' order does not settle send the row to FP64 too, and so
+ * does any other near pair of it.  The scores of a 256-expert row lie some 1e-3
+ * apart and the bound is about 1e-6, so few rows go there.
  */
 #include "experts.cuh"
 #include "mpkexperts.h"
@@ -212,13 +215,17 @@ __device__ __forceinline__ bool group_kept(unsigned long long gk, const RouteSha
  * of this warp's shared memory.  Slot `lane` has `mine` so far, slot k being the
  * first loser, and `close` says that the next slot's value is close; where that is
  * no exact tie (the same logit and bias) the order is decided again, and so is the
- * whole choice where the first loser is involved or `whole` is set.  (With 32 slots
- * no lane holds the first loser and every row with a bias is decided here.) */
+ * whole choice where the first loser is involved, as the tie of the last slot or in
+ * the near pair, or `whole` is set.  (With 32 slots no lane holds the first loser
+ * and every row with a bias is decided here.) */
 template <typename T>
 __device__ __noinline__ int slow_choice(const T* __restrict__ row, const float* __restrict__ bias, RouteShape sh,
                                         unsigned long long* keys, int lane, int mine, bool close, bool whole) {
     const int nj = __shfl_down_sync(FULL, mine, 1);
-    if (close && mine >= 0 && nj >= 0) close = !(to_f(row[mine]) == to_f(row[nj]) && bias[mine] == bias[nj]);
+    const bool tie = close && mine >= 0 && nj >= 0 && to_f(row[mine]) == to_f(row[nj]) && bias[mine] == bias[nj];
+    close = close && !tie;
+    const bool cut_tie = __any_sync(FULL, tie && lane == sh.k - 1), others = __any_sync(FULL, close);
+    whole = whole || (cut_tie && others);
     const bool order_only = !__any_sync(FULL, whole || (close && lane == sh.k - 1));
     if (!__any_sync(FULL, whole || close)) return mine;
     if (lane >= sh.k) mine = -1;
@@ -534,7 +541,20 @@ k_route(const T* __restrict__ logits, long long n, long long ld, const float* __
                 const unsigned nk = __shfl_down_sync(FULL, mykey, 1);
                 close = lane < sh.k && lane < 31 && live(nk) && near(of_key(mykey), of_key(nk));
             }
-            const bool whole = slow || (bias && sh.k == 32);
+            bool whole = slow || (bias && sh.k == 32);
+            if (__any_sync(FULL, close && lane == sh.k - 1)) {
+                /* the last slot may tie with the first loser: another that is near it is no higher only where
+                 * the bias is the same and the logit no higher */
+                const unsigned tk = __shfl_sync(FULL, mykey, sh.k - 1);
+                const int tj = __shfl_sync(FULL, mine, sh.k - 1);
+                const float tx = to_f(row[tj]), tb = bias[tj];
+#pragma unroll
+                for (int v = 0; v < VPL; ++v)
+                    if (live(key[v]) && key[v] <= tk && near(of_key(tk), of_key(key[v]))) {
+                        const int j = VPL * lane + v;
+                        if (!(bias[j] == tb && to_f(row[j]) <= tx)) whole = true;
+                    }
+            }
             if (__any_sync(FULL, whole || close)) mine = slow_choice(row, bias, sh, keys64, lane, mine, close, whole);
             if (lane >= sh.k) mine = -1;
             xi = mine >= 0 ? to_f(row[mine]) : -INFINITY;

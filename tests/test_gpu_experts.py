@@ -694,3 +694,34 @@ def test_mirror_refuses_on_the_gpu():
         M.expert_gemm(x.half(), w.transpose(1, 2), plan)
     with pytest.raises(ValueError):
         M.expert_gemm(x.half(), w, plan, out=torch.empty(8, 15, dtype=torch.float16, device="cuda"))
+
+
+@pytest.mark.parametrize("score,bias,row,top_k", [("sigmoid", 0.0, [18, 18, 18.125], 1), ("sigmoid", 0.0, [20, 20, 21], 1),
+                                                  ("sigmoid", 0.0, [20, 20, 21], 2), ("sigmoid", 0.0, [20, 21, 21], 2),
+                                                  ("softmax", 0.1, [10, -15, -15, -14.9375], 2)])
+def test_route_ties_at_the_cut(score, bias, row, top_k):
+    """The last slot and the first loser have the same logit and bias, and FP32 cannot tell another loser, or the slot
+    before, from them: the higher logit is chosen."""
+    x = torch.tensor([row, row[::-1], row], dtype=torch.float32, device="cuda")
+    check_route(x, top_k, score=score, bias=torch.full((len(row),), bias, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts,top_k", [(5, 2), (64, 1), (64, 6), (256, 8), (256, 31), (1000, 7)])
+def test_route_ties_at_the_cut_of_coarse_logits(experts, top_k, score, dtype):
+    """Few distinct logits and equal biases: exact ties everywhere, between values that FP32 scores round to one
+    another (sigmoids of 16 to 20; softmax values 1e-11 beside a bias of 0.1) but FP64 tells apart."""
+    rng = np.random.default_rng(experts + top_k)
+    x = rng.integers(0, 9, size=(40, experts)) / 2 + (16 if score == "sigmoid" else -16)
+    x[20:] = np.where(rng.random((20, experts)) < 0.9, x[20:].min(), x[20:])     # most at the lowest value
+    if score == "softmax":
+        x[:, 0] = 10
+    x = torch.from_numpy(x.astype(np.float32)).to(TYPES[dtype]).cuda()
+    check_route(x, top_k, score=score, bias=torch.full((experts,), 0.1 if score == "softmax" else 0.0, device="cuda"))
+    if experts % 4 == 0:
+        check_route(x, min(top_k, experts // 2), score=score, bias=torch.full((experts,), 0.1, device="cuda"), groups=4,
+                    top_groups=2, group_score="top2")
+    # biases one step apart: what is near a tie at the cut may have another bias
+    steps = torch.from_numpy((np.float32(0.1) + rng.integers(0, 3, experts) * np.float32(2.0 ** -27)).astype(np.float32)).cuda()
+    check_route(x, top_k, score=score, bias=steps)
