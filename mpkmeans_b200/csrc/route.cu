@@ -470,21 +470,27 @@ k_route(const T* __restrict__ logits, long long n, long long ld, const float* __
 #pragma unroll
             for (int v = 0; v < VPL; ++v) key[v] = key_of(x[v]);
         }
-        /* Error bounds of c.  e^d from exp2_fast is off by (2^-22 + 1.5 |d| 2^-24) of itself: the instruction,
-         * and the rounding of d log2 e.  A sigmoid turns that into s (1 - s) of it, under 2^-23, and adds 2^-23 s
-         * for the reciprocal and 2^-24 for the sum, 2.1 2^-23 in all; a softmax value adds its argument's rounding, |d| 2^-24, and the
-         * sum's and reciprocal's error, which all scores share: under 2^-20 of the row's largest score in all, and
-         * (1 + 0.7 |d|) 2^-22 of the score itself, under 2^-16 of it wherever it does not underflow.  Adding the
-         * bias rounds by 2^-24 |c|. */
+        /* Error bounds of c, in units of 2^-24.  e^d from exp2_fast is off by 4 + 2.3 |d| of itself: the instruction,
+         * and for a softmax value the roundings of d = x - mx, of its product with log2 e and of that constant (1.3 |d|
+         * for a sigmoid, whose argument is exact).
+         * A sigmoid turns that into s (1 - s) of it, under 1.1, and adds 2 s for the reciprocal and s for the sum: 4.1.
+         * A softmax value e / sum <= smax is off by 4 smax for e (the largest of e^d (4 + 2.3 |d|)) and smax for the
+         * product.  The sum's error is shared by all of the row's values and moves a difference of two by no more than
+         * its share of smax: VPL + 4 for VPL - 1 additions in a lane and 5 between lanes, the mean of the exponentials'
+         * errors, 4 + 2.3 ln E (the mean of |d| is an entropy, ln E at most), and 2 for the reciprocal.  Two values:
+         * VPL + 20 + 2.3 ln E, 29 for one expert a lane, 41 for 8, 68 for 32; the VPL + 40 below is above it for all.
+         * Relative to a value alone, 5 + 2.3 |d| and the shared part come to under 2^-15 wherever e^d does not
+         * underflow.  Adding the bias rounds by |c|. */
+        constexpr float kSoftmaxTol = (VPL + 40) * 0x1.0p-24f;
         auto near = [&](float a, float b) {
-            const float tol = bias ? (softmax ? 0x1.0p-18f : 0x1.4p-21f) * smax + 0x1.1p-24f * (fabsf(a) + fabsf(b))
+            const float tol = bias ? (softmax ? kSoftmaxTol : 0x1.4p-21f) * smax + 0x1.1p-24f * (fabsf(a) + fabsf(b))
                                    : 0x1.0p-15f * (fabsf(a) + fabsf(b)) + 1e-37f;
             return !(a - b > tol);
         };
         /* A group's value may be the sum of two c of opposite signs: twice the bound, and roundings (of both and of
          * the sum) that are relative to the largest |c|, not to the sum. */
         auto near_groups = [&](float a, float b) {
-            return bias ? !(a - b > (softmax ? 0x1.0p-17f * smax : 0x1.4p-20f) + 0x1.0p-21f * most) : near(a, b);
+            return bias ? !(a - b > (softmax ? 2.f * kSoftmaxTol * smax : 0x1.4p-20f) + 0x1.0p-21f * most) : near(a, b);
         };
         bool slow = false;                                         /* the groups are not certain */
         if constexpr (GROUPS != 0) {

@@ -725,3 +725,19 @@ def test_route_ties_at_the_cut_of_coarse_logits(experts, top_k, score, dtype):
     # biases one step apart: what is near a tie at the cut may have another bias
     steps = torch.from_numpy((np.float32(0.1) + rng.integers(0, 3, experts) * np.float32(2.0 ** -27)).astype(np.float32)).cuda()
     check_route(x, top_k, score=score, bias=steps)
+
+
+@pytest.mark.parametrize("experts", [256, 512, 1024])
+def test_route_near_ties_of_wide_rows(experts):
+    """Softmax rows whose sum is many roundings long, with biases that put pairs of choice values within one another's
+    error bound: c of one expert is that of the next to 1e-8."""
+    rng = np.random.default_rng(experts)
+    for scale in (0.01, 2.0):
+        x = (scale * rng.normal(size=(30, experts))).astype(np.float32)
+        s = R.softmax(x.astype(np.float64)).mean(0)
+        bias = (0.1 - s).astype(np.float32)                    # all c of an average row equal
+        check_route(torch.from_numpy(x).cuda(), 8, bias=torch.from_numpy(bias).cuda())
+        same = np.tile(x[:1], (30, 1)) + (rng.integers(-2, 3, x.shape) * 2.0 ** -22 * np.abs(x)).astype(np.float32)
+        bias = (0.1 - R.softmax(x[:1].astype(np.float64))[0]).astype(np.float32)
+        for top_k in (1, 8):
+            check_route(torch.from_numpy(same).cuda(), top_k, bias=torch.from_numpy(bias).cuda())
