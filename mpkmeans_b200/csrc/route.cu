@@ -990,9 +990,12 @@ cudaError_t launch_behind(void (*kern)(P...), int grid, int block, int smem, cud
 template <int PER>
 cudaError_t run_plan(const int* ids, long long m, int E, int B, const int* work, int* offsets, int* order, int* pos,
                      cudaStream_t s) {
-    const int smem = (kPlanWarps + 2) * E * (int)sizeof(int) + kPlanThreads * PER * 6;
+    const auto bytes = [](int experts) { return (kPlanWarps + 2) * experts * (int)sizeof(int) + kPlanThreads * PER * 6; };
+    const int smem = bytes(E);
     if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(k_plan<PER>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        /* the limit belongs to the kernel, not to this call: every call sets the same */
+        const cudaError_t e =
+            cudaFuncSetAttribute(k_plan<PER>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes(MPK_MAX_EXPERTS));
         if (e != cudaSuccess) return e;
     }
     if (!work) {

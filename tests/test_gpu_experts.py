@@ -741,3 +741,32 @@ def test_route_near_ties_of_wide_rows(experts):
         bias = (0.1 - R.softmax(x[:1].astype(np.float64))[0]).astype(np.float32)
         for top_k in (1, 8):
             check_route(torch.from_numpy(same).cuda(), top_k, bias=torch.from_numpy(bias).cuda())
+
+
+def test_plans_of_two_threads():
+    """Two host threads that plan at once with different numbers of experts: every call returns its plan."""
+    import threading
+    sets = [(random_ids(e, 2000, 3, e, 0.1), e) for e in (1024, 40)]
+    want = [R.plan(ids.cpu().numpy(), e) for ids, e in sets]
+    plans, errors = [[], []], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(400):
+                    plans[i].append(M.expert_plan(*sets[i]))
+        except Exception as e:                                 # handed to the test's own thread
+            errors.append(e)
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors
+    for got, w in zip(plans, want):
+        for p in got:
+            for a, b in zip((p.offsets, p.order, p.pos), w):
+                assert np.array_equal(a.cpu().numpy(), b)
