@@ -718,6 +718,10 @@ constexpr int kPlanOne = 2 * kPlanChunk;
 __device__ __forceinline__ void next_launch_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_last_launch() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+/* A word that an earlier launch may write while this kernel runs: read where it stands, behind wait_for_last_launch
+ * (no read-only load, none moved before the wait). */
+__device__ __forceinline__ int waited_for(const int* p) { return *static_cast<const volatile int*>(p); }
+
 __device__ __forceinline__ int plan_id(const int* ids, long long i, long long end, int E) {
     const int a = i < end ? ids[i] : -1;
     return (unsigned)a < (unsigned)E ? a : -1;
@@ -762,7 +766,7 @@ __device__ __forceinline__ int block_scan(int v, int* part, int& tot) {
  * behind them. */
 template <int PER>
 __global__ void __launch_bounds__(kPlanThreads)
-k_plan(const int* __restrict__ ids, long long m, int E, const int* __restrict__ work, int* __restrict__ offsets,
+k_plan(const int* __restrict__ ids, long long m, int E, const int* work, int* __restrict__ offsets,
        int* __restrict__ order, int* __restrict__ pos) {
     constexpr int CHUNK = kPlanThreads * PER;
     extern __shared__ int plan_sm[];
@@ -808,13 +812,13 @@ k_plan(const int* __restrict__ ids, long long m, int E, const int* __restrict__ 
         const int lbase = lcarry + block_scan(own, part, ltot);
         int gbase = lbase;
         if (work) {
-            gbase = gcarry + block_scan(e < E ? work[(size_t)E * B + e] : 0, part, gtot);
+            gbase = gcarry + block_scan(e < E ? waited_for(work + (size_t)E * B + e) : 0, part, gtot);
             gcarry += gtot;
         }
         lcarry += ltot;
         if (e < E) {
             local[e] = lbase;
-            first[e] = gbase + (work ? work[(size_t)e * B + blockIdx.x] : 0);
+            first[e] = gbase + (work ? waited_for(work + (size_t)e * B + blockIdx.x) : 0);
             if (blockIdx.x == 0) offsets[e] = gbase;
         }
     }
@@ -862,7 +866,7 @@ k_plan_count(const int* __restrict__ ids, long long m, int E, int* __restrict__ 
 
 /* One warp an expert: its counts over the blocks become their exclusive prefix,
  * its total goes behind them. */
-__global__ void k_plan_scan(int* __restrict__ work, int E, int B) {
+__global__ void k_plan_scan(int* work, int E, int B) {
     const int lane = threadIdx.x & 31, e = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
     next_launch_may_start();
     wait_for_last_launch();
@@ -870,7 +874,7 @@ __global__ void k_plan_scan(int* __restrict__ work, int E, int B) {
     int* row = work + (size_t)e * B;
     int run = 0;
     for (int b0 = 0; b0 < B; b0 += 32) {
-        const int v = b0 + lane < B ? row[b0 + lane] : 0;
+        const int v = b0 + lane < B ? waited_for(row + b0 + lane) : 0;
         int incl = v;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {

@@ -770,3 +770,35 @@ def test_plans_of_two_threads():
         for p in got:
             for a, b in zip((p.offsets, p.order, p.pos), w):
                 assert np.array_equal(a.cpu().numpy(), b)
+
+
+def test_plans_of_many_blocks_captured_and_replayed():
+    """Two plans of several blocks in one graph with one scratch, replayed on other ids."""
+    experts, n, top_k = 160, 20000, 2
+    ids = [random_ids(i, n, top_k, experts, 0.1, 1.0) for i in range(2)]
+    need = int(M.lib().mpkExpertPlanBytes(n, top_k, experts))
+    assert need > 0
+    work = torch.full((need // 4,), -1, dtype=torch.int32, device="cuda")
+    outs = [[torch.empty(c, dtype=torch.int32, device="cuda") for c in (experts + 1, n * top_k, n * top_k)] for _ in ids]
+
+    def both():
+        stream = torch.cuda.current_stream().cuda_stream
+        for i, o in zip(ids, outs):
+            assert M.lib().mpkExpertPlan(stream, i.data_ptr(), n, top_k, experts, *(t.data_ptr() for t in o),
+                                         work.data_ptr(), need) == M.MPK_OK
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        both()
+    for seed in range(10, 16):
+        for j, i in enumerate(ids):
+            i.copy_(random_ids(seed + 100 * j, n, top_k, experts, 0.1, 1.0))
+        graph.replay()
+        for i, o in zip(ids, outs):
+            for a, b in zip(o, R.plan(i.cpu().numpy(), experts)):
+                assert np.array_equal(a.cpu().numpy(), b.reshape(-1))
