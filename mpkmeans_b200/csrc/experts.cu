@@ -208,14 +208,17 @@ __device__ __forceinline__ uint4 eight(const T* row, int c, int k) {
 
 /* R rows of one expert (from sorted row r, there of them real) times kFewF of its
  * outputs from f: lane l takes elements 8 l ... of every 256.  Rows and outputs
- * that do not exist repeat one that does, so that no load waits on a branch. */
+ * that do not exist repeat one that does, so that no load waits on a branch; a row
+ * that the plan names no token for reads token 0 and is set to zero at the end. */
 template <typename T, int R>
 __device__ __forceinline__ void few_rows(const ExpertArgs& a, const T* we, int f, int r, int there, int lane) {
     const T* x[R];
     const T* w[kFewF];
+    bool named = true;                       /* the row of this lane's output, lane % R */
 #pragma unroll
     for (int i = 0; i < R; ++i) {
         const long long q = x_row(a, r + min(i, there - 1));
+        if (lane % R == i) named = q >= 0;
         x[i] = static_cast<const T*>(a.x) + max(q, 0LL) * a.ldx;
     }
 #pragma unroll
@@ -269,7 +272,7 @@ __device__ __forceinline__ void few_rows(const ExpertArgs& a, const T* we, int f
         }
     const int j = lane / R, i = lane % R;
     if (j < kFewF && i < there && f + j < a.width)
-        static_cast<T*>(a.out)[(long long)(r + i) * a.ldo + f + j] = from_f<T>(mine);
+        static_cast<T*>(a.out)[(long long)(r + i) * a.ldo + f + j] = from_f<T>(named ? mine : 0.f);
 }
 
 /* FWD for a handful of rows: bound by reading the chosen experts' matrices once,
@@ -325,23 +328,27 @@ cudaError_t launch_few(const ExpertArgs& a, cudaStream_t s) {
 
 constexpr int kCopyThreads = 256;
 
-/* out[r] = x[order[r] / top_k] for the sorted rows there are, V elements a copy: a
- * warp a row, eight copies in flight a lane.  Bound by memory: 32768 rows of 4096
+/* out[r] = x[order[r] / top_k] for the *rows sorted rows there are (zeros where the
+ * entry names no row), V elements a copy: a warp a row, eight copies in flight a lane.  Bound by memory: 32768 rows of 4096
  * from 8192 tokens take 61 us, 5.5 TB/s. */
 template <int V>
 __global__ void __launch_bounds__(kCopyThreads)
-k_sort_rows(const uint16_t* __restrict__ x, long long ldx, const int* __restrict__ order, int top_k, int m, int k,
-            uint16_t* __restrict__ out, long long ldo) {
+k_sort_rows(const uint16_t* __restrict__ x, long long ldx, const int* __restrict__ order,
+            const int* __restrict__ rows, int top_k, int m, int k, uint16_t* __restrict__ out, long long ldo) {
     using W = typename std::conditional<V == 8, uint4, uint16_t>::type;
     const int lane = threadIdx.x & 31;
     const long long warps = (long long)gridDim.x * (kCopyThreads / 32);
     const int pieces = (k + V - 1) / V;
     for (long long r = (long long)blockIdx.x * (kCopyThreads / 32) + (threadIdx.x >> 5); r < m; r += warps) {
         const int entry = order[r];
-        if ((unsigned)entry >= (unsigned)m) continue;          /* behind the last routed row */
-        const W* src = reinterpret_cast<const W*>(x + (long long)(entry / top_k) * ldx);
         W* dst = reinterpret_cast<W*>(out + r * ldo);
         int c = lane;
+        if ((unsigned)entry >= (unsigned)m) {
+            if (r < *rows)                                     /* not behind the last routed row */
+                for (; c < pieces; c += 32) dst[c] = W{};
+            continue;
+        }
+        const W* src = reinterpret_cast<const W*>(x + (long long)(entry / top_k) * ldx);
         for (; c + 7 * 32 < pieces; c += 8 * 32) {
             W v[8];
 #pragma unroll
@@ -551,9 +558,11 @@ mpkStatus run_product(ExpertArgs& a, void* work, cudaStream_t s) {
         uint16_t* out = static_cast<uint16_t*>(work);
         const long long xrows = a.m / a.top_k;
         if (a.k % 8 == 0 && aligned16(x, xrows > 1 ? a.ldx : 8, 2))
-            k_sort_rows<8><<<grid, kCopyThreads, 0, s>>>(x, a.ldx, a.order, a.top_k, (int)a.m, a.k, out, sorted.ldx);
+            k_sort_rows<8><<<grid, kCopyThreads, 0, s>>>(x, a.ldx, a.order, a.offsets + a.experts, a.top_k, (int)a.m,
+                                                           a.k, out, sorted.ldx);
         else
-            k_sort_rows<1><<<grid, kCopyThreads, 0, s>>>(x, a.ldx, a.order, a.top_k, (int)a.m, a.k, out, sorted.ldx);
+            k_sort_rows<1><<<grid, kCopyThreads, 0, s>>>(x, a.ldx, a.order, a.offsets + a.experts, a.top_k, (int)a.m,
+                                                           a.k, out, sorted.ldx);
         if (cudaGetLastError() != cudaSuccess) return MPK_ERR_CUDA;
     }
     return launch_experts_tc(sorted, s) == cudaSuccess ? MPK_OK : MPK_ERR_CUDA;

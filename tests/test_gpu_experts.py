@@ -802,3 +802,49 @@ def test_plans_of_many_blocks_captured_and_replayed():
         for i, o in zip(ids, outs):
             for a, b in zip(o, R.plan(i.cpu().numpy(), experts)):
                 assert np.array_equal(a.cpu().numpy(), b.reshape(-1))
+
+
+@pytest.mark.parametrize("pad", [0, 3])
+@pytest.mark.parametrize("n,top_k,experts,k,width", [(1, 1, 1, 64, 72), (4, 2, 4, 72, 40), (8, 2, 1, 520, 64), (40, 2, 20, 136, 64),
+                                                     (200, 2, 3, 136, 264), (300, 2, 20, 72, 64), (30, 2, 3, 37, 33)])
+def test_products_of_entries_that_name_no_row(n, top_k, experts, k, width, pad):
+    """Entries outside the rows inside an expert's segment count as rows of zeros, whichever kernel runs and whatever
+    the scratch held; the token that no entry names is not read."""
+    dtype = torch.bfloat16
+    plan = M.expert_plan(random_ids(n, n, top_k, experts), experts)
+    m = n * top_k
+    order = plan.order.clone()
+    none = torch.tensor([-1, m, 2 ** 31 - 1, -2 ** 31], dtype=torch.int32, device="cuda")
+    bad = order < top_k                                          # those of token 0
+    order[bad] = none[torch.arange(int(bad.sum()), device="cuda") % 4]
+    x = torch.full((n, k + pad), float("nan"), dtype=dtype, device="cuda")[:, :k]
+    x[1:] = normal(1, n - 1, k, dtype=dtype)
+    w = normal(2, experts, width, k, dtype=dtype, scale=k ** -0.5)
+    g = normal(3, m, width, dtype=dtype)
+    off = plan.offsets.cpu().numpy()
+    clean = f64(x)
+    clean[0] = 0
+    xs = R.gathered(clean, np.where(bad.cpu().numpy(), -1, order.cpu().numpy()), top_k)
+    lib, stream = M.lib(), torch.cuda.current_stream().cuda_stream
+    ldx = x.stride(0)
+
+    def scratch(grad_w):
+        need = int(lib.mpkExpertGemmBytes(grad_w, m, experts, k))
+        work = torch.full((need // 2 + 8,), float("nan"), dtype=dtype, device="cuda")
+        return work, work.data_ptr(), need
+
+    y = torch.empty(m, width, dtype=dtype, device="cuda")
+    work, address, need = scratch(0)
+    assert lib.mpkExpertGemm(stream, 2, x.data_ptr(), ldx, w.data_ptr(), k, width * k, plan.offsets.data_ptr(),
+                             order.data_ptr(), top_k, m, experts, width, k, y.data_ptr(), width, address, need) == M.MPK_OK
+    want, mag = R.gemm(xs, f64(w), off), R.gemm(np.abs(xs), np.abs(f64(w)), off)
+    assert np.all(np.abs(f64(y) - want) <= product_tolerance(want, mag, k, dtype))
+    assert torch.all(y[bad] == 0)
+    dw = torch.empty(experts, width, k, dtype=dtype, device="cuda")
+    work, address, need = scratch(1)
+    assert lib.mpkExpertGemmGradW(stream, 2, g.data_ptr(), width, x.data_ptr(), ldx, plan.offsets.data_ptr(),
+                                  order.data_ptr(), top_k, m, experts, width, k, dw.data_ptr(), k, width * k, address,
+                                  need) == M.MPK_OK
+    want, mag = R.gemm_grad_w(f64(g), xs, off), R.gemm_grad_w(np.abs(f64(g)), np.abs(xs), off)
+    most = int((off[1:] - off[:-1]).max())
+    assert np.all(np.abs(f64(dw) - want) <= product_tolerance(want, mag, most, dtype))
