@@ -304,11 +304,12 @@ __device__ __forceinline__ float rcp_fast(float x) {
 constexpr float kLog2e = 1.44269504f;
 
 /* A chosen score up to a factor that the row's slots share, m being the largest
- * chosen logit: e^(x - m) for softmax, and for sigmoids that are all below e^-60,
- * where sigmoid(x) = e^x to the last bit.  As in FP64, a sigmoid below -745 is 0. */
+ * chosen logit: e^(x - m) for softmax, and e^(x - m) / (1 + e^x) for sigmoids that
+ * are all below 1/2, whose ratios FP32 then holds wherever their own values would
+ * underflow.  As in FP64, a sigmoid below -745 is 0. */
 __device__ __forceinline__ float chosen_score(float x, float m, bool softmax) {
     if (softmax) return expf(x - m);
-    if (m < -60.f) return x < -745.f ? 0.f : expf(x - m);
+    if (m < 0.f) return x < -745.f ? 0.f : __fdividef(expf(x - m), 1.f + expf(x));
     return __fdividef(1.f, 1.f + expf(-x));
 }
 

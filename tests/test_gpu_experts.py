@@ -848,3 +848,22 @@ def test_products_of_entries_that_name_no_row(n, top_k, experts, k, width, pad):
     want, mag = R.gemm_grad_w(f64(g), xs, off), R.gemm_grad_w(np.abs(f64(g)), np.abs(xs), off)
     most = int((off[1:] - off[:-1]).max())
     assert np.all(np.abs(f64(dw) - want) <= product_tolerance(want, mag, most, dtype))
+
+
+def test_route_far_sigmoids_keep_their_ratios():
+    """Chosen sigmoids below the FP32 range beside one that is not: e^x of the lower, over the sum."""
+    x = torch.full((5, 8), -300.0, device="cuda")
+    for t, (a, b, c) in enumerate([(-50, -95.5, -110), (-59.5, -88, -104), (-30, -87.5, -90), (-0.5, -70, -85), (0.5, -40, -80)]):
+        x[t, 2], x[t, 5], x[t, 7] = a, b, c
+    for k in (2, 3):
+        check_route(x, k, score="sigmoid")
+        check_route(x, k, score="sigmoid", bias=torch.linspace(0, 1, 8, device="cuda").square()[[0, 1, 7, 2, 3, 6, 4, 5]].contiguous())
+    ids, _ = M.route(x, 3, score="sigmoid")
+    for slot in (1, 2):                                        # the gradient of one small weight: w (1 - s) (1 - w) there
+        g = torch.zeros(5, 3, device="cuda")
+        g[:, slot] = 1.0
+        want = R.route_grad(f64(g), f64(x), ids.cpu().numpy(), score="sigmoid")
+        got = f64(M.route_grad(g, x, ids, score="sigmoid"))
+        at = np.arange(5), ids[:, slot].cpu().numpy()
+        # the weight as in weights_close with logits of up to 300, and three factors
+        assert np.all(np.abs(got - want)[at] <= 900 * U32 * np.abs(want[at]) + 1e-37)
