@@ -77,6 +77,7 @@ constexpr int BOX = 64 * 64 * 2;                 /* one 64 x 64 MN-major box */
 constexpr int kSmemMax = 232448;
 constexpr int kMisc = 1024 + 8 * (MPK_MAX_EXPERTS + 1);
 constexpr int kInfo = 4;                         /* tiles between the producer and the epilogue */
+constexpr int kAsk = 4;                          /* answers between asking for a tile and CTA 1's having read it */
 constexpr int kMostTiles = 1 << 29;              /* more than any plan's; offsets that are none stay below it */
 constexpr int kGroup = 8;                        /* row tiles that sweep the f tiles together */
 
@@ -113,11 +114,10 @@ static_assert(sizeof(Tile) % 16 == 0, "moved in 16-byte words");
 
 template <int STAGES>
 struct EMisc {
-    uint4 next[2];              /* answers to ask_next (CTA 0) */
-    int passed[2];              /* the same as CTA 0 passes them to CTA 1 */
-    int pad[2];
+    uint4 next[kAsk];              /* answers to ask_next (CTA 0) */
+    int passed[kAsk];           /* the same as CTA 0 passes them to CTA 1 */
     Tile info[kInfo];           /* the tiles the producer has started */
-    uint64_t full[STAGES], empty[STAGES], t_full[2], t_empty[2], s_full[2], s_empty[2], i_full[kInfo], i_empty[kInfo], fin;
+    uint64_t full[STAGES], empty[STAGES], t_full[2], t_empty[2], s_full[kAsk], s_empty[kAsk], i_full[kInfo], i_empty[kInfo], fin;
     uint32_t tmem_slot;
     int abort_flag;
 };
@@ -165,6 +165,21 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volati
     int ok = 0;
     if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort_flag, &g_experts_status) ? 1 : 0;
     return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+
+/* Arrival on, and wait for, a barrier by which one CTA of a pair tells the other that it may write, or has written,
+ * a word of shared memory: release and acquire at the cluster's scope. */
+__device__ __forceinline__ void arrive_released(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" :: "r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ bool wait_acquired(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+    if (!mbar_wait(bar, parity, abort_flag, &g_experts_status)) return false;
+    uint32_t ok;                                 /* the phase is complete: true at once */
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return ok != 0;
 }
 
 __device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity) {
@@ -297,9 +312,10 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
         const int arrivals = gathers ? 2 : 1;
         for (int i = 0; i < STAGES; ++i) { mbar_init(&ms.full[i], arrivals); mbar_init(&ms.empty[i], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&ms.t_full[i], 1); mbar_init(&ms.t_empty[i], (PAIR ? 2 : 1) * kEpiWarps); }
-        /* answers are read by the producers, tiles by this CTA's MMA issuer, epilogue and gather warps */
-        for (int i = 0; i < 2; ++i) { mbar_init(&ms.s_full[i], 1); mbar_init(&ms.s_empty[i], PAIR ? 2 : 1); }
-        const int readers = (rank == 0 ? 1 : 0) + kEpiWarps + (gathers ? kGatherWarps : 0);
+        /* answers are read by the producers, tiles by this CTA's MMA issuer (in CTA 1 the warp that would be it),
+         * epilogue and gather warps */
+        for (int i = 0; i < kAsk; ++i) { mbar_init(&ms.s_full[i], 1); mbar_init(&ms.s_empty[i], PAIR ? 2 : 1); }
+        const int readers = 1 + kEpiWarps + (gathers ? kGatherWarps : 0);
         for (int i = 0; i < kInfo; ++i) { mbar_init(&ms.i_full[i], 1); mbar_init(&ms.i_empty[i], readers); }
         mbar_init(&ms.fin, 1);
         ms.abort_flag = 0;
@@ -368,8 +384,10 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
         while (ok) {
             /* The next index is asked for as this tile starts, no earlier: once given it is this cluster's. */
             if (lane == 0 && rank == 0 && u >= 0) {
-                const int sl = asked & 1;
-                ok = mbar_wait(&ms.s_empty[sl], ((uint32_t)(asked >> 1) & 1u) ^ 1u, abort_flag, &g_experts_status);
+                const int sl = asked % kAsk;
+                const uint32_t parity = ((uint32_t)(asked / kAsk) & 1u) ^ 1u;
+                ok = PAIR ? wait_acquired(&ms.s_empty[sl], parity, abort_flag)
+                          : mbar_wait(&ms.s_empty[sl], parity, abort_flag, &g_experts_status);
                 if (ok) {
                     mbar_expect_tx(&ms.s_full[sl], 16);
                     ask_next(&ms.next[sl], &ms.s_full[sl]);
@@ -455,14 +473,15 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
             }
             if (!ok) break;
             /* the answer to this tile's question */
-            const int sl = (asked - 1) & 1;
+            const int sl = (asked - 1) % kAsk;
             int x = -1, got = 0;
             if (lane == 0) {
                 if (rank == 1) mbar_expect_tx(&ms.s_full[sl], 4);
-                got = mbar_wait(&ms.s_full[sl], (uint32_t)((asked - 1) >> 1) & 1u, abort_flag, &g_experts_status) ? 1 : 0;
+                const uint32_t parity = (uint32_t)((asked - 1) / kAsk) & 1u;
+                if (rank == 1) got = wait_acquired(&ms.s_full[sl], parity, abort_flag) ? 1 : 0;
+                else got = mbar_wait(&ms.s_full[sl], parity, abort_flag, &g_experts_status) ? 1 : 0;
                 if (got && rank == 1) {
-                    x = *const_cast<volatile int*>(&ms.passed[sl]);
-                    mbar_arrive_cluster(peer_addr(&ms.s_empty[sl], 0));
+                    x = *const_cast<volatile int*>(&ms.passed[sl]);     /* warp 1 says so to CTA 0 */
                 } else if (got) {
                     x = read_next(&ms.next[sl]);
                     fence_async_proxy();
@@ -476,7 +495,7 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
         }
         if (!ok && lane == 0) {
             /* let what is in flight land before the CTA exits */
-            if (asked > 0 && rank == 0) drain_wait(&ms.s_full[(asked - 1) & 1], (uint32_t)((asked - 1) >> 1) & 1u);
+            if (asked > 0 && rank == 0) drain_wait(&ms.s_full[(asked - 1) % kAsk], (uint32_t)((asked - 1) / kAsk) & 1u);
             if (!PAIR) {
 #pragma unroll
                 for (int i = 0; i < STAGES; ++i)
@@ -532,6 +551,19 @@ k_experts_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
             if (PAIR) umma_commit_pair(peer_addr(&ms.fin, 0));
             else umma_commit(&ms.fin);
             drain_wait(&ms.fin, 0);
+        }
+        if (PAIR && lane == 0 && rank == 1) {
+            /* CTA 1's MMA issuer has no MMAs: it tells CTA 0 that a passed index was read, once the producer has
+             * passed on that tile.  (The release at the cluster's scope waits for the SM's stores: in the producer
+             * it cost the gradient of 64 x 1024 x 2048 weights 4 %.) */
+            for (int n = 0;; ++n) {
+                const int sl = n % kInfo;
+                if (!mbar_wait(&ms.i_full[sl], (uint32_t)(n / kInfo) & 1u, abort_flag, &g_experts_status)) break;
+                const int u = ms.info[sl].u;
+                mbar_arrive(&ms.i_empty[sl]);
+                if (n > 0) arrive_released(peer_addr(&ms.s_empty[(n - 1) % kAsk], 0));
+                if (u < 0) break;
+            }
         }
     } else if (warp >= 2 + kEpiWarps) {
         /* ----------------------------------------------------- gather --- */

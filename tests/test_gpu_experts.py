@@ -867,3 +867,21 @@ def test_route_far_sigmoids_keep_their_ratios():
         at = np.arange(5), ids[:, slot].cpu().numpy()
         # the weight as in weights_close with logits of up to 300, and three factors
         assert np.all(np.abs(got - want)[at] <= 900 * U32 * np.abs(want[at]) + 1e-37)
+
+
+@pytest.mark.parametrize("experts,n,top_k,k,width", [(64, 1500, 2, 512, 1024), (8, 3000, 4, 1024, 512)])
+def test_products_of_many_tiles_a_cluster(experts, n, top_k, k, width):
+    """Every cluster takes over more tiles than it has places for their indices: right, and the same bit for bit in
+    every call, whichever cluster took which."""
+    dtype = torch.bfloat16
+    s = setup_products(5, n, top_k, experts, k, width, dtype, True, 0.05, 1)
+    check_products(*s, True, dtype)
+    plan, _, x, _, w, g = s
+
+    def run():
+        return M.expert_gemm(x, w, plan), M.expert_gemm_grad_x(g, w, plan), M.expert_gemm_grad_w(g, x, plan)
+
+    first = run()
+    for _ in range(20):
+        for a, b in zip(first, run()):
+            assert torch.equal(a, b)
