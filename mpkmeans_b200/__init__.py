@@ -595,11 +595,16 @@ def _array(name: str, t, dtype, *shape: int) -> int:
 
 def _run(fn_name: str, tensors: tuple, *args) -> None:
     """Call fn_name(stream, *args) on the tensors' device (all on one) and torch's
-    current stream there, the stream that outputs and scratch are allocated on."""
+    current stream there, the stream that outputs and scratch are allocated on.  The
+    calls record nothing for autograd: a tensor that needs a gradient is refused while
+    torch records."""
     device = tensors[0].get_device()
     for t in tensors:
         if t.get_device() != device:
             raise ValueError(f"{fn_name}: tensors on {tensors[0].device} and {t.device}")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{fn_name}: a tensor needs a gradient, which this call does not record; "
+                             "call it under torch.no_grad() (or in a torch.autograd.Function)")
     stream = torch._C._cuda_getCurrentRawStream(device)
     fn = getattr(_lib or lib(), fn_name)
     if device == torch._C._cuda_getDevice():

@@ -160,3 +160,10 @@ def test_reference_gradient_against_differences(score, renormalize):
             down[t, j] -= h
             # central differences: error h^2 / 6 times a third derivative of order one
             assert abs((loss(up) - loss(down)) / (2 * h) - want[t, j]) < 1e-8
+
+
+def test_mirror_refuses_to_lose_a_gradient():
+    """While torch records, a tensor that needs a gradient is refused before anything is called."""
+    M._types()
+    with pytest.raises(ValueError, match="no_grad"):
+        M._run("mpkRoute", (torch.zeros(2), torch.zeros(2, requires_grad=True)))

@@ -885,3 +885,25 @@ def test_products_of_many_tiles_a_cluster(experts, n, top_k, k, width):
     for _ in range(20):
         for a, b in zip(first, run()):
             assert torch.equal(a, b)
+
+
+def test_calls_refuse_to_lose_a_gradient():
+    """The calls record no gradient: an input that needs one is refused while torch records, and taken otherwise."""
+    x = normal(1, 6, 8).requires_grad_(True)
+    with pytest.raises(ValueError, match="no_grad"):
+        M.route(x, 2)
+    with torch.no_grad():
+        ids, weights = M.route(x, 2)
+    plan = M.expert_plan(ids, 8)
+    half = normal(2, 6, 16, dtype=torch.float16)
+    w = torch.nn.Parameter(normal(3, 8, 24, 16, dtype=torch.float16))
+    y = normal(4, 12, 16).requires_grad_(True)
+    for call in (lambda: M.expert_gemm(half, w, plan), lambda: M.expert_combine(y, plan, weights),
+                 lambda: M.expert_combine(y.detach(), plan, weights.clone().requires_grad_(True)),
+                 lambda: M.expert_gemm_grad_x(normal(5, 12, 24, dtype=torch.float16), w, plan),
+                 lambda: M.route_grad(weights, x, ids)):
+        with pytest.raises(ValueError, match="no_grad"):
+            call()
+        with torch.no_grad():
+            call()
+    assert torch.equal(M.expert_gemm(half, w.detach(), plan), M.expert_gemm(half, w.data, plan))
