@@ -907,3 +907,26 @@ def test_calls_refuse_to_lose_a_gradient():
         with torch.no_grad():
             call()
     assert torch.equal(M.expert_gemm(half, w.detach(), plan), M.expert_gemm(half, w.data, plan))
+
+
+@pytest.mark.parametrize("gather", [True, False])
+@pytest.mark.parametrize("n,top_k,experts,k,width", [(2, 2, 5, 37, 19), (40, 2, 10, 101, 67), (200, 2, 20, 75, 133), (300, 2, 3, 197, 301)])
+def test_products_odd_widths_in_aligned_rows(n, top_k, experts, k, width, gather):
+    """Rows of any length that start on 16-byte boundaries: the tensor-core and few-rows kernels, whose last pieces of a
+    row hold what lies behind it (NaN here)."""
+    dtype = torch.float16
+    plan, off, x, xs, w, g = setup_products(6, n, top_k, experts, k, width, dtype, gather, 0.1, 0.5)
+
+    def aligned(t, value=float("nan")):
+        big = torch.full((*t.shape[:-1], (t.shape[-1] + 7) // 8 * 8 + 8), value, dtype=dtype, device="cuda")
+        view = big[..., :t.shape[-1]]
+        view.copy_(t)
+        return view
+
+    outs = [aligned(torch.zeros(shape, dtype=dtype, device="cuda"), 7.0) for shape in
+            ((n * top_k, width), (n * top_k, k), (experts, width, k))]
+    check_products(plan, off, aligned(x), xs, aligned(w), aligned(g), gather, dtype, outs)
+    for o in outs:
+        whole = o._base
+        o.fill_(7.0)
+        assert torch.all(whole == 7.0)
