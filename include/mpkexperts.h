@@ -12,8 +12,9 @@
  * t * top_k + s is slot s of token t.  All pointers named dX are device pointers
  * of the current device, owned by the caller; work runs on `stream`, is only
  * enqueued (no synchronisation, no allocation, no state kept between calls) and
- * can be captured into a CUDA graph (after one call outside a capture, which
- * loads the kernels).  Outputs and scratch overlap nothing else.  Leading dimensions (ld...) count elements.
+ * can be captured into a CUDA graph (after one call of the same sizes outside a
+ * capture, which loads the kernels).  Outputs and scratch overlap nothing else.
+ * Leading dimensions (ld...) count elements.
  * A call with n = 0 (or m = 0) writes only what its comment says.  Bad arguments
  * return MPK_ERR_INVALID before anything is enqueued.  The tensor-core products'
  * waits are bounded (4 s): one that runs out ends the kernel with its output
@@ -89,10 +90,12 @@ void mpkRouteParamsInit(mpkRouteParams* p);
  *   dWeights n x top_k FP32: scale * s_i, or scale * s_i / sum of the chosen s.
  * An expert whose logit or bias is -inf is masked: it is never chosen.  Slots
  * that no expert is left for hold id -1 and weight 0; chosen scores that are all
- * zero (sigmoids of logits below -745) give weights of 0.  The choice is the one that
- * exact arithmetic makes: logits are compared where the order of c is theirs;
- * elsewhere FP32 scores that lie within their error bound of one another
- * are compared again in FP64.  A row with a NaN logit (or +inf, under softmax)
+ * zero (sigmoids of logits below -745) give weights of 0.  Logits are compared
+ * where the order of c is theirs (no bias, groups by their maximum); elsewhere the
+ * choice is the one that c in FP64 makes, values that FP64 rounds to one another
+ * being ties: FP32 scores that lie within their error bound of one another are
+ * compared again in FP64 (with a bias and top_k = 32 all rows are, which takes three
+ * times as long as top_k = 31).  A row with a NaN logit (or +inf, under softmax)
  * gets NaN weights and ids inside [-1, experts) that mean nothing. */
 mpkStatus mpkRoute(cudaStream_t stream, const mpkRouteParams* p, const void* dLogits, int type, long long n,
                    long long ld, const float* dBias, int* dIds, float* dWeights);
@@ -123,7 +126,7 @@ mpkStatus mpkExpertPlan(cudaStream_t stream, const int* dIds, long long n, int t
  *   mpkExpertGemmGradW: dGW_e = sum_r GY[r] X[r]^T, dGW experts x (width x k)
  * for the rows r of every expert e.  X[r] is row r of dX when dOrder is NULL
  * (dX has m rows) and row dOrder[r] / top_k of dX (n = m / top_k token rows)
- * otherwise.  Rows of dY and dGX that no expert owns ([dOffsets[experts], m)) are
+ * otherwise, zeros where dOrder[r] is none of the m entries.  Rows of dY and dGX that no expert owns ([dOffsets[experts], m)) are
  * set to zero; an expert without rows gets a zero gradient.  Nothing past row m
  * and nothing between a row's end and its stride is written.
  * With dOrder, dWork is scratch of mpkExpertGemmBytes(0 for Gemm, 1 for GradW, ...)
@@ -131,7 +134,9 @@ mpkStatus mpkExpertPlan(cudaStream_t stream, const int* dIds, long long n, int t
  * experts have few rows and the product gathers them itself); without, it is not
  * looked at.
  * width and k in 1 .. 2^20; any alignment of the element type: rows that start
- * on 16-byte boundaries (addresses and strides) run on the tensor cores. */
+ * on 16-byte boundaries (addresses and strides) run on the tensor cores, and so do
+ * gathered ones that are copied first; with others the product takes ten times as
+ * long or more (15 to 19 TFLOP/s). */
 size_t mpkExpertGemmBytes(int grad_w, long long m, int experts, int k);
 mpkStatus mpkExpertGemm(cudaStream_t stream, int type, const void* dX, long long ldx, const void* dW, long long ldw,
                         long long strideW, const int* dOffsets, const int* dOrder, int top_k, long long m,

@@ -44,7 +44,7 @@ __device__ __forceinline__ long long x_row(const ExpertArgs& a, long long r) {
     return (unsigned)entry < (unsigned long long)a.m ? entry / a.top_k : -1;
 }
 
-/* The kernel of odd layouts, about 19 TFLOP/s: its loads are single elements.
+/* The kernel of odd layouts, 15 to 19 TFLOP/s: its loads are single elements.
  * One 64 x 64 tile of one expert's output a block, operands staged in shared
  * memory 16 deep, 4 x 4 sums a thread.  FWD and GRADX: blockIdx.x counts the row
  * tiles of all experts (their number T is known on the device only; with D rows
@@ -533,7 +533,10 @@ size_t copy_bytes(int mode, long long m, int experts, int k) {
 /* Up to so many rows the product is a pass over the chosen matrices by plain loads
  * (k_experts_few).  Measured against the 32-row tiles, 64 experts of 1024 x 2048:
  * 16 rows 12 : 20 us, 64 rows 28 : 33 us, 128 rows 45 : 44 us; 8 experts of 1536 x
- * 2048: 16 rows 13 : 18 us, 32 rows 21 : 18 us. */
+ * 2048: 16 rows 13 : 18 us, 32 rows 21 : 18 us.  These are even loads.  All rows on
+ * one expert walk its matrix once for every four: 64 rows on one of 64 experts of
+ * 1024 x 2048 take 74 us in a whole call where 66, on tiles, take 19; the counts are
+ * on the device, so the choice cannot see it. */
 long long few_limit(int experts) { return experts < 16 ? 16 : experts; }
 
 /* With a sorted copy the product sees plain sorted rows; the tiled kernel gathers

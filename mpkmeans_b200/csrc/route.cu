@@ -10,7 +10,9 @@
  * and ranked against each other.  (Taking the maximum top_k times, rescanning the
  * registers of the lane that held it, was a third of 1800 instructions a row.)
  * Bound by instruction issue: 32768 x 256 FP32 takes 24 us with softmax, 41 to 47 with
- * sigmoid, bias and groups.
+ * sigmoid, bias and groups.  Equal biases with BF16 logits, whose ties send many rows
+ * to slow_choice, 37 to 39 us without groups and up to 66 with; 1024 experts with a
+ * bias 184 to 242 us.
  *
  * The choice is exact, as the assignment's is: without a bias, and with groups
  * scored by their maximum, the order of c is the order of l and the keys are the
@@ -397,7 +399,8 @@ __device__ __forceinline__ void top_keys(unsigned (&key)[VPL], int takes, uint2*
 
 /* Blocks an SM that the registers are cut to, so that slow_choice, which is called
  * from the main path but rarely runs, does not set their number.  (256 experts with
- * a bias: 6, 8, 10 and 12 blocks took 40, 44, 41 and 46 us; without: no difference.) */
+ * a bias: 6, 8, 10 and 12 blocks took 40, 44, 41 and 46 us; without: no difference.
+ * Other widths were not tried with other numbers.) */
 constexpr int route_blocks(int vpl, bool by_score) { return vpl <= 4 ? 12 : vpl > 8 ? 1 : by_score ? 6 : 10; }
 
 /* BY_SCORE: keys are choice values c (a bias, or groups by their two best), else
@@ -595,9 +598,9 @@ k_route(const T* __restrict__ logits, long long n, long long ld, const float* __
  * The first three need the chosen logits only: k_route_grad_slots gives a token
  * 2^log_k lanes, one a slot, and a warp 32 / 2^log_k tokens, whose rows it fills with
  * zeros before the slots' terms go in (ordered by __syncwarp; slots of one expert
- * all write their sum).  (A warp a token took 263 instructions a row and 14 us for
- * 30001 x 60.)  The last form reads and writes whole rows: k_route_grad_whole, one
- * warp a token. */
+ * all write their sum): 4 to 5 us on the device for 30001 x 60.  (A warp a token took
+ * 263 instructions a row and 14 us.)  The last form reads and writes whole rows: k_route_grad_whole, one
+ * warp a token (22.7 us for 32768 x 256 FP32, whose 67 MB take 10.3 at least). */
 template <typename T, typename W>
 __global__ void __launch_bounds__(32 * kRouteWarps)
 k_route_grad_slots(const T* __restrict__ logits, long long n, long long ld, RouteShape sh, const int* __restrict__ ids,
